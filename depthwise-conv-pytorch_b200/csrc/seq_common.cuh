@@ -1,0 +1,197 @@
+// Shared pieces of the sequence operators (causal depthwise conv1d, gated linear recurrence, layer
+// norm): rows of channels that lie side by side, loaded V channels at a time and worked on in fp32.
+#pragma once
+
+#include "api_checks.cuh"
+#include "common.cuh"
+
+namespace dwb {
+
+// One operand of a sequence operator: element (b, t, c) at data[b * bs + t * rs + c].
+template <typename T> struct SeqIn {
+  const T *p;
+  long long bs, rs;
+  __device__ __forceinline__ const T *row(int b, long long t) const { return p + b * bs + t * rs; }
+};
+
+// One element as fp32.  Plain loads throughout these kernels: many stand behind a bounds or a null
+// check, and the load intrinsics of some types are assembly that the compiler may execute before it.
+template <typename T> __device__ __forceinline__ float read(const T *p) { return Elem<T>::to_acc(*p); }
+
+// V adjacent elements as they lie in memory, moved by one load or store.
+template <int BYTES> struct RawVec;
+template <> struct RawVec<2> { using type = unsigned short; };
+template <> struct RawVec<4> { using type = uint32_t; };
+template <> struct RawVec<8> { using type = uint2; };
+template <> struct RawVec<16> { using type = uint4; };
+
+template <typename T, int V> struct Pack {
+  using Raw = typename RawVec<V * (int)sizeof(T)>::type;
+  static __device__ __forceinline__ Raw load(const T *p) { return *reinterpret_cast<const Raw *>(p); }
+  static __device__ __forceinline__ void store(T *p, const Raw &r) { *reinterpret_cast<Raw *>(p) = r; }
+  static __device__ __forceinline__ Raw zero() {
+    Raw r;
+    memset(&r, 0, sizeof(r));
+    return r;
+  }
+  static __device__ __forceinline__ void unpack(const Raw &r, float (&f)[V]) {
+    if constexpr (sizeof(T) == 4) {
+      memcpy(f, &r, sizeof(r));
+    } else if constexpr (V == 1) {
+      f[0] = Pack16<T>::from_bits(r);
+    } else {
+      uint32_t w[V / 2];
+      memcpy(w, &r, sizeof(r));
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        const float2 q = Pack16<T>::unpack(w[i]);
+        f[2 * i] = q.x;
+        f[2 * i + 1] = q.y;
+      }
+    }
+  }
+  static __device__ __forceinline__ Raw pack(const float (&f)[V]) {
+    Raw r;
+    if constexpr (sizeof(T) == 4) {
+      memcpy(&r, f, sizeof(r));
+    } else if constexpr (V == 1) {
+      r = Pack16<T>::to_bits(f[0]);
+    } else {
+      uint32_t w[V / 2];
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) w[i] = Pack16<T>::pack(f[2 * i], f[2 * i + 1]);
+      memcpy(&r, w, sizeof(r));
+    }
+    return r;
+  }
+};
+
+// ---- packed sequences --------------------------------------------------------------------------
+
+// The list of packed sequences, or (offsets null) one sequence per batch element.
+struct SeqList {
+  int T, C;
+  const int *offsets;  // S + 1 entries, or null
+  int S;               // sequences (with offsets), else the batch size
+};
+
+// Entry j as a row number inside [0, T], whatever the caller wrote there.
+__device__ __forceinline__ int seq_bound(const SeqList &q, int j) {
+  const int v = q.offsets[j];
+  return v < 0 ? 0 : (v > q.T ? q.T : v);
+}
+
+// Where row t lies.
+struct SeqSpan {
+  int seq;      // its sequence, -1 for a row of none
+  int begin;    // first row of the sequence (of the run of rows of none)
+  int next;     // first row behind it that belongs to something else, > t
+};
+
+// Last j with offsets[j] <= t, by bisection; every value read is clamped, so a list that is not
+// ascending gives some sequence, never an access outside the tensors.
+__device__ __forceinline__ SeqSpan seq_locate(const SeqList &q, int t) {
+  int lo = 0, hi = q.S;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (seq_bound(q, mid) <= t) lo = mid;
+    else hi = mid;
+  }
+  const int s = seq_bound(q, lo), e = seq_bound(q, lo + 1);
+  SeqSpan r;
+  if (s <= t && t < e) {
+    r.seq = lo; r.begin = s; r.next = e;
+  } else if (s > t) {  // before the first sequence
+    r.seq = -1; r.begin = 0; r.next = s;
+  } else {  // behind the last one
+    r.seq = -1; r.begin = e <= t ? e : t; r.next = q.T;
+  }
+  return r;
+}
+
+// ---- column sums -------------------------------------------------------------------------------
+
+// Where the sum of one column of a [parts][M] table of fp32 partial sums goes: the first `split`
+// columns to `first`, the rest to `second`; column m = k * C + c of the first part lands at
+// c * K + k (the filter layout), K = 1 keeps the order.
+struct ColumnSumOut {
+  void *first, *second;
+  int dtype;
+  int C, K;             // split = C * K
+  const float *decay;   // non-null: the sum of column c times scale * sigmoid(decay[c])
+  float scale;
+};
+
+constexpr int COLSUM_LANES = 32, COLSUM_WARPS = 8;
+
+__device__ __forceinline__ void store_as(void *p, long long i, float v, int dtype) {
+  if (dtype == DWCONV_B200_F32) static_cast<float *>(p)[i] = v;
+  else if (dtype == DWCONV_B200_F16) static_cast<__half *>(p)[i] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// Every column is added in the same order on every run: warp w takes parts w, w + 8, ...
+static __global__ void __launch_bounds__(COLSUM_LANES *COLSUM_WARPS)
+column_sum_kernel(const float *__restrict__ part, long long parts, int M, ColumnSumOut out) {
+  __shared__ float s[COLSUM_WARPS][COLSUM_LANES];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int m = blockIdx.x * COLSUM_LANES + lane;
+  float acc = 0.f;
+  if (m < M)
+    for (long long p = w; p < parts; p += COLSUM_WARPS) acc += part[p * M + m];
+  s[w][lane] = acc;
+  __syncthreads();
+  if (w != 0 || m >= M) return;
+  float v = 0.f;
+#pragma unroll
+  for (int i = 0; i < COLSUM_WARPS; ++i) v += s[i][lane];
+  const int split = out.C * out.K;
+  if (out.decay != nullptr && m < split) v *= out.scale / (1.f + expf(-out.decay[m]));
+  if (m < split) {
+    const int k = m / out.C, c = m - k * out.C;
+    if (out.first) store_as(out.first, (long long)c * out.K + k, v, out.dtype);
+  } else if (out.second) {
+    store_as(out.second, m - split, v, out.dtype);
+  }
+}
+
+inline void launch_column_sum(const float *part, long long parts, int M, const ColumnSumOut &out,
+                              cudaStream_t st) {
+  column_sum_kernel<<<ceil_div(M, COLSUM_LANES), COLSUM_LANES * COLSUM_WARPS, 0, st>>>(part, parts, M, out);
+}
+
+// ---- host checks -------------------------------------------------------------------------------
+
+inline bool seq_dtype_ok(int dtype) {
+  return dtype == DWCONV_B200_F32 || dtype == DWCONV_B200_F16 || dtype == DWCONV_B200_BF16;
+}
+
+inline int check_sequence(const dwconv_b200_sequence *s) {
+  if (s == nullptr || s->B <= 0 || s->C <= 0 || s->T < 0 || s->S < 0) return DWCONV_B200_BAD_ARGUMENT;
+  if (s->offsets != nullptr && (s->B != 1 || s->S < 1 || !aligned_to(s->offsets, 4)))
+    return DWCONV_B200_BAD_ARGUMENT;
+  // row numbers are 32-bit (with room for a tile behind the last); offsets into tensors 64-bit
+  if (s->T > (1 << 30) || s->C > (1 << 26) || s->B > (1 << 26) || s->S > (1 << 26))
+    return DWCONV_B200_TOO_LARGE;
+  return DWCONV_B200_OK;
+}
+
+inline int check_rows(const dwconv_b200_rows *r, size_t es) {
+  if (r == nullptr || r->data == nullptr) return DWCONV_B200_BAD_ARGUMENT;
+  return aligned_to(r->data, es) ? DWCONV_B200_OK : DWCONV_B200_MISALIGNED;
+}
+
+// Whether rows can be moved `v` elements (v * es bytes) at a time.
+inline bool rows_vector(const dwconv_b200_rows &r, int v, size_t es) {
+  return aligned_to(r.data, v * es) && r.batch_stride % v == 0 && r.row_stride % v == 0;
+}
+
+template <typename T> inline SeqIn<T> seq_in(const dwconv_b200_rows &r) {
+  return SeqIn<T>{static_cast<const T *>(r.data), r.batch_stride, r.row_stride};
+}
+
+inline SeqList seq_list(const dwconv_b200_sequence &s) {
+  return SeqList{s.T, s.C, static_cast<const int *>(s.offsets), s.offsets ? s.S : s.B};
+}
+
+}  // namespace dwb

@@ -19,6 +19,7 @@
 
 #include <string>
 #include <tuple>
+#include <vector>
 
 #include "dwconv_b200.h"
 
@@ -272,6 +273,392 @@ at::Tensor dwconv2d_backward_kernel(at::Tensor input, at::Tensor out_grad, const
   return dkernel;
 }
 
+// ---- sequence operators ----------------------------------------------------------------
+// (no counterpart in the reference; the checks' texts equal those of dwconv_b200/sequence.py, which
+// has the same functions over ctypes)
+
+using OptTensor = c10::optional<at::Tensor>;
+
+const void *ptr(const OptTensor &t) { return t.has_value() ? t->data_ptr() : nullptr; }
+
+int sequence_dtype(const at::Tensor &t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return DWCONV_B200_F32;
+    case at::kHalf: return DWCONV_B200_F16;
+    case at::kBFloat16: return DWCONV_B200_BF16;
+    default:
+      TORCH_CHECK(false, "dwconv_b200: unsupported dtype ", t.dtype(), " (float32, float16, bfloat16)");
+  }
+  return -1;
+}
+
+// channels side by side; any other strides are read as they are
+at::Tensor rows_of(const at::Tensor &t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+
+dwconv_b200_rows rows_arg(const at::Tensor &t) { return {t.data_ptr(), t.stride(0), t.stride(1)}; }
+
+// shape and device of one operand against the input's
+void check_operand(const char *fn, const char *name, const at::Tensor &t, at::IntArrayRef shape, at::ScalarType type,
+                   const at::Tensor &input) {
+  TORCH_CHECK(t.device() == input.device() && t.scalar_type() == type, "dwconv_b200.", fn, ": ", name, " must be ",
+              c10::scalarTypeToTypeMeta(type), " on ", input.device(), ", got ", t.dtype(), " on ", t.device());
+  if (t.sizes() != shape) {
+    std::string want = "(";
+    for (size_t i = 0; i < shape.size(); ++i)
+      want += std::to_string(shape[i]) + (i + 1 < shape.size() ? ", " : shape.size() == 1 ? "," : "");
+    TORCH_CHECK(false, "dwconv_b200.", fn, ": ", name, " must be ", want, "), got ", shape_text(t));
+  }
+}
+
+dwconv_b200_sequence check_sequences(const char *fn, const at::Tensor &input, const OptTensor &offsets) {
+  check_cuda(input, "input");
+  sequence_dtype(input);
+  TORCH_CHECK(input.dim() == 3, "dwconv_b200.", fn, ": expected input [B, T, C], got ", shape_text(input));
+  for (int d = 0; d < 3; ++d)
+    TORCH_CHECK(input.size(d) <= (1ll << 30), "dwconv_b200.", fn, ": input is too large: ", shape_text(input));
+  dwconv_b200_sequence s{(int)input.size(0), (int)input.size(1), (int)input.size(2), nullptr, 0};
+  if (offsets.has_value()) {
+    const at::Tensor &o = *offsets;
+    TORCH_CHECK(o.device() == input.device() && o.scalar_type() == at::kInt && o.dim() == 1 && o.is_contiguous() &&
+                    o.size(0) >= 2,
+                "dwconv_b200.", fn, ": offsets must be a contiguous 1-d int32 tensor of at least 2 row numbers on ",
+                input.device());
+    TORCH_CHECK(s.B == 1, "dwconv_b200.", fn, ": packed sequences (offsets) need a batch of 1, got ", s.B);
+    s.offsets = o.data_ptr();
+    s.S = (int)o.size(0) - 1;
+  }
+  return s;
+}
+
+int64_t state_count(const dwconv_b200_sequence &s) { return s.offsets ? s.S : s.B; }
+bool no_rows(const at::Tensor &input) { return input.numel() == 0; }
+
+at::Tensor state_or_zeros(const OptTensor &state, at::IntArrayRef shape, const at::TensorOptions &options) {
+  return state.has_value() ? state->clone(at::MemoryFormat::Contiguous) : at::zeros(shape, options);
+}
+
+OptTensor contiguous(const OptTensor &t) { return t.has_value() ? OptTensor(t->contiguous()) : OptTensor(); }
+
+struct Conv1d {
+  dwconv_b200_sequence s;
+  int taps;
+  std::vector<int64_t> state;
+};
+
+Conv1d check_conv1d(const char *fn, const at::Tensor &input, const at::Tensor &weight, const OptTensor &bias,
+                    const OptTensor &initial, const OptTensor &offsets) {
+  Conv1d c;
+  c.s = check_sequences(fn, input, offsets);
+  TORCH_CHECK(weight.dim() == 3 && weight.size(0) == c.s.C && weight.size(1) == 1 && weight.size(2) >= 1 &&
+                  weight.size(2) <= DWCONV_B200_MAX_TAPS,
+              "dwconv_b200.", fn, ": weight must be [C, 1, taps] with C = ", c.s.C, " and 1 to ", DWCONV_B200_MAX_TAPS,
+              " taps, got ", shape_text(weight));
+  c.taps = (int)weight.size(2);
+  check_operand(fn, "weight", weight, weight.sizes(), input.scalar_type(), input);
+  if (bias.has_value()) check_operand(fn, "bias", *bias, {c.s.C}, input.scalar_type(), input);
+  c.state = {state_count(c.s), c.taps - 1, c.s.C};
+  if (initial.has_value()) check_operand(fn, "initial_state", *initial, c.state, input.scalar_type(), input);
+  return c;
+}
+
+std::tuple<at::Tensor, OptTensor> conv1d_causal(const at::Tensor &input, const at::Tensor &weight,
+                                                const OptTensor &bias, int64_t act, const OptTensor &initial,
+                                                const OptTensor &offsets, bool want_state) {
+  const char *fn = "depthwise_conv1d_causal";
+  const Conv1d c = check_conv1d(fn, input, weight, bias, initial, offsets);
+  c10::cuda::CUDAGuard guard(input.device());
+  at::Tensor y = at::empty(input.sizes(), input.options(), at::MemoryFormat::Contiguous);
+  OptTensor state;
+  if (no_rows(input)) {
+    if (want_state) state = state_or_zeros(initial, c.state, input.options());
+    return {y, state};
+  }
+  if (want_state) state = at::empty(c.state, input.options());
+  const at::Tensor x = rows_of(input), w = weight.contiguous();
+  const OptTensor b = contiguous(bias), init = contiguous(initial);
+  const dwconv_b200_rows xr = rows_arg(x);
+  check_status(dwconv_b200_conv1d_causal(&xr, w.data_ptr(), ptr(b), ptr(init), y.data_ptr(),
+                                         state.has_value() ? state->data_ptr() : nullptr, sequence_dtype(x), &c.s,
+                                         c.taps, (int)act, stream_of(x)),
+               fn);
+  return {y, state};
+}
+
+// gradients of input, weight, bias, initial state (the last two: as asked)
+std::tuple<at::Tensor, at::Tensor, OptTensor, OptTensor> conv1d_causal_backward(
+    const at::Tensor &input, const at::Tensor &weight, const OptTensor &bias, int64_t act, const OptTensor &initial,
+    const OptTensor &offsets, const OptTensor &grad, const OptTensor &grad_state, bool want_initial) {
+  const char *fn = "depthwise_conv1d_causal backward";
+  const Conv1d c = check_conv1d(fn, input, weight, bias, initial, offsets);
+  c10::cuda::CUDAGuard guard(input.device());
+  if (grad.has_value()) check_operand(fn, "grad_output", *grad, input.sizes(), input.scalar_type(), input);
+  if (grad_state.has_value()) check_operand(fn, "grad_state", *grad_state, c.state, input.scalar_type(), input);
+  OptTensor db, dinit;
+  if (no_rows(input)) {
+    if (bias.has_value()) db = at::zeros(bias->sizes(), input.options());
+    if (want_initial) dinit = state_or_zeros(grad_state, c.state, input.options());
+    return {at::empty(input.sizes(), input.options()), at::zeros(weight.sizes(), input.options()), db, dinit};
+  }
+  at::Tensor dx = at::empty(input.sizes(), input.options(), at::MemoryFormat::Contiguous);
+  at::Tensor dw = at::empty(weight.sizes(), input.options(), at::MemoryFormat::Contiguous);
+  if (bias.has_value()) db = at::empty({c.s.C}, input.options());
+  if (want_initial) dinit = at::empty(c.state, input.options());
+  const at::Tensor x = rows_of(input), w = weight.contiguous();
+  const at::Tensor g = grad.has_value() ? rows_of(*grad) : at::zeros(input.sizes(), input.options());
+  const OptTensor b = contiguous(bias), init = contiguous(initial), gs = contiguous(grad_state);
+  const int code = sequence_dtype(x);
+  const size_t nbytes = dwconv_b200_conv1d_causal_workspace_bytes(code, &c.s, c.taps);
+  TORCH_CHECK(nbytes != 0, "dwconv_b200.", fn, ": invalid geometry");
+  at::Tensor ws = at::empty({(int64_t)nbytes}, input.options().dtype(at::kByte));
+  const dwconv_b200_rows xr = rows_arg(x), gr = rows_arg(g);
+  check_status(dwconv_b200_conv1d_causal_backward(
+                   &xr, w.data_ptr(), ptr(b), ptr(init), &gr, ptr(gs), dx.data_ptr(), dw.data_ptr(),
+                   db.has_value() ? db->data_ptr() : nullptr, dinit.has_value() ? dinit->data_ptr() : nullptr,
+                   ws.data_ptr(), nbytes, code, &c.s, c.taps, (int)act, stream_of(x)),
+               fn);
+  return {dx, dw, db, dinit};
+}
+
+// A state that a step updates in place.
+void check_state(const char *fn, const at::Tensor &state, at::IntArrayRef shape, at::ScalarType type,
+                 const at::Tensor &input) {
+  check_operand(fn, "state", state, shape, type, input);
+  TORCH_CHECK(state.is_contiguous(), "dwconv_b200.", fn, ": state is updated in place and must be contiguous");
+}
+
+// The kernels write through raw pointers: a graph that saved this state must learn of it.
+void note_written(const at::Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+int64_t check_step_input(const char *fn, const at::Tensor &input) {
+  check_cuda(input, "input");
+  sequence_dtype(input);
+  TORCH_CHECK(input.dim() == 2, "dwconv_b200.", fn, ": expected input [B, C], got ", shape_text(input));
+  for (int d = 0; d < 2; ++d)
+    TORCH_CHECK(input.size(d) <= (1ll << 30), "dwconv_b200.", fn, ": input is too large: ", shape_text(input));
+  return input.size(1);
+}
+
+at::Tensor conv1d_causal_step(const at::Tensor &input, const at::Tensor &weight, const at::Tensor &state,
+                              const OptTensor &bias, int64_t act) {
+  const char *fn = "depthwise_conv1d_causal_step";
+  const int64_t C = check_step_input(fn, input), B = input.size(0);
+  TORCH_CHECK(weight.dim() == 3 && weight.size(0) == C && weight.size(1) == 1 && weight.size(2) >= 1 &&
+                  weight.size(2) <= DWCONV_B200_MAX_TAPS,
+              "dwconv_b200.", fn, ": weight must be [C, 1, taps] with C = ", C, " and 1 to ", DWCONV_B200_MAX_TAPS,
+              " taps, got ", shape_text(weight));
+  check_operand(fn, "weight", weight, weight.sizes(), input.scalar_type(), input);
+  if (bias.has_value()) check_operand(fn, "bias", *bias, {C}, input.scalar_type(), input);
+  const int taps = (int)weight.size(2);
+  check_state(fn, state, {B, taps - 1, C}, input.scalar_type(), input);
+  c10::cuda::CUDAGuard guard(input.device());
+  at::Tensor y = at::empty({B, C}, input.options());
+  if (no_rows(input)) return y;
+  note_written(state);
+  const at::Tensor x = rows_of(input), w = weight.contiguous();
+  const OptTensor b = contiguous(bias);
+  check_status(dwconv_b200_conv1d_causal_step(x.data_ptr(), x.stride(0), w.data_ptr(), ptr(b), state.data_ptr(),
+                                              y.data_ptr(), sequence_dtype(x), (int)B, (int)C, taps, (int)act,
+                                              stream_of(x)),
+               fn);
+  return y;
+}
+
+struct Recurrence {
+  dwconv_b200_sequence s;
+  std::vector<int64_t> state;
+};
+
+Recurrence check_recurrence(const char *fn, const at::Tensor &input, const at::Tensor &u, const at::Tensor &v,
+                            const at::Tensor &decay, const OptTensor &initial, const OptTensor &offsets, double scale) {
+  Recurrence r;
+  r.s = check_sequences(fn, input, offsets);
+  check_operand(fn, "recurrence_gate", u, input.sizes(), input.scalar_type(), input);
+  check_operand(fn, "input_gate", v, input.sizes(), input.scalar_type(), input);
+  check_operand(fn, "decay", decay, {r.s.C}, at::kFloat, input);
+  r.state = {state_count(r.s), r.s.C};
+  if (initial.has_value()) check_operand(fn, "initial_state", *initial, r.state, at::kFloat, input);
+  TORCH_CHECK(scale > 0, "dwconv_b200.", fn, ": scale must be positive");
+  return r;
+}
+
+// (y, final state or None, what the backward starts from or None)
+std::tuple<at::Tensor, OptTensor, OptTensor> recurrence(const at::Tensor &input, const at::Tensor &gate_u,
+                                                        const at::Tensor &gate_v, const at::Tensor &decay,
+                                                        const OptTensor &initial, const OptTensor &offsets,
+                                                        double scale, bool want_state, bool want_backward) {
+  const char *fn = "gated_linear_recurrence";
+  const Recurrence r = check_recurrence(fn, input, gate_u, gate_v, decay, initial, offsets, scale);
+  c10::cuda::CUDAGuard guard(input.device());
+  at::Tensor y = at::empty(input.sizes(), input.options(), at::MemoryFormat::Contiguous);
+  const auto wide = input.options().dtype(at::kFloat);
+  OptTensor state, ckpt;
+  if (no_rows(input)) {
+    if (want_state) state = state_or_zeros(initial, r.state, wide);
+    if (want_backward) ckpt = at::empty({0}, wide);
+    return {y, state, ckpt};
+  }
+  if (want_state) state = at::empty(r.state, wide);
+  if (want_backward) {
+    const size_t nbytes = dwconv_b200_recurrence_checkpoint_bytes(&r.s);
+    TORCH_CHECK(nbytes != 0, "dwconv_b200.", fn, ": invalid geometry");
+    ckpt = at::empty({(int64_t)(nbytes / 4)}, wide);
+  }
+  const at::Tensor x = rows_of(input), u = rows_of(gate_u), v = rows_of(gate_v), d = decay.contiguous();
+  const OptTensor init = contiguous(initial);
+  const dwconv_b200_rows xr = rows_arg(x), ur = rows_arg(u), vr = rows_arg(v);
+  check_status(dwconv_b200_recurrence(&xr, &ur, &vr, d.data_ptr<float>(), (const float *)ptr(init), y.data_ptr(),
+                                      state.has_value() ? state->data_ptr<float>() : nullptr,
+                                      ckpt.has_value() ? ckpt->data_ptr<float>() : nullptr, sequence_dtype(x), &r.s,
+                                      (float)scale, stream_of(x)),
+               fn);
+  return {y, state, ckpt};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, OptTensor> recurrence_backward(
+    const at::Tensor &input, const at::Tensor &gate_u, const at::Tensor &gate_v, const at::Tensor &decay,
+    const OptTensor &initial, const OptTensor &offsets, double scale, const at::Tensor &ckpt, const OptTensor &grad,
+    const OptTensor &grad_state, bool want_initial) {
+  const char *fn = "gated_linear_recurrence backward";
+  const Recurrence r = check_recurrence(fn, input, gate_u, gate_v, decay, initial, offsets, scale);
+  c10::cuda::CUDAGuard guard(input.device());
+  if (grad.has_value()) check_operand(fn, "grad_output", *grad, input.sizes(), input.scalar_type(), input);
+  if (grad_state.has_value()) check_operand(fn, "grad_state", *grad_state, r.state, at::kFloat, input);
+  const auto wide = input.options().dtype(at::kFloat);
+  at::Tensor dx = at::empty(input.sizes(), input.options(), at::MemoryFormat::Contiguous);
+  at::Tensor du = at::empty_like(dx), dv = at::empty_like(dx);
+  OptTensor dinit;
+  if (no_rows(input)) {
+    if (want_initial) dinit = state_or_zeros(grad_state, r.state, wide);
+    return {dx, du, dv, at::zeros(decay.sizes(), wide), dinit};
+  }
+  at::Tensor dd = at::empty(decay.sizes(), wide);
+  if (want_initial) dinit = at::empty(r.state, wide);
+  const at::Tensor x = rows_of(input), u = rows_of(gate_u), v = rows_of(gate_v), d = decay.contiguous();
+  const at::Tensor g = grad.has_value() ? rows_of(*grad) : at::zeros(input.sizes(), input.options());
+  const OptTensor init = contiguous(initial), gs = contiguous(grad_state);
+  const size_t nbytes = dwconv_b200_recurrence_workspace_bytes(&r.s);
+  TORCH_CHECK(nbytes != 0, "dwconv_b200.", fn, ": invalid geometry");
+  at::Tensor ws = at::empty({(int64_t)nbytes}, input.options().dtype(at::kByte));
+  const dwconv_b200_rows xr = rows_arg(x), ur = rows_arg(u), vr = rows_arg(v), gr = rows_arg(g);
+  check_status(dwconv_b200_recurrence_backward(
+                   &xr, &ur, &vr, d.data_ptr<float>(), (const float *)ptr(init), ckpt.data_ptr<float>(), &gr,
+                   (const float *)ptr(gs), dx.data_ptr(), du.data_ptr(), dv.data_ptr(), dd.data_ptr<float>(),
+                   dinit.has_value() ? dinit->data_ptr<float>() : nullptr, ws.data_ptr(), nbytes, sequence_dtype(x),
+                   &r.s, (float)scale, stream_of(x)),
+               fn);
+  return {dx, du, dv, dd, dinit};
+}
+
+at::Tensor recurrence_step(const at::Tensor &input, const at::Tensor &gate_u, const at::Tensor &gate_v,
+                           const at::Tensor &decay, const at::Tensor &state, double scale) {
+  const char *fn = "gated_linear_recurrence_step";
+  const int64_t C = check_step_input(fn, input), B = input.size(0);
+  check_operand(fn, "recurrence_gate", gate_u, input.sizes(), input.scalar_type(), input);
+  check_operand(fn, "input_gate", gate_v, input.sizes(), input.scalar_type(), input);
+  check_operand(fn, "decay", decay, {C}, at::kFloat, input);
+  check_state(fn, state, {B, C}, at::kFloat, input);
+  TORCH_CHECK(scale > 0, "dwconv_b200.", fn, ": scale must be positive");
+  c10::cuda::CUDAGuard guard(input.device());
+  at::Tensor y = at::empty({B, C}, input.options());
+  if (no_rows(input)) return y;
+  note_written(state);
+  const at::Tensor x = rows_of(input), u = rows_of(gate_u), v = rows_of(gate_v), d = decay.contiguous();
+  check_status(dwconv_b200_recurrence_step(x.data_ptr(), x.stride(0), u.data_ptr(), u.stride(0), v.data_ptr(),
+                                           v.stride(0), d.data_ptr<float>(), state.data_ptr<float>(), y.data_ptr(),
+                                           sequence_dtype(x), (int)B, (int)C, (float)scale, stream_of(x)),
+               fn);
+  return y;
+}
+
+// The rows of a tensor of any rank over its last dimension, as they lie where one stride steps
+// through them, else as a contiguous copy.
+at::Tensor norm_rows(const at::Tensor &t) {
+  const int64_t C = t.size(-1);
+  const at::Tensor a = rows_of(t);
+  if (a.dim() == 2) return a;
+  if (a.dim() == 1) return a.unsqueeze(0);
+  int64_t stride = 0, span = 1;  // stride of the rows, and what the next outer dimension must step by
+  bool ok = true, any = false;
+  for (int64_t d = a.dim() - 2; d >= 0 && ok; --d) {
+    if (a.size(d) == 1) continue;
+    if (!any) {
+      any = true;
+      stride = a.stride(d);
+    } else {
+      ok = a.stride(d) == stride * span;
+    }
+    span *= a.size(d);
+  }
+  if (!ok) return a.contiguous().view({-1, C});
+  return a.as_strided({span, C}, {any ? stride : C, 1}, a.storage_offset());
+}
+
+int64_t check_norm(const char *fn, const at::Tensor &input, const OptTensor &weight, const OptTensor &bias, double eps) {
+  check_cuda(input, "input");
+  sequence_dtype(input);
+  TORCH_CHECK(input.dim() >= 1 && input.size(-1) >= 1 && input.size(-1) <= (1 << 26), "dwconv_b200.", fn,
+              ": expected input [..., C], got ", shape_text(input));
+  const int64_t C = input.size(-1);
+  if (weight.has_value()) check_operand(fn, "weight", *weight, {C}, input.scalar_type(), input);
+  if (bias.has_value()) check_operand(fn, "bias", *bias, {C}, input.scalar_type(), input);
+  TORCH_CHECK(eps >= 0, "dwconv_b200.", fn, ": eps must not be negative");
+  return C;
+}
+
+// (y, (mean, rstd) of each row or None)
+std::tuple<at::Tensor, OptTensor> layer_norm(const at::Tensor &input, const OptTensor &weight, const OptTensor &bias,
+                                             double eps, bool want_backward) {
+  const char *fn = "layer_norm";
+  const int64_t C = check_norm(fn, input, weight, bias, eps), rows = input.numel() / C;
+  c10::cuda::CUDAGuard guard(input.device());
+  at::Tensor y = at::empty(input.sizes(), input.options(), at::MemoryFormat::Contiguous);
+  OptTensor stats;
+  if (want_backward) stats = at::empty({rows, 2}, input.options().dtype(at::kFloat));
+  if (rows == 0) return {y, stats};
+  const at::Tensor x = norm_rows(input);
+  const OptTensor w = contiguous(weight), b = contiguous(bias);
+  check_status(dwconv_b200_layer_norm(x.data_ptr(), x.stride(0), ptr(w), ptr(b), y.data_ptr(),
+                                      stats.has_value() ? stats->data_ptr<float>() : nullptr, sequence_dtype(x), rows,
+                                      (int)C, (float)eps, stream_of(x)),
+               fn);
+  return {y, stats};
+}
+
+std::tuple<at::Tensor, OptTensor, OptTensor> layer_norm_backward(const at::Tensor &input, const OptTensor &weight,
+                                                                 const at::Tensor &stats, const at::Tensor &grad,
+                                                                 bool want_weight, bool want_bias) {
+  const char *fn = "layer_norm backward";
+  const int64_t C = check_norm(fn, input, weight, OptTensor(), 0.), rows = input.numel() / C;
+  check_operand(fn, "grad_output", grad, input.sizes(), input.scalar_type(), input);
+  c10::cuda::CUDAGuard guard(input.device());
+  at::Tensor dx = at::empty(input.sizes(), input.options(), at::MemoryFormat::Contiguous);
+  OptTensor dw, db, ws;
+  if (rows == 0) {
+    if (want_weight) dw = at::zeros({C}, input.options());
+    if (want_bias) db = at::zeros({C}, input.options());
+    return {dx, dw, db};
+  }
+  if (want_weight) dw = at::empty({C}, input.options());
+  if (want_bias) db = at::empty({C}, input.options());
+  const at::Tensor x = norm_rows(input), g = norm_rows(grad);
+  const OptTensor w = contiguous(weight);
+  const int code = sequence_dtype(x);
+  size_t nbytes = 0;
+  if (want_weight || want_bias) {
+    nbytes = dwconv_b200_layer_norm_workspace_bytes(code, rows, (int)C);
+    TORCH_CHECK(nbytes != 0, "dwconv_b200.", fn, ": invalid geometry");
+    ws = at::empty({(int64_t)nbytes}, input.options().dtype(at::kByte));
+  }
+  check_status(dwconv_b200_layer_norm_backward(
+                   x.data_ptr(), x.stride(0), ptr(w), stats.data_ptr<float>(), g.data_ptr(), g.stride(0), dx.data_ptr(),
+                   dw.has_value() ? dw->data_ptr() : nullptr, db.has_value() ? db->data_ptr() : nullptr,
+                   ws.has_value() ? ws->data_ptr() : nullptr, nbytes, code, rows, (int)C, stream_of(x)),
+               fn);
+  return {dx, dw, db};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -283,4 +670,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("dwconv2d", &dwconv2d);
   m.def("dwconv2d_small", &dwconv2d_small);
   m.def("dwconv2d_backward_kernel", &dwconv2d_backward_kernel);
+  m.def("conv1d_causal", &conv1d_causal);
+  m.def("conv1d_causal_backward", &conv1d_causal_backward);
+  m.def("conv1d_causal_step", &conv1d_causal_step);
+  m.def("recurrence", &recurrence);
+  m.def("recurrence_backward", &recurrence_backward);
+  m.def("recurrence_step", &recurrence_step);
+  m.def("layer_norm", &layer_norm);
+  m.def("layer_norm_backward", &layer_norm_backward);
 }

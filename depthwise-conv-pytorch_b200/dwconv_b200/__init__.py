@@ -4,8 +4,13 @@ from .dwconv import (DepthwiseConv2d, DepthwiseConv2dFunction, check_options,  #
                      use_dwconv2d_small)
 from . import _C  # noqa: F401
 from .host import HostMapsPipeline, HostMapsStep  # noqa: F401
+from .sequence import (CausalDepthwiseConv1d, GatedLinearRecurrence, LayerNorm,  # noqa: F401
+                       RecurrentMixer, depthwise_conv1d_causal, depthwise_conv1d_causal_step,
+                       gated_linear_recurrence, gated_linear_recurrence_step, layer_norm)
 from .stack import (EFFICIENTNET_B0_DEPTHWISE, DepthwiseStack, StackStep,  # noqa: F401
                     from_conv2d, to_conv2d)
 
 __all__ = ["depthwise_conv2d", "depthwise_conv2d_epilogue", "DepthwiseConv2d", "HostMapsStep", "HostMapsPipeline", "DepthwiseStack", "StackStep",
-           "from_conv2d", "to_conv2d"]
+           "from_conv2d", "to_conv2d", "depthwise_conv1d_causal", "depthwise_conv1d_causal_step",
+           "gated_linear_recurrence", "gated_linear_recurrence_step", "layer_norm", "CausalDepthwiseConv1d",
+           "GatedLinearRecurrence", "LayerNorm", "RecurrentMixer"]

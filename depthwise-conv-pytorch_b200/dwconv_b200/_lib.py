@@ -28,6 +28,21 @@ class Shape(ctypes.Structure):
                 ("N", "C", "H", "W", "kh", "kw", "sh", "sw", "ph", "pw", "Ho", "Wo")]
 
 
+class Sequence(ctypes.Structure):
+    """Mirror of ``dwconv_b200_sequence``."""
+    _fields_ = [("B", ctypes.c_int), ("T", ctypes.c_int), ("C", ctypes.c_int),
+                ("offsets", ctypes.c_void_p), ("S", ctypes.c_int)]
+
+
+class Rows(ctypes.Structure):
+    """Mirror of ``dwconv_b200_rows``."""
+    _fields_ = [("data", ctypes.c_void_p), ("batch_stride", ctypes.c_longlong),
+                ("row_stride", ctypes.c_longlong)]
+
+
+MAX_TAPS = 8
+
+
 def _load():
     path = os.environ.get("DWCONV_B200_LIB", LIB_PATH)
     if not os.path.exists(path):
@@ -37,6 +52,8 @@ def _load():
     lib = ctypes.CDLL(path)
     vp, ci, sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
     sp = ctypes.POINTER(Shape)
+    ll, cf = ctypes.c_longlong, ctypes.c_float
+    qp, rp = ctypes.POINTER(Sequence), ctypes.POINTER(Rows)
     sig = {
         "dwconv_b200_version": (ci, []),
         "dwconv_b200_status_string": (ctypes.c_char_p, [ci]),
@@ -73,6 +90,18 @@ def _load():
         "dwconv_b200_backward_exchange": (ci, [vp, vp, vp, vp, vp, vp, sz, ci, sp, vp, vp]),
         "dwconv_b200_backward_filter_allreduce": (ci, [vp, vp, vp, vp, sz, ci, sp, vp, vp]),
         "dwconv_b200_backward_allreduce": (ci, [vp, vp, vp, vp, vp, vp, sz, ci, sp, vp, vp]),
+        "dwconv_b200_conv1d_causal": (ci, [rp, vp, vp, vp, vp, vp, ci, qp, ci, ci, vp]),
+        "dwconv_b200_conv1d_causal_workspace_bytes": (sz, [ci, qp, ci]),
+        "dwconv_b200_conv1d_causal_backward": (ci, [rp, vp, vp, vp, rp] + [vp] * 6 + [sz, ci, qp, ci, ci, vp]),
+        "dwconv_b200_conv1d_causal_step": (ci, [vp, ll, vp, vp, vp, vp] + [ci] * 5 + [vp]),
+        "dwconv_b200_recurrence_checkpoint_bytes": (sz, [qp]),
+        "dwconv_b200_recurrence_workspace_bytes": (sz, [qp]),
+        "dwconv_b200_recurrence": (ci, [rp, rp, rp, vp, vp, vp, vp, vp, ci, qp, cf, vp]),
+        "dwconv_b200_recurrence_backward": (ci, [rp, rp, rp, vp, vp, vp, rp] + [vp] * 7 + [sz, ci, qp, cf, vp]),
+        "dwconv_b200_recurrence_step": (ci, [vp, ll, vp, ll, vp, ll, vp, vp, vp, ci, ci, ci, cf, vp]),
+        "dwconv_b200_layer_norm": (ci, [vp, ll, vp, vp, vp, vp, ci, ll, ci, cf, vp]),
+        "dwconv_b200_layer_norm_workspace_bytes": (sz, [ci, ll, ci]),
+        "dwconv_b200_layer_norm_backward": (ci, [vp, ll, vp, vp, vp, ll, vp, vp, vp, vp, sz, ci, ll, ci, vp]),
     }
     for name, (res, args) in sig.items():
         try:
@@ -140,6 +169,11 @@ EXPORTS = (
     "dwconv_b200_exchange_bytes", "dwconv_b200_exchange_create", "dwconv_b200_exchange_connect",
     "dwconv_b200_exchange_destroy", "dwconv_b200_exchange_finish",
     "dwconv_b200_backward_filter_exchange",
+    "dwconv_b200_conv1d_causal", "dwconv_b200_conv1d_causal_workspace_bytes",
+    "dwconv_b200_conv1d_causal_backward", "dwconv_b200_conv1d_causal_step",
+    "dwconv_b200_recurrence_checkpoint_bytes", "dwconv_b200_recurrence_workspace_bytes",
+    "dwconv_b200_recurrence", "dwconv_b200_recurrence_backward", "dwconv_b200_recurrence_step",
+    "dwconv_b200_layer_norm", "dwconv_b200_layer_norm_workspace_bytes", "dwconv_b200_layer_norm_backward",
 )
 
 

@@ -390,6 +390,129 @@ DWCONV_B200_API int dwconv_b200_backward_filter_static(const void *x, const void
                                                        int dtype, const dwconv_b200_shape *shape,
                                                        void *stream);
 
+/* ------------------------------------------------------------------------
+ * Sequence operators: rows of C channels in time order, channels side by side
+ * ([B, T, C]).  No counterpart in the reference, which has two-dimensional maps
+ * only; they are the per-channel operators of models that mix tokens with a
+ * short causal depthwise convolution and a gated linear recurrence, and the norm
+ * in front of them.  f32 / f16 / bf16 data, all arithmetic and state in fp32 and
+ * one rounding per stored value.  Results do not depend on timing: every sum has
+ * one fixed order.
+ *
+ * Packed sequences: with `offsets` (device memory, S + 1 ascending row numbers,
+ * offsets[0] = 0) B is 1 and sequence j is rows offsets[j] .. offsets[j+1]-1 of
+ * the T rows; a sequence may be empty.  Rows of no sequence (behind
+ * offsets[S]) give zeros in every output.  The list is read on the device, its
+ * values are clamped to [0, T]: a list that is not ascending gives unspecified
+ * values, never an access out of bounds.
+ *
+ * Per-sequence states are [count, ...] with count = S for packed rows, else B.
+ * ---------------------------------------------------------------------- */
+typedef struct dwconv_b200_sequence {
+  int B;               /* batch elements (1 with offsets) */
+  int T;               /* rows of each; 0 is allowed */
+  int C;               /* channels */
+  const void *offsets; /* int32 [S + 1] on the device, or NULL */
+  int S;               /* packed sequences */
+} dwconv_b200_sequence;
+
+/* An input: element (b, t, c) at data[b * batch_stride + t * row_stride + c] (strides in elements;
+ * any, overlapping ones included).  Outputs are contiguous [B, T, C]. */
+typedef struct dwconv_b200_rows {
+  const void *data;
+  long long batch_stride, row_stride;
+} dwconv_b200_rows;
+
+#define DWCONV_B200_MAX_TAPS 8
+
+/* Causal depthwise convolution of a sequence:
+ *   p[t,c] = bias[c] + sum_k w[c,0,k] * x[t - (taps-1) + k, c],   y = act(p)
+ * where rows before the sequence are the rows of `initial` [count, taps-1, C] (oldest first), or
+ * zero when it is NULL.  w [C,1,taps] and bias [C] (or NULL) in the data's type, taps 1 to
+ * DWCONV_B200_MAX_TAPS; `final_state` [count, taps-1, C], or NULL, receives the last taps-1 rows of
+ * each sequence (those of `initial` where it is shorter): what the next piece takes as `initial`. */
+DWCONV_B200_API int dwconv_b200_conv1d_causal(const dwconv_b200_rows *x, const void *w, const void *bias,
+                                              const void *initial, void *y, void *final_state, int dtype,
+                                              const dwconv_b200_sequence *seq, int taps, int activation,
+                                              void *stream);
+
+/* Scratch bytes of dwconv_b200_conv1d_causal_backward (a multiple of 16; 0: bad arguments). */
+DWCONV_B200_API size_t dwconv_b200_conv1d_causal_workspace_bytes(int dtype, const dwconv_b200_sequence *seq,
+                                                                 int taps);
+
+/* Gradients of the above.  dy, and dfinal (the gradient of final_state, or NULL), in; dx [B,T,C],
+ * dw [C,1,taps], dbias [C] and dinitial [count, taps-1, C] (either of the last two may be NULL) out.
+ * The activation's input is recomputed from x. */
+DWCONV_B200_API int dwconv_b200_conv1d_causal_backward(const dwconv_b200_rows *x, const void *w,
+                                                       const void *bias, const void *initial,
+                                                       const dwconv_b200_rows *dy, const void *dfinal,
+                                                       void *dx, void *dw, void *dbias, void *dinitial,
+                                                       void *workspace, size_t workspace_bytes, int dtype,
+                                                       const dwconv_b200_sequence *seq, int taps,
+                                                       int activation, void *stream);
+
+/* One row for each of B sequences: x [B, C] (rows `x_stride` elements apart), `state` [B, taps-1, C]
+ * read and shifted in place, y [B, C].  Same values as dwconv_b200_conv1d_causal with T = 1. */
+DWCONV_B200_API int dwconv_b200_conv1d_causal_step(const void *x, long long x_stride, const void *w,
+                                                   const void *bias, void *state, void *y, int dtype, int B,
+                                                   int C, int taps, int activation, void *stream);
+
+/* Gated linear recurrence, channel by channel:
+ *   r = sigmoid(u), i = sigmoid(v), a = exp(-scale * softplus(decay[c]) * r)
+ *   h[t] = a * h[t-1] + sqrt(1 - a^2) * i * x[t],     y[t] = h[t]
+ * x, u (recurrence gate) and v (input gate) are inputs of one type; `decay` [C], `initial` [count, C]
+ * (or NULL: zeros) and `final_state` [count, C] (or NULL) are fp32, scale > 0.  `checkpoints`, or NULL:
+ * receives the states that dwconv_b200_recurrence_backward starts from,
+ * dwconv_b200_recurrence_checkpoint_bytes bytes, 16-byte aligned. */
+DWCONV_B200_API size_t dwconv_b200_recurrence_checkpoint_bytes(const dwconv_b200_sequence *seq);
+DWCONV_B200_API int dwconv_b200_recurrence(const dwconv_b200_rows *x, const dwconv_b200_rows *u,
+                                           const dwconv_b200_rows *v, const float *decay,
+                                           const float *initial, void *y, float *final_state,
+                                           float *checkpoints, int dtype, const dwconv_b200_sequence *seq,
+                                           float scale, void *stream);
+
+/* Scratch bytes of dwconv_b200_recurrence_backward (a multiple of 16; 0: bad arguments). */
+DWCONV_B200_API size_t dwconv_b200_recurrence_workspace_bytes(const dwconv_b200_sequence *seq);
+
+/* Gradients of the above from the same inputs, the forward call's `checkpoints`, dy and dfinal
+ * (fp32 [count, C], or NULL): dx, du, dv [B,T,C] in the data's type, ddecay [C] and dinitial
+ * [count, C] (or NULL) in fp32.  The states between checkpoints are recomputed in fp32. */
+DWCONV_B200_API int dwconv_b200_recurrence_backward(const dwconv_b200_rows *x, const dwconv_b200_rows *u,
+                                                    const dwconv_b200_rows *v, const float *decay,
+                                                    const float *initial, const float *checkpoints,
+                                                    const dwconv_b200_rows *dy, const float *dfinal,
+                                                    void *dx, void *du, void *dv, float *ddecay,
+                                                    float *dinitial, void *workspace,
+                                                    size_t workspace_bytes, int dtype,
+                                                    const dwconv_b200_sequence *seq, float scale,
+                                                    void *stream);
+
+/* One row for each of B sequences: x, u, v [B, C] (rows *_stride elements apart), `state` fp32 [B, C]
+ * updated in place, y [B, C]. */
+DWCONV_B200_API int dwconv_b200_recurrence_step(const void *x, long long x_stride, const void *u,
+                                                long long u_stride, const void *v, long long v_stride,
+                                                const float *decay, float *state, void *y, int dtype,
+                                                int B, int C, float scale, void *stream);
+
+/* Layer norm over C values side by side, `rows` of them `x_stride` elements apart:
+ *   y = (x - mean) * rstd * w + b,  rstd = 1 / sqrt(var + eps)
+ * w and b [C] in the data's type, each may be NULL (1 resp. 0); y [rows, C] contiguous.  `stats`,
+ * or NULL: fp32 [rows, 2], receives (mean, rstd) of each row for the backward. */
+DWCONV_B200_API int dwconv_b200_layer_norm(const void *x, long long x_stride, const void *w, const void *b,
+                                           void *y, float *stats, int dtype, long long rows, int C,
+                                           float eps, void *stream);
+
+/* Scratch bytes of dwconv_b200_layer_norm_backward (a multiple of 16; 0: bad arguments). */
+DWCONV_B200_API size_t dwconv_b200_layer_norm_workspace_bytes(int dtype, long long rows, int C);
+
+/* dx [rows, C], and dw, db [C] (each may be NULL) in the data's type, from x, w, the forward's
+ * `stats` and dy. */
+DWCONV_B200_API int dwconv_b200_layer_norm_backward(const void *x, long long x_stride, const void *w,
+                                                    const float *stats, const void *dy, long long dy_stride,
+                                                    void *dx, void *dw, void *db, void *workspace,
+                                                    size_t workspace_bytes, int dtype, long long rows,
+                                                    int C, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
