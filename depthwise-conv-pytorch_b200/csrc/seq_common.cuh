@@ -118,8 +118,7 @@ struct ColumnSumOut {
   void *first, *second;
   int dtype;
   int C, K;             // split = C * K
-  const float *decay;   // non-null: the sum of column c times scale * sigmoid(decay[c])
-  float scale;
+  const float *decay;   // non-null: the sum of column c times sigmoid(decay[c]) / softplus(decay[c])
 };
 
 constexpr int COLSUM_LANES = 32, COLSUM_WARPS = 8;
@@ -146,7 +145,11 @@ column_sum_kernel(const float *__restrict__ part, long long parts, int M, Column
 #pragma unroll
   for (int i = 0; i < COLSUM_WARPS; ++i) v += s[i][lane];
   const int split = out.C * out.K;
-  if (out.decay != nullptr && m < split) v *= out.scale / (1.f + expf(-out.decay[m]));
+  if (out.decay != nullptr && m < split) {
+    const float d = out.decay[m];
+    // the quotient tends to 1 for far negative values, where both vanish
+    v *= d < -80.f ? 1.f : 1.f / ((1.f + expf(-d)) * (d > 20.f ? d : log1pf(expf(d))));
+  }
   if (m < split) {
     const int k = m / out.C, c = m - k * out.C;
     if (out.first) store_as(out.first, (long long)c * out.K + k, v, out.dtype);

@@ -575,7 +575,7 @@ int dwconv_b200_conv1d_causal_backward(const dwconv_b200_rows *x, const void *w,
   e = api_launch_status();
   if (e) return e;
   launch_column_sum(a.part, conv_parts(*seq), (taps + 1) * seq->C,
-                    ColumnSumOut{dw, dbias, dtype, seq->C, taps, nullptr, 0.f}, st);
+                    ColumnSumOut{dw, dbias, dtype, seq->C, taps, nullptr}, st);
   return api_launch_status();
 }
 

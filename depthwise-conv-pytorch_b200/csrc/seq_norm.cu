@@ -514,7 +514,7 @@ int dwconv_b200_layer_norm_backward(const void *x, long long x_stride, const voi
     e = api_launch_status();
     if (e) return e;
   }
-  if (params) launch_column_sum(part, parts, 2 * C, ColumnSumOut{dw, db, dtype, C, 1, nullptr, 0.f}, st);
+  if (params) launch_column_sum(part, parts, 2 * C, ColumnSumOut{dw, db, dtype, C, 1, nullptr}, st);
   return api_launch_status();
 }
 

@@ -1,14 +1,17 @@
 // Gated linear recurrence over [B, T, C] sequences: a scan along T with its gates computed on the
 // way, the backward pass, and the one-row step (declarations: include/dwconv_b200.h).
 //
-//   r = sigmoid(u), i = sigmoid(v), z = scale softplus(decay) r
-//   d = 1 - exp(-z),  a = 1 - d,  beta = sqrt(1 - a^2) = sqrt(d (2 - d))
-//   h[t] = a h[t-1] + beta i x,   y = h
-// and with g[t] = dy[t] + a[t+1] g[t+1]:
-//   dx = g beta i,  dv = dx x (1 - i),  dz = g (a^2 / beta i x - a h[t-1]),  du = dz z (1 - r),
-//   ddecay = scale sigmoid(decay) sum_t dz r,  dinitial = a[0] g[0].
-// d, not a, is what is computed: for the long memories such models use z is small, and 1 - exp(-z)
-// by its power series keeps both 1 - a and beta to a few units in the last place.
+//   r = sigmoid(u), i = sigmoid(v), z = k r with k = scale softplus(decay)
+//   a = exp(-z),  beta = sqrt(1 - a^2),  h[t] = a h[t-1] + beta i x,  y = h
+// and with g[t] = dy[t] + a[t+1] g[t+1], rho = z / beta:
+//   dx = g beta i,  dv = dx x (1 - i),  dz z = g a (a i x rho - z h[t-1]),  du = dz z (1 - r),
+//   ddecay = sigmoid(decay) / softplus(decay) sum_t dz z,  dinitial = a[0] g[0].
+// For the long memories such models use z is small.  There a = 1 + (exp(-z) - 1) comes from the power
+// series of the bracket, and with t = sqrt(r) = rsqrt(1 + exp(-u))
+//   beta = sqrt(2 k) t p(z),  rho = sqrt(k / 2) t / p(z),  p(z) = sqrt((1 - exp(-2 z)) / (2 z)),
+// p and 1 / p by their power series: no difference of nearly equal numbers, and two special-function
+// calls per gate (the special-function unit is one of the three things that bound these kernels, beside
+// memory and the issue of instructions).
 //
 // Bound by memory: forward x, u, v in and y out; backward x, u, v, dy in and dx, du, dv out.
 //
@@ -16,14 +19,18 @@
 // of W * L rows.  A warp reduces its rows to one pair (P, H): the state that leaves them is
 // P h + H.  Pairs meet in shared memory, every warp folds those in front of it onto the state that
 // enters the tile, and walks its rows once more from registers.  Tiles follow one another along T.
-// Where there are too few (channel block, batch) pairs to fill the device, a cluster of CTAs takes
+// Where there are too few (channel block, batch) pairs to fill the device evenly, a cluster of CTAs takes
 // neighbouring tiles together and passes its tiles' pairs through distributed shared memory: one
-// cluster barrier per CTAs * W * L rows, no pass over the data for it, and the same order of
+// cluster barrier per CTAs * W * L rows, no second pass over the data for it, and the same order of
 // operations on every run.
+//
+// A warp copies the rows of its next tile to shared memory by 16-byte asynchronous copies as soon
+// as those of the current one are in registers, so that the barriers, folds and stores run under
+// them.  Tensors without 16-byte rows are read two elements per lane instead, without copies ahead.
 //
 // The forward pass keeps the fp32 state that enters each tile (1 / (W L) of the rows); the backward
 // pass starts from it, so it reads y nowhere and its h[t-1] have not been rounded to the data's type.
-#include <mutex>
+#include <atomic>
 
 #include "seq_common.cuh"
 
@@ -32,10 +39,9 @@ namespace {
 
 constexpr int REC_L = 8, REC_W = 8, REC_TILE = REC_L * REC_W, REC_GROUP = 64;
 constexpr int REC_THREADS = REC_W * 32;
-constexpr int REC_MAX_CLUSTER = 8;
-// Largest z for which the power series is used alone: its first omitted term, z^6 / 5040 relative, is
-// 5e-8 there.
-constexpr float REC_SERIES = 0.25f;
+constexpr int REC_MAX_CLUSTER = 16;  // 16 needs the non-portable attribute
+// Largest z for which the power series are used: what they omit is 5e-8 of exp(-z) - 1 and 2e-9 of p there.
+constexpr float REC_SERIES = 0.125f;
 
 // ---- arithmetic on channel pairs ---------------------------------------------------------------
 
@@ -43,7 +49,9 @@ __device__ __forceinline__ float2 f2(float v) { return make_float2(v, v); }
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
-__device__ __forceinline__ float2 neg2(float2 a) { return make_float2(-a.x, -a.y); }
+// The same value, of which the compiler does not know that: what is computed from it again is not kept in
+// a register meanwhile.
+__device__ __forceinline__ void forget(float2 &v) { asm volatile("" : "+f"(v.x), "+f"(v.y)); }
 
 __device__ __forceinline__ float ex2f(float v) {
   float r;
@@ -63,59 +71,85 @@ __device__ __forceinline__ float rsqf(float v) {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-// 1 / (1 + 2^(-v log2 e)); an overflowing exponential gives 0.
-__device__ __forceinline__ float2 sigmoid2(float2 v) {
+// 1 + exp(-v)
+__device__ __forceinline__ float2 one_plus_exp2(float2 v) {
   const float2 e = mul2(v, f2(-LOG2E));
-  const float2 s = add2(make_float2(ex2f(e.x), ex2f(e.y)), f2(1.f));
+  return add2(make_float2(ex2f(e.x), ex2f(e.y)), f2(1.f));
+}
+// sigmoid and its square root; an overflowing exponential gives 0
+__device__ __forceinline__ float2 sigmoid2(float2 v) {
+  const float2 s = one_plus_exp2(v);
   return make_float2(rcpf(s.x), rcpf(s.y));
 }
+__device__ __forceinline__ float2 root_sigmoid2(float2 v) {
+  const float2 s = one_plus_exp2(v);
+  return make_float2(rsqf(s.x), rsqf(s.y));
+}
+__device__ __forceinline__ float2 one_minus2(float2 v) { return fma2(v, f2(-1.f), f2(1.f)); }
 
-// 1 - exp(-z), z >= 0.  `series`: every z of this warp is at most REC_SERIES.
-__device__ __forceinline__ float2 decay2(float2 z, bool series) {
-  float2 p = fma2(z, f2(-1.f / 720.f), f2(1.f / 120.f));
-  p = fma2(p, neg2(z), f2(1.f / 24.f));
-  p = fma2(p, neg2(z), f2(1.f / 6.f));
-  p = fma2(p, neg2(z), f2(0.5f));
-  p = fma2(p, neg2(z), f2(1.f));
-  float2 d = mul2(z, p);
-  if (!series) {
-    const float2 e = mul2(z, f2(-LOG2E));
-    if (!(z.x <= REC_SERIES)) d.x = 1.f - ex2f(e.x);
-    if (!(z.y <= REC_SERIES)) d.y = 1.f - ex2f(e.y);
-  }
-  return d;
+__device__ __forceinline__ float2 horner2(float2 p, float2 s, float c) { return fma2(p, s, f2(c)); }
+// exp(s) - 1, p(-s) and 1 / p(-s) for -REC_SERIES <= s <= 0, from the Taylor expansions of
+// exp(s), exp(s / 2) sqrt(sinh(s) / s) and its reciprocal about 0.
+__device__ __forceinline__ float2 expm1_series2(float2 s) {
+  float2 p = horner2(f2(1.f / 120.f), s, 1.f / 24.f);
+  p = horner2(p, s, 1.f / 6.f);
+  p = horner2(p, s, 0.5f);
+  return mul2(s, horner2(p, s, 1.f));
+}
+__device__ __forceinline__ float2 p_series2(float2 s) {
+  float2 p = horner2(f2(3.f / 1280.f), s, 79.f / 5760.f);
+  p = horner2(p, s, 1.f / 16.f);
+  p = horner2(p, s, 5.f / 24.f);
+  p = horner2(p, s, 0.5f);
+  return horner2(p, s, 1.f);
+}
+__device__ __forceinline__ float2 inverse_p_series2(float2 s) {
+  float2 p = horner2(f2(-19.f / 11520.f), s, -1.f / 640.f);
+  p = horner2(p, s, 1.f / 48.f);
+  p = horner2(p, s, 1.f / 24.f);
+  p = horner2(p, s, -0.5f);
+  return horner2(p, s, 1.f);
 }
 
-// a = exp(-z) from d = 1 - exp(-z): their difference from 1 where d is small, the exponential itself
-// where a is, so that each is good to a few units in its own last place.
-__device__ __forceinline__ float2 keep2(float2 z, float2 d, bool series) {
-  float2 a = add2(f2(1.f), neg2(d));
-  if (!series) {
-    const float2 e = mul2(z, f2(-LOG2E));
-    if (!(z.x <= REC_SERIES)) a.x = ex2f(e.x);
-    if (!(z.y <= REC_SERIES)) a.y = ex2f(e.y);
+// What a lane keeps of its channels: -k and sqrt(2 k).
+struct Rate {
+  float2 ks, root;
+};
+
+// 1 - a^2 for any s, kept off zero so that its reciprocal root stays finite (z = 0: closed gate).
+__device__ __forceinline__ float2 beta_square2(float2 s) {
+  float2 m = expm1_series2(s);
+  const float2 e = mul2(s, f2(LOG2E));
+  if (!(s.x >= -REC_SERIES)) m.x = ex2f(e.x) - 1.f;
+  if (!(s.y >= -REC_SERIES)) m.y = ex2f(e.y) - 1.f;
+  const float2 t = fma2(m, m, add2(m, m));
+  float2 r;  // a NaN stays one
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r.x) : "f"(-t.x), "f"(1e-37f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r.y) : "f"(-t.y), "f"(1e-37f));
+  return r;
+}
+__device__ __forceinline__ float2 rsq2(float2 q) { return make_float2(rsqf(q.x), rsqf(q.y)); }
+
+// a = exp(s), good to a few units in its own last place; SERIES: no s of this CTA's channels is below
+// -REC_SERIES.
+template <bool SERIES> __device__ __forceinline__ float2 keep2(float2 s) {
+  float2 a = add2(expm1_series2(s), f2(1.f));
+  if constexpr (!SERIES) {
+    const float2 e = mul2(s, f2(LOG2E));
+    if (!(s.x >= -REC_SERIES)) a.x = ex2f(e.x);
+    if (!(s.y >= -REC_SERIES)) a.y = ex2f(e.y);
   }
   return a;
 }
-
-// d (2 - d) = 1 - a^2, kept off zero so that its reciprocal root stays finite (z = 0: closed gate).
-__device__ __forceinline__ float2 beta_square2(float2 d) {
-  const float2 q = fma2(neg2(d), d, add2(d, d));
-  float2 r;  // a NaN stays one
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r.x) : "f"(q.x), "f"(1e-37f));
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r.y) : "f"(q.y), "f"(1e-37f));
-  return r;
+template <bool SERIES> __device__ __forceinline__ float2 beta2(float2 t, float2 s, const Rate &k) {
+  if constexpr (SERIES) return mul2(mul2(t, k.root), p_series2(s));
+  const float2 q = beta_square2(s);
+  return mul2(q, rsq2(q));
 }
-
-struct Gates {
-  float2 r, i, d;
-};
-__device__ __forceinline__ Gates gates(float2 u, float2 v, float2 kz, bool series) {
-  Gates g;
-  g.r = sigmoid2(u);
-  g.i = sigmoid2(v);
-  g.d = decay2(mul2(kz, g.r), series);
-  return g;
+template <bool SERIES> __device__ __forceinline__ float2 rho2(float2 t, float2 s, const Rate &k) {
+  if constexpr (SERIES) return mul2(mul2(t, mul2(k.root, f2(0.5f))), inverse_p_series2(s));
+  const float2 r = mul2(s, rsq2(beta_square2(s)));
+  return make_float2(-r.x, -r.y);
 }
 
 __device__ __forceinline__ float softplus(float v) { return v > 20.f ? v : log1pf(expf(v)); }
@@ -129,6 +163,10 @@ template <typename T> struct Pair<T, true> {
   using Raw = typename P::Raw;
   static __device__ __forceinline__ int channel(int g, int lane) { return g * REC_GROUP + 2 * lane; }
   static __device__ __forceinline__ Raw zero() { return P::zero(); }
+  static __device__ __forceinline__ Raw closed() {
+    const float f[2] = {-__int_as_float(0x7f800000), -__int_as_float(0x7f800000)};
+    return P::pack(f);
+  }
   static __device__ __forceinline__ Raw load(const T *p, bool on0, bool) {
     return on0 ? P::load(p) : P::zero();
   }
@@ -146,6 +184,10 @@ template <typename T> struct Pair<T, false> {
   struct Raw { T a, b; };
   static __device__ __forceinline__ int channel(int g, int lane) { return g * REC_GROUP + lane; }
   static __device__ __forceinline__ Raw zero() { return Raw{Elem<T>::from_acc(0.f), Elem<T>::from_acc(0.f)}; }
+  static __device__ __forceinline__ Raw closed() {
+    const T inf = Elem<T>::from_acc(-__int_as_float(0x7f800000));
+    return Raw{inf, inf};
+  }
   static __device__ __forceinline__ Raw load(const T *p, bool on0, bool on1) {
     Raw r = zero();
     if (on0) r.a = p[0];
@@ -161,6 +203,52 @@ template <typename T> struct Pair<T, false> {
   }
 };
 
+// ---- copies ahead ------------------------------------------------------------------------------
+
+// 16 bytes to shared memory, or 16 zero bytes.
+__device__ __forceinline__ void copy16(uint32_t to, const void *from, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_done() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncwarp();
+}
+
+// The rows of one tensor that a warp works on, [REC_L][REC_GROUP] in shared memory, copied by its lanes.
+template <typename T> struct RowCopy {
+  static constexpr int E = 16 / (int)sizeof(T), CHUNKS = REC_GROUP / E, ROWS = 32 / CHUNKS, PASSES = REC_L / ROWS;
+  const T *from;  // this lane's chunk of row `sub` of the tensor's row 0
+  long long rs;
+  uint32_t to;
+  int sub;
+  bool on;
+  __device__ __forceinline__ void init(const SeqIn<T> &in, T *stage, int b, int grp, int C, int lane) {
+    const int col = (lane % CHUNKS) * E;
+    sub = lane / CHUNKS;
+    on = grp * REC_GROUP + col < C;
+    from = in.p + (long long)b * in.bs + (on ? grp * REC_GROUP + col : 0);
+    rs = in.rs;
+    to = (uint32_t)__cvta_generic_to_shared(stage + sub * REC_GROUP + col);
+  }
+  // rows t0 .. t0 + REC_L - 1; zeros at T and behind
+  __device__ __forceinline__ void start(int t0, int T_) const {
+    const T *p = from + (long long)(t0 + sub) * rs;
+#pragma unroll
+    for (int k = 0; k < PASSES; ++k) {
+      const bool in = on && t0 + sub + k * ROWS < T_;
+      copy16(to + k * ROWS * REC_GROUP * (int)sizeof(T), in ? p + (long long)(k * ROWS) * rs : from, in);
+    }
+  }
+};
+
+// Rows at T and behind: a gate of -infinity is closed, the state passes through it.  A lane writes what
+// it reads itself.
+template <typename T> __device__ __forceinline__ void close_rows(T *gate, int rows, int lane) {
+#pragma unroll
+  for (int j = 0; j < REC_L; ++j)
+    if (j >= rows) Pack<T, 2>::store(gate + j * REC_GROUP + 2 * lane, Pair<T, true>::closed());
+}
+
 // ---- rows of a warp ----------------------------------------------------------------------------
 
 // Which of a warp's L rows begin a sequence, end one, or belong to none (bit j: row t0 + j).
@@ -168,19 +256,14 @@ struct RowMasks {
   unsigned start, end, none;
 };
 
+// For packed sequences.
 struct RowWalk {
-  SeqSpan sp;
-  __device__ __forceinline__ void init(const SeqList &q, int b) {
-    sp = q.offsets ? SeqSpan{-1, 0, 0} : SeqSpan{b, 0, q.T};
-  }
+  SeqSpan sp{-1, 0, 0};
   template <int L> __device__ __forceinline__ RowMasks masks(const SeqList &q, int t0) {
     RowMasks m{0u, 0u, 0u};
-    if (q.offsets == nullptr || (sp.seq >= 0 && t0 >= sp.begin && t0 + L <= sp.next)) {
+    if (sp.seq >= 0 && t0 >= sp.begin && t0 + L <= sp.next) {
       if (t0 == sp.begin) m.start = 1u;
-      const int last = sp.next - 1 - t0;
-      if (last >= 0 && last < L) m.end = 1u << last;
-      const int rows = q.T - t0;
-      if (rows < L) m.none = rows <= 0 ? (1u << L) - 1u : ((1u << L) - 1u) & ~((1u << rows) - 1u);
+      if (sp.next == t0 + L) m.end = 1u << (L - 1);
       return m;
     }
     for (int j = 0; j < L; ++j) {
@@ -201,10 +284,6 @@ struct RowWalk {
   }
 };
 
-__device__ __forceinline__ int seq_index(const SeqList &q, int b, int t) {
-  return q.offsets ? seq_locate(q, t).seq : b;
-}
-
 __device__ __forceinline__ float2 load_state(const float *s, long long j, int C, int c, int c1, bool on0, bool on1) {
   return make_float2(on0 ? s[j * C + c] : 0.f, on1 ? s[j * C + c1] : 0.f);
 }
@@ -213,24 +292,30 @@ __device__ __forceinline__ void store_state(float *s, long long j, int C, int c,
   if (on1) s[j * C + c1] = v.y;
 }
 
-// A pair whose rows begin a sequence takes nothing from in front of it, whatever stands there (an
-// infinity times zero would not be zero): its P is -1, which no product of decays is, and stays -1
-// whatever it is multiplied by (a NaN would take the sign away).
+// Folding pairs.  PACKED: a pair whose rows begin a sequence takes nothing from in front of it, whatever
+// stands there (an infinity times zero would not be zero): its P is -1, which no product of decays is, and
+// stays -1 whatever it is multiplied by (a NaN would take the sign away).
 __device__ __forceinline__ bool cut(float2 P) { return __float_as_int(P.x) < 0; }
-__device__ __forceinline__ float2 join(float2 P, float2 Q) { return cut(P) || cut(Q) ? f2(-1.f) : mul2(P, Q); }
-__device__ __forceinline__ float2 apply(float2 P, float2 H, float2 h) { return cut(P) ? H : fma2(P, h, H); }
+template <bool PACKED> __device__ __forceinline__ float2 join(float2 P, float2 Q) {
+  return PACKED && (cut(P) || cut(Q)) ? f2(-1.f) : mul2(P, Q);
+}
+template <bool PACKED> __device__ __forceinline__ float2 apply(float2 P, float2 H, float2 h) {
+  return PACKED && cut(P) ? H : fma2(P, h, H);
+}
 
 // ---- thread-block clusters ---------------------------------------------------------------------
 
-__device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void store_peer(const void *mine, int rank, float4 v) {
   uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(mine)), "r"(rank));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
                : "memory");
 }
+
+// The warp's number, known to the compiler to be the same in all its lanes.
+__device__ __forceinline__ int uniform_warp() { return __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0); }
 
 struct RecParams {
   SeqList q;
@@ -239,68 +324,102 @@ struct RecParams {
 };
 
 // Sequences without a row: what enters leaves.
-__device__ __forceinline__ void empty_states(const RecParams &p, int b, int warp, const float *from, float *to, int c,
-                                             int c1, bool on0, bool on1) {
-  if (p.q.offsets == nullptr) {
-    if (p.q.T == 0 && warp == 0)
-      store_state(to, b, p.q.C, c, c1, on0, on1, from ? load_state(from, b, p.q.C, c, c1, on0, on1) : f2(0.f));
-    return;
-  }
+__device__ __forceinline__ void empty_states(const RecParams &p, int warp, const float *from, float *to, int c, int c1,
+                                             bool on0, bool on1) {
   for (int j = warp; j < p.q.S; j += REC_W)
     if (seq_bound(p.q, j) >= seq_bound(p.q, j + 1))
       store_state(to, j, p.q.C, c, c1, on0, on1, from ? load_state(from, j, p.q.C, c, c1, on0, on1) : f2(0.f));
 }
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(REC_THREADS)
-recurrence_forward_kernel(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v, const float *__restrict__ decay,
-                          const float *__restrict__ initial, T *__restrict__ y, float *__restrict__ fin,
-                          float *__restrict__ ckpt, RecParams p) {
-  using Q = Pair<T, VEC>;
-  constexpr int L = REC_L, W = REC_W;
-  __shared__ float4 agg[2][W][32];
-  __shared__ float4 far[2][REC_MAX_CLUSTER][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// Shared memory of a CTA: the staged rows (FAST), the warps' pairs (twice, for one barrier per tile),
+// backward the rows' decays, the tiles' pairs of the cluster (twice).
+constexpr int REC_PAIRS = 2 * REC_W * 32 * (int)sizeof(float4);
+template <typename T> constexpr int rec_stage_bytes(int tensors) {
+  return tensors * REC_TILE * REC_GROUP * (int)sizeof(T);
+}
+constexpr int REC_DECAYS = REC_TILE * REC_GROUP * (int)sizeof(float);
+inline size_t rec_smem(int stage, bool backward, int cs) {
+  return (size_t)stage + REC_PAIRS + (backward ? REC_PAIRS / 2 + REC_DECAYS : 0) + (cs > 1 ? 2 * cs * 32 * sizeof(float4) : 0);
+}
+
+// FAST: 16-byte rows, copied ahead; otherwise read where they are used, channels c and c + 32 per lane.
+template <typename T, bool FAST, bool PACKED, bool SERIES>
+__device__ __forceinline__ void forward_body(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v, const float *__restrict__ initial,
+             T *__restrict__ y, float *__restrict__ fin, float *__restrict__ ckpt, const RecParams &p, const Rate &k) {
+  using Q = Pair<T, FAST>;
+  constexpr int L = REC_L, W = REC_W, NT = 3;
+  extern __shared__ __align__(16) unsigned char smem[];
+  T *stage = reinterpret_cast<T *>(smem);
+  float4(*agg)[W][32] = reinterpret_cast<float4(*)[W][32]>(smem + (FAST ? rec_stage_bytes<T>(NT) : 0));
+  float4 *far = reinterpret_cast<float4 *>(agg + 2);  // [2][cs][32]
+  const int lane = threadIdx.x & 31, warp = uniform_warp();
   const int rank = (int)(blockIdx.x % p.cs);
   const long long pair = blockIdx.x / p.cs;
   const int grp = (int)(pair % p.groups), b = (int)(pair / p.groups);
-  const int C = p.q.C, c = Q::channel(grp, lane), c1 = VEC ? c + 1 : c + 32;
+  const int C = p.q.C, c = Q::channel(grp, lane), c1 = FAST ? c + 1 : c + 32;
   const bool on0 = c < C, on1 = c1 < C;
+  const int tiles = ceil_div(p.q.T, REC_TILE), steps = ceil_div(tiles, p.cs);
+  T *mine = stage + warp * (NT * L * REC_GROUP);
+  RowCopy<T> cx, cu, cv;
+  auto start_copies = [&](int tile) {
+    const int t = tile * REC_TILE + warp * L;
+    cx.start(t, p.q.T);
+    cu.start(t, p.q.T);
+    cv.start(t, p.q.T);
+  };
+  if constexpr (FAST) {
+    cx.init(x, mine, b, grp, C, lane);
+    cu.init(u, mine + L * REC_GROUP, b, grp, C, lane);
+    cv.init(v, mine + 2 * L * REC_GROUP, b, grp, C, lane);
+    if (steps > 0) start_copies(rank);
+  }
   if (p.cs > 1) {  // a peer's shared memory may be written once it runs
     cluster_arrive();
     cluster_wait();
   }
-  if (fin != nullptr && rank == 0) empty_states(p, b, warp, initial, fin, c, c1, on0, on1);
-  const float2 kz = make_float2(on0 ? p.scale * softplus(decay[c]) : 0.f,
-                                on1 ? p.scale * softplus(decay[c1]) : 0.f);
-  const bool series = __all_sync(0xffffffffu, kz.x <= REC_SERIES && kz.y <= REC_SERIES);
-  const int tiles = ceil_div(p.q.T, REC_TILE), steps = ceil_div(tiles, p.cs);
+  if (PACKED && fin != nullptr && rank == 0) empty_states(p, warp, initial, fin, c, c1, on0, on1);
   RowWalk walk;
-  walk.init(p.q, b);
   float2 carry = f2(0.f);
+  if (!PACKED && initial != nullptr) carry = load_state(initial, b, C, c, c1, on0, on1);
   for (int it = 0; it < steps; ++it) {
     const int tile = it * p.cs + rank, t0 = tile * REC_TILE + warp * L, half = it & 1;
-    const RowMasks m = walk.masks<L>(p.q, t0);
-    typename Q::Raw rx[L], ru[L], rv[L];
+    const int rows = p.q.T - t0;
+    RowMasks m{0u, 0u, 0u};
+    if (PACKED) m = walk.masks<L>(p.q, t0);
+    float2 a[L], bb[L], P = f2(1.f), H = f2(0.f);
     {
-      const T *px = x.row(b, t0) + c, *pu = u.row(b, t0) + c, *pv = v.row(b, t0) + c;
+      typename Q::Raw rx[L], ru[L], rv[L];
+      if constexpr (FAST) {
+        copies_done();
+        if (!PACKED && rows < L) close_rows<T>(mine + L * REC_GROUP, rows, lane);
+#pragma unroll
+        for (int j = 0; j < L; ++j) {
+          rx[j] = Q::P::load(mine + j * REC_GROUP + 2 * lane);
+          ru[j] = Q::P::load(mine + (L + j) * REC_GROUP + 2 * lane);
+          rv[j] = Q::P::load(mine + (2 * L + j) * REC_GROUP + 2 * lane);
+        }
+      } else {
+        const T *px = x.row(b, t0) + c, *pu = u.row(b, t0) + c, *pv = v.row(b, t0) + c;
+#pragma unroll
+        for (int j = 0; j < L; ++j) {
+          rx[j] = Q::load(px + j * x.rs, j < rows && on0, j < rows && on1);
+          ru[j] = Q::load(pu + j * u.rs, j < rows && on0, j < rows && on1);
+          if (!PACKED && j >= rows) ru[j] = Q::closed();
+          rv[j] = Q::load(pv + j * v.rs, j < rows && on0, j < rows && on1);
+        }
+      }
 #pragma unroll
       for (int j = 0; j < L; ++j) {
-        const bool in = !(m.none >> j & 1u);
-        rx[j] = Q::load(px + j * x.rs, in && on0, in && on1);
-        ru[j] = Q::load(pu + j * u.rs, in && on0, in && on1);
-        rv[j] = Q::load(pv + j * v.rs, in && on0, in && on1);
+        const float2 t = root_sigmoid2(Q::get(ru[j])), s = mul2(k.ks, mul2(t, t));
+        a[j] = keep2<SERIES>(s);
+        bb[j] = mul2(beta2<SERIES>(t, s, k), mul2(sigmoid2(Q::get(rv[j])), Q::get(rx[j])));
       }
     }
-    float2 a[L], bb[L], P = f2(1.f), H = f2(0.f);
-#pragma unroll
-    for (int j = 0; j < L; ++j) {
-      const Gates g = gates(Q::get(ru[j]), Q::get(rv[j]), kz, series);
-      const float2 q = beta_square2(g.d);
-      a[j] = keep2(mul2(kz, g.r), g.d, series);
-      bb[j] = mul2(mul2(q, make_float2(rsqf(q.x), rsqf(q.y))), mul2(g.i, Q::get(rx[j])));
+    if constexpr (FAST) {
+      __syncwarp();
+      if (it + 1 < steps) start_copies(tile + p.cs);
     }
-    if ((m.start | m.none) == 0u) {
+    if (!PACKED || (m.start | m.none) == 0u) {
 #pragma unroll
       for (int j = 0; j < L; ++j) {
         P = mul2(P, a[j]);
@@ -315,11 +434,11 @@ recurrence_forward_kernel(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v, const float *__res
           H = f2(0.f);
         } else if (m.start >> j & 1u) {
           if (initial != nullptr)
-            bb[j] = fma2(a[j], load_state(initial, seq_index(p.q, b, t0 + j), C, c, c1, on0, on1), bb[j]);
+            bb[j] = fma2(a[j], load_state(initial, seq_locate(p.q, t0 + j).seq, C, c, c1, on0, on1), bb[j]);
           P = f2(-1.f);
           H = bb[j];
         } else {
-          P = join(P, a[j]);
+          P = join<PACKED>(P, a[j]);
           H = fma2(a[j], H, bb[j]);
         }
       }
@@ -328,223 +447,262 @@ recurrence_forward_kernel(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v, const float *__res
     __syncthreads();
     float2 h = carry;
     if (p.cs > 1) {
-      // the CTA's pair, folded by as many warps as it has peers, one peer each
+      // the CTA's pair, folded by each of the warps that pass it on
+      float4 *there = far + (half * p.cs + rank) * 32 + lane;
       if (warp < p.cs) {
         float2 TP = f2(1.f), TH = f2(0.f);
 #pragma unroll
-        for (int k = 0; k < W; ++k) {
-          const float4 e = agg[half][k][lane];
+        for (int w = 0; w < W; ++w) {
+          const float4 e = agg[half][w][lane];
           const float2 P2 = make_float2(e.x, e.y), H2 = make_float2(e.z, e.w);
-          TH = apply(P2, H2, TH);
-          TP = join(TP, P2);
+          TH = apply<PACKED>(P2, H2, TH);
+          TP = join<PACKED>(TP, P2);
         }
-        store_peer(&far[half][rank][lane], warp, make_float4(TP.x, TP.y, TH.x, TH.y));
+        for (int peer = warp; peer < p.cs; peer += W) store_peer(there, peer, make_float4(TP.x, TP.y, TH.x, TH.y));
       }
       cluster_arrive();
       cluster_wait();
-      for (int k = 0; k < p.cs; ++k) {
-        if (k == rank) h = carry;
-        const float4 e = far[half][k][lane];
-        carry = apply(make_float2(e.x, e.y), make_float2(e.z, e.w), carry);
+      for (int w = 0; w < p.cs; ++w) {
+        if (w == rank) h = carry;
+        const float4 e = far[(half * p.cs + w) * 32 + lane];
+        carry = apply<PACKED>(make_float2(e.x, e.y), make_float2(e.z, e.w), carry);
       }
     }
     if (ckpt != nullptr && warp == 0 && tile < tiles)
       store_state(ckpt, (long long)b * tiles + tile, C, c, c1, on0, on1, h);
+    float2 in = h;
 #pragma unroll
-    for (int k = 0; k < W; ++k) {
-      if (p.cs > 1 && k == warp) break;
-      const float4 e = agg[half][k][lane];
-      if (k == warp) carry = h;  // cs 1: the state of this warp, while h runs on to the tile's end
-      h = apply(make_float2(e.x, e.y), make_float2(e.z, e.w), h);
+    for (int w = 0; w < W; ++w) {
+      if (w == warp) {
+        in = h;
+        if (p.cs > 1) break;
+      }
+      const float4 e = agg[half][w][lane];
+      h = apply<PACKED>(make_float2(e.x, e.y), make_float2(e.z, e.w), h);
     }
-    if (p.cs == 1) {
-      const float2 next = h;
-      h = carry;
-      carry = next;
-    }
-    T *py = y + ((long long)b * p.q.T + t0) * C + c;
+    if (p.cs == 1) carry = h;
+    h = in;
+    T *py = y + ((long long)b * p.q.T + t0) * C;
+    if (rows >= L && (!PACKED || (m.start | m.none | m.end) == 0u)) {
 #pragma unroll
-    for (int j = 0; j < L; ++j) {
-      h = ((m.start | m.none) >> j & 1u) ? bb[j] : fma2(a[j], h, bb[j]);
-      const bool in = t0 + j < p.q.T;
-      Q::store(py + (long long)j * C, h, in && on0, in && on1);
-      if ((m.end >> j & 1u) && fin != nullptr)
-        store_state(fin, seq_index(p.q, b, t0 + j), C, c, c1, on0, on1, h);
+      for (int j = 0; j < L; ++j) {
+        h = fma2(a[j], h, bb[j]);
+        Q::store(py + (unsigned)(j * C + c), h, on0, on1);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < L; ++j) {
+        h = PACKED && ((m.start | m.none) >> j & 1u) ? bb[j] : fma2(a[j], h, bb[j]);
+        Q::store(py + (unsigned)(j * C + c), h, j < rows && on0, j < rows && on1);
+        if (PACKED && (m.end >> j & 1u) && fin != nullptr)
+          store_state(fin, seq_locate(p.q, t0 + j).seq, C, c, c1, on0, on1, h);
+      }
     }
   }
+  if (!PACKED && fin != nullptr && rank == 0 && warp == 0) store_state(fin, b, C, c, c1, on0, on1, carry);
 }
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(REC_THREADS)
-recurrence_backward_kernel(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v, const float *__restrict__ decay,
-                           const float *__restrict__ initial, const float *__restrict__ ckpt, SeqIn<T> dy,
-                           const float *__restrict__ dfin, T *__restrict__ dx, T *__restrict__ du, T *__restrict__ dv,
-                           float *__restrict__ dinit, float *__restrict__ part, RecParams p) {
-  using Q = Pair<T, VEC>;
-  constexpr int L = REC_L, W = REC_W;
-  __shared__ float4 agg[2][W][32];   // P, H of each warp's rows
-  __shared__ float2 aggq[2][W][32];  // what leaves them towards earlier rows
-  __shared__ float4 far[2][REC_MAX_CLUSTER][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+template <typename T, bool FAST, bool PACKED, bool SERIES>
+__device__ __forceinline__ void backward_body(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v, const float *__restrict__ initial,
+              const float *__restrict__ ckpt, SeqIn<T> dy, const float *__restrict__ dfin, T *__restrict__ dx,
+              T *__restrict__ du, T *__restrict__ dv, float *__restrict__ dinit, float *__restrict__ part,
+              const RecParams &p, const Rate &k) {
+  using Q = Pair<T, FAST>;
+  constexpr int L = REC_L, W = REC_W, NT = 4;
+  extern __shared__ __align__(16) unsigned char smem[];
+  T *stage = reinterpret_cast<T *>(smem);
+  // P, H of each warp's rows, and what leaves them towards earlier rows
+  float4(*agg)[W][32] = reinterpret_cast<float4(*)[W][32]>(smem + (FAST ? rec_stage_bytes<T>(NT) : 0));
+  float2(*aggq)[W][32] = reinterpret_cast<float2(*)[W][32]>(agg + 2);
+  float2(*keep)[32] = reinterpret_cast<float2(*)[32]>(aggq + 2) + uniform_warp() * L;  // a of this warp's rows
+  float4 *far = reinterpret_cast<float4 *>(reinterpret_cast<float2(*)[32]>(aggq + 2) + W * L);  // [2][cs][32]
+  const int lane = threadIdx.x & 31, warp = uniform_warp();
   const int rank = (int)(blockIdx.x % p.cs);
   const long long pair = blockIdx.x / p.cs;
   const int grp = (int)(pair % p.groups), b = (int)(pair / p.groups);
-  const int C = p.q.C, c = Q::channel(grp, lane), c1 = VEC ? c + 1 : c + 32;
+  const int C = p.q.C, c = Q::channel(grp, lane), c1 = FAST ? c + 1 : c + 32;
   const bool on0 = c < C, on1 = c1 < C;
+  const int tiles = ceil_div(p.q.T, REC_TILE), steps = ceil_div(tiles, p.cs);
+  T *mine = stage + warp * (NT * L * REC_GROUP);
+  RowCopy<T> cx, cu, cv, cg;
+  auto start_copies = [&](int tile) {
+    const int t = tile * REC_TILE + warp * L;
+    cx.start(t, p.q.T);
+    cu.start(t, p.q.T);
+    cv.start(t, p.q.T);
+    cg.start(t, p.q.T);
+  };
+  if constexpr (FAST) {
+    cx.init(x, mine, b, grp, C, lane);
+    cu.init(u, mine + L * REC_GROUP, b, grp, C, lane);
+    cv.init(v, mine + 2 * L * REC_GROUP, b, grp, C, lane);
+    cg.init(dy, mine + 3 * L * REC_GROUP, b, grp, C, lane);
+    if (steps > 0) start_copies((steps - 1) * p.cs + rank);
+  }
   if (p.cs > 1) {
     cluster_arrive();
     cluster_wait();
   }
-  if (dinit != nullptr && rank == 0) empty_states(p, b, warp, dfin, dinit, c, c1, on0, on1);
-  const float2 kz = make_float2(on0 ? p.scale * softplus(decay[c]) : 0.f,
-                                on1 ? p.scale * softplus(decay[c1]) : 0.f);
-  const bool series = __all_sync(0xffffffffu, kz.x <= REC_SERIES && kz.y <= REC_SERIES);
-  const int tiles = ceil_div(p.q.T, REC_TILE), steps = ceil_div(tiles, p.cs);
+  if (PACKED && dinit != nullptr && rank == 0) empty_states(p, warp, dfin, dinit, c, c1, on0, on1);
   RowWalk walk;
-  walk.init(p.q, b);
   float2 carry = f2(0.f), ddecay = f2(0.f);
+  if (!PACKED && dfin != nullptr) carry = load_state(dfin, b, C, c, c1, on0, on1);
   for (int it = steps - 1; it >= 0; --it) {
     const int tile = it * p.cs + rank, t0 = tile * REC_TILE + warp * L, half = it & 1;
-    const RowMasks m = walk.masks<L>(p.q, t0);
+    const int rows = p.q.T - t0;
+    RowMasks mk{0u, 0u, 0u};
+    if (PACKED) mk = walk.masks<L>(p.q, t0);
+    const unsigned special = mk.start | mk.none;
+    float2 h = f2(0.f);
+    if (tile < tiles) h = load_state(ckpt, (long long)b * tiles + tile, C, c, c1, on0, on1);
     typename Q::Raw rx[L];
-    float2 r[L], i[L], d[L], g[L];
+    float2 t[L], i[L], g[L];
     {
       typename Q::Raw ru[L], rv[L], rg[L];
-      const T *px = x.row(b, t0) + c, *pu = u.row(b, t0) + c, *pv = v.row(b, t0) + c, *pg = dy.row(b, t0) + c;
+      if constexpr (FAST) {
+        copies_done();
+        if (!PACKED && rows < L) close_rows<T>(mine + L * REC_GROUP, rows, lane);
 #pragma unroll
-      for (int j = 0; j < L; ++j) {
-        const bool in = !(m.none >> j & 1u);
-        rx[j] = Q::load(px + j * x.rs, in && on0, in && on1);
-        ru[j] = Q::load(pu + j * u.rs, in && on0, in && on1);
-        rv[j] = Q::load(pv + j * v.rs, in && on0, in && on1);
-        rg[j] = Q::load(pg + j * dy.rs, in && on0, in && on1);
+        for (int j = 0; j < L; ++j) {
+          rx[j] = Q::P::load(mine + j * REC_GROUP + 2 * lane);
+          ru[j] = Q::P::load(mine + (L + j) * REC_GROUP + 2 * lane);
+          rv[j] = Q::P::load(mine + (2 * L + j) * REC_GROUP + 2 * lane);
+          rg[j] = Q::P::load(mine + (3 * L + j) * REC_GROUP + 2 * lane);
+        }
+      } else {
+        const T *px = x.row(b, t0) + c, *pu = u.row(b, t0) + c, *pv = v.row(b, t0) + c, *pg = dy.row(b, t0) + c;
+#pragma unroll
+        for (int j = 0; j < L; ++j) {
+          rx[j] = Q::load(px + j * x.rs, j < rows && on0, j < rows && on1);
+          ru[j] = Q::load(pu + j * u.rs, j < rows && on0, j < rows && on1);
+          if (!PACKED && j >= rows) ru[j] = Q::closed();
+          rv[j] = Q::load(pv + j * v.rs, j < rows && on0, j < rows && on1);
+          rg[j] = Q::load(pg + j * dy.rs, j < rows && on0, j < rows && on1);
+        }
       }
 #pragma unroll
       for (int j = 0; j < L; ++j) {
-        const Gates gt = gates(Q::get(ru[j]), Q::get(rv[j]), kz, series);
-        r[j] = gt.r;
-        i[j] = gt.i;
-        d[j] = gt.d;
+        if (PACKED && (mk.none >> j & 1u)) rx[j] = ru[j] = rv[j] = rg[j] = Q::zero();
+        t[j] = root_sigmoid2(Q::get(ru[j]));
+        i[j] = sigmoid2(Q::get(rv[j]));
         g[j] = Q::get(rg[j]);
       }
     }
-    float2 h = f2(0.f);
-    if (tile < tiles) h = load_state(ckpt, (long long)b * tiles + tile, C, c, c1, on0, on1);
-    const unsigned special = m.start | m.none;
-    if (m.end != 0u && dfin != nullptr) {
+    if constexpr (FAST) {
+      __syncwarp();
+      if (it > 0) start_copies(tile - p.cs);
+    }
+    if (PACKED && mk.end != 0u && dfin != nullptr) {
 #pragma unroll
       for (int j = 0; j < L; ++j)
-        if (m.end >> j & 1u)
-          g[j] = add2(g[j], load_state(dfin, seq_index(p.q, b, t0 + j), C, c, c1, on0, on1));
+        if (mk.end >> j & 1u)
+          g[j] = add2(g[j], load_state(dfin, seq_locate(p.q, t0 + j).seq, C, c, c1, on0, on1));
     }
-    // what the rows do to a state going down, and to a gradient going up
-    auto input = [&](int j, float2 &q, float2 &rs) {
-      q = beta_square2(d[j]);
-      rs = make_float2(rsqf(q.x), rsqf(q.y));
-      return mul2(i[j], Q::get(rx[j]));
-    };
+    // what the rows do to a state going down (P, H), and what they pass to a gradient going up
+    // (G = sum_j a[0] .. a[j] g[j], up to the first row that begins a sequence)
     float2 P = f2(1.f), H = f2(0.f), G = f2(0.f);
 #pragma unroll
     for (int j = 0; j < L; ++j) {
-      float2 q, rs;
-      const float2 ix = input(j, q, rs);
-      const float2 a = keep2(mul2(kz, r[j]), d[j], series);
-      float2 bb = mul2(mul2(q, rs), ix);
-      if (special >> j & 1u) {
-        if (m.none >> j & 1u) bb = f2(0.f);
+      const float2 s = mul2(k.ks, mul2(t[j], t[j])), a = keep2<SERIES>(s);
+      keep[j][lane] = a;
+      float2 bb = mul2(beta2<SERIES>(t[j], s, k), mul2(i[j], Q::get(rx[j])));
+      if (PACKED && (special >> j & 1u)) {
+        if (mk.none >> j & 1u) bb = f2(0.f);
         else if (initial != nullptr)
-          bb = fma2(a, load_state(initial, seq_index(p.q, b, t0 + j), C, c, c1, on0, on1), bb);
+          bb = fma2(a, load_state(initial, seq_locate(p.q, t0 + j).seq, C, c, c1, on0, on1), bb);
         P = f2(-1.f);
         H = bb;
       } else {
-        P = special ? join(P, a) : mul2(P, a);
+        P = join<PACKED>(P, a);
         H = fma2(a, H, bb);
+        if (!PACKED || !cut(P)) G = fma2(P, g[j], G);
       }
     }
 #pragma unroll
-    for (int j = L - 1; j >= 0; --j) {
-      const float2 a = keep2(mul2(kz, r[j]), d[j], series);
-      G = (special >> j & 1u) ? f2(0.f) : mul2(a, add2(g[j], G));
+    for (int j = 0; j < L; ++j) {
+      forget(t[j]);
+      forget(i[j]);
     }
     agg[half][warp][lane] = make_float4(P.x, P.y, H.x, H.y);
     aggq[half][warp][lane] = G;
     __syncthreads();
     float2 q = carry;
     if (p.cs > 1) {
+      float4 *there = far + (half * p.cs + rank) * 32 + lane;
       if (warp < p.cs) {
         float2 TP = f2(1.f), TG = f2(0.f);
 #pragma unroll
-        for (int k = W - 1; k >= 0; --k) {
-          const float4 e = agg[half][k][lane];
-          const float2 P2 = make_float2(e.x, e.y), G2 = aggq[half][k][lane];
-          TG = apply(P2, G2, TG);
-          TP = join(TP, P2);
+        for (int w = W - 1; w >= 0; --w) {
+          const float4 e = agg[half][w][lane];
+          const float2 P2 = make_float2(e.x, e.y);
+          TG = apply<PACKED>(P2, aggq[half][w][lane], TG);
+          TP = join<PACKED>(TP, P2);
         }
-        store_peer(&far[half][rank][lane], warp, make_float4(TP.x, TP.y, TG.x, TG.y));
+        for (int peer = warp; peer < p.cs; peer += W) store_peer(there, peer, make_float4(TP.x, TP.y, TG.x, TG.y));
       }
       cluster_arrive();
       cluster_wait();
-      for (int k = p.cs - 1; k >= 0; --k) {
-        if (k == rank) q = carry;
-        const float4 e = far[half][k][lane];
-        carry = apply(make_float2(e.x, e.y), make_float2(e.z, e.w), carry);
+      for (int w = p.cs - 1; w >= 0; --w) {
+        if (w == rank) q = carry;
+        const float4 e = far[(half * p.cs + w) * 32 + lane];
+        carry = apply<PACKED>(make_float2(e.x, e.y), make_float2(e.z, e.w), carry);
       }
     }
+    float2 in = q;
 #pragma unroll
-    for (int k = W - 1; k >= 0; --k) {
-      if (p.cs > 1 && k == warp) break;
-      if (k == warp) carry = q;
-      const float4 e = agg[half][k][lane];
-      q = apply(make_float2(e.x, e.y), aggq[half][k][lane], q);
+    for (int w = W - 1; w >= 0; --w) {
+      if (w == warp) {
+        in = q;
+        if (p.cs > 1) break;
+      }
+      const float4 e = agg[half][w][lane];
+      q = apply<PACKED>(make_float2(e.x, e.y), aggq[half][w][lane], q);
     }
-    if (p.cs == 1) {
-      const float2 next = q;
-      q = carry;
-      carry = next;
-    }
-    for (int k = 0; k < warp; ++k) {
-      const float4 e = agg[half][k][lane];
-      h = apply(make_float2(e.x, e.y), make_float2(e.z, e.w), h);
+    if (p.cs == 1) carry = q;
+    q = in;
+    for (int w = 0; w < warp; ++w) {
+      const float4 e = agg[half][w][lane];
+      h = apply<PACKED>(make_float2(e.x, e.y), make_float2(e.z, e.w), h);
     }
 #pragma unroll
     for (int j = L - 1; j >= 0; --j) {
-      const float2 a = keep2(mul2(kz, r[j]), d[j], series);
       g[j] = add2(g[j], q);
-      q = mul2(a, g[j]);
-      if (special >> j & 1u) {
-        if ((m.start >> j & 1u) && dinit != nullptr)
-          store_state(dinit, seq_index(p.q, b, t0 + j), C, c, c1, on0, on1, q);
+      q = mul2(keep[j][lane], g[j]);
+      if (PACKED && (special >> j & 1u)) {
+        if ((mk.start >> j & 1u) && dinit != nullptr)
+          store_state(dinit, seq_locate(p.q, t0 + j).seq, C, c, c1, on0, on1, q);
         q = f2(0.f);
       }
     }
-    const long long at = ((long long)b * p.q.T + t0) * C + c;
+    const long long at = ((long long)b * p.q.T + t0) * C;
+    T *px = dx + at, *pu = du + at, *pv = dv + at;
     float2 sum = f2(0.f);
 #pragma unroll
     for (int j = 0; j < L; ++j) {
-      float2 bq, rs;
-      const float2 ix = input(j, bq, rs);
-      const float2 a = keep2(mul2(kz, r[j]), d[j], series), beta = mul2(bq, rs);
-      if (special >> j & 1u) {
+      const float2 a = keep[j][lane], r = mul2(t[j], t[j]), s = mul2(k.ks, r);
+      const float2 beta = beta2<SERIES>(t[j], s, k), rho = rho2<SERIES>(t[j], s, k);
+      const float2 xv = Q::get(rx[j]), ix = mul2(i[j], xv);
+      if (PACKED && (special >> j & 1u)) {
         h = f2(0.f);
-        if ((m.start >> j & 1u) && initial != nullptr)
-          h = load_state(initial, seq_index(p.q, b, t0 + j), C, c, c1, on0, on1);
-        if (m.none >> j & 1u) g[j] = f2(0.f);
+        if ((mk.start >> j & 1u) && initial != nullptr)
+          h = load_state(initial, seq_locate(p.q, t0 + j).seq, C, c, c1, on0, on1);
+        if (mk.none >> j & 1u) g[j] = f2(0.f);
       }
       const float2 ddx = mul2(g[j], mul2(beta, i[j]));
-      const float2 ddv = mul2(mul2(ddx, Q::get(rx[j])), add2(f2(1.f), neg2(i[j])));
-      // dz / g = a (a / beta i x - h[t-1])
-      const float2 dz = mul2(mul2(g[j], a), fma2(mul2(a, rs), ix, neg2(h)));
-      const float2 z = mul2(kz, r[j]);
-      const float2 ddu = mul2(mul2(dz, z), add2(f2(1.f), neg2(r[j])));
-      sum = fma2(dz, r[j], sum);
+      const float2 ddv = mul2(mul2(ddx, xv), one_minus2(i[j]));
+      const float2 dzz = mul2(mul2(g[j], a), fma2(mul2(a, rho), ix, mul2(s, h)));
+      const float2 ddu = mul2(dzz, one_minus2(r));
+      sum = add2(sum, dzz);
       h = fma2(a, h, mul2(beta, ix));
-      const bool in = t0 + j < p.q.T;
-      Q::store(dx + at + (long long)j * C, ddx, in && on0, in && on1);
-      Q::store(du + at + (long long)j * C, ddu, in && on0, in && on1);
-      Q::store(dv + at + (long long)j * C, ddv, in && on0, in && on1);
+      const bool live = j < rows;
+      const unsigned o = (unsigned)(j * C + c);
+      Q::store(px + o, ddx, live && on0, live && on1);
+      Q::store(pu + o, ddu, live && on0, live && on1);
+      Q::store(pv + o, ddv, live && on0, live && on1);
     }
     ddecay = add2(ddecay, sum);
   }
+  if (!PACKED && dinit != nullptr && rank == 0 && warp == 0) store_state(dinit, b, C, c, c1, on0, on1, carry);
   // this CTA's part of ddecay: the warps' sums in order
   __syncthreads();
   aggq[0][warp][lane] = ddecay;
@@ -552,9 +710,46 @@ recurrence_backward_kernel(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v, const float *__re
   if (warp == 0) {
     float2 s = aggq[0][0][lane];
 #pragma unroll
-    for (int k = 1; k < W; ++k) s = add2(s, aggq[0][k][lane]);
+    for (int w = 1; w < W; ++w) s = add2(s, aggq[0][w][lane]);
     store_state(part, (long long)b * p.cs + rank, C, c, c1, on0, on1, s);
   }
+}
+
+// Of this lane's channels, 0 beyond the last.
+__device__ __forceinline__ Rate rate_of(const float *decay, float scale, int c, int c1, bool on0, bool on1) {
+  const float2 k = make_float2(on0 ? scale * softplus(decay[c]) : 0.f, on1 ? scale * softplus(decay[c1]) : 0.f);
+  return Rate{make_float2(-k.x, -k.y), make_float2(sqrtf(2.f * k.x), sqrtf(2.f * k.y))};
+}
+template <typename T, bool FAST> __device__ __forceinline__ Rate cta_rate(const float *decay, const RecParams &p) {
+  const int grp = (int)(blockIdx.x / p.cs % p.groups), c = Pair<T, FAST>::channel(grp, threadIdx.x & 31);
+  const int c1 = FAST ? c + 1 : c + 32;
+  return rate_of(decay, p.scale, c, c1, c < p.q.C, c1 < p.q.C);
+}
+
+template <typename T, bool FAST, bool PACKED>
+__global__ void __launch_bounds__(REC_THREADS, 3)
+recurrence_forward_kernel(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v, const float *__restrict__ decay,
+                          const float *__restrict__ initial, T *__restrict__ y, float *__restrict__ fin,
+                          float *__restrict__ ckpt, RecParams p) {
+  const Rate k = cta_rate<T, FAST>(decay, p);
+  // the same in every warp of the CTA: they have its channels in common
+  if (__all_sync(0xffffffffu, k.ks.x >= -REC_SERIES && k.ks.y >= -REC_SERIES))
+    forward_body<T, FAST, PACKED, true>(x, u, v, initial, y, fin, ckpt, p, k);
+  else
+    forward_body<T, FAST, PACKED, false>(x, u, v, initial, y, fin, ckpt, p, k);
+}
+
+template <typename T, bool FAST, bool PACKED>
+__global__ void __launch_bounds__(REC_THREADS, 2)
+recurrence_backward_kernel(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v, const float *__restrict__ decay,
+                           const float *__restrict__ initial, const float *__restrict__ ckpt, SeqIn<T> dy,
+                           const float *__restrict__ dfin, T *__restrict__ dx, T *__restrict__ du, T *__restrict__ dv,
+                           float *__restrict__ dinit, float *__restrict__ part, RecParams p) {
+  const Rate k = cta_rate<T, FAST>(decay, p);
+  if (__all_sync(0xffffffffu, k.ks.x >= -REC_SERIES && k.ks.y >= -REC_SERIES))
+    backward_body<T, FAST, PACKED, true>(x, u, v, initial, ckpt, dy, dfin, dx, du, dv, dinit, part, p, k);
+  else
+    backward_body<T, FAST, PACKED, false>(x, u, v, initial, ckpt, dy, dfin, dx, du, dv, dinit, part, p, k);
 }
 
 template <typename T, bool VEC>
@@ -573,49 +768,70 @@ recurrence_step_kernel(const T *__restrict__ x, long long xs, const T *__restric
   const typename Q::Raw rx = Q::load(x + b * xs + c, on0, on1), ru = Q::load(u + b * us + c, on0, on1),
                         rv = Q::load(v + b * vs + c, on0, on1);
   const float2 h0 = load_state(state, b, C, c, c1, on0, on1);
-  const float2 kz = make_float2(on0 ? p.scale * softplus(decay[c]) : 0.f,
-                                on1 ? p.scale * softplus(decay[c1]) : 0.f);
-  const Gates g = gates(Q::get(ru), Q::get(rv), kz, false);
-  const float2 q = beta_square2(g.d);
-  const float2 bb = mul2(mul2(q, make_float2(rsqf(q.x), rsqf(q.y))), mul2(g.i, Q::get(rx)));
-  const float2 h = fma2(keep2(mul2(kz, g.r), g.d, false), h0, bb);
+  const Rate k = rate_of(decay, p.scale, c, c1, on0, on1);
+  const float2 t = root_sigmoid2(Q::get(ru)), sz = mul2(k.ks, mul2(t, t));
+  const float2 bb = mul2(beta2<false>(t, sz, k), mul2(sigmoid2(Q::get(rv)), Q::get(rx)));
+  const float2 h = fma2(keep2<false>(sz), h0, bb);
   store_state(state, b, C, c, c1, on0, on1, h);
   Q::store(y + b * C + c, h, on0, on1);
 }
 
 // ---- host --------------------------------------------------------------------------------------
 
-// CTAs of a cluster along T: as many (a power of two, never more than there are tiles) as give every SM
-// two CTAs.
-inline int rec_cluster(const dwconv_b200_sequence &s) {
-  const long long ctas = (long long)ceil_div(s.C, REC_GROUP) * s.B;
+// CTAs of a cluster along T (a power of two, never more than there are tiles): the choice whose rounds of
+// resident CTAs, each a start-up worth about two tiles and its tiles, take least; a cluster's exchange
+// counts as a quarter of a tile and what it folds.
+inline int rec_cluster(const dwconv_b200_sequence &s, bool backward) {
+  const long long pairs = (long long)ceil_div(s.C, REC_GROUP) * s.B, slots = 148 * (backward ? 2 : 3);
   const int tiles = ceil_div(s.T, REC_TILE);
-  int cs = 1;
-  while (cs < REC_MAX_CLUSTER && cs * 2 <= tiles && ctas * cs < 2 * 148) cs <<= 1;
-  return cs;
+  int best = 1;
+  long long cost = 0;
+  for (int cs = 1; cs <= REC_MAX_CLUSTER && (cs == 1 || cs <= tiles); cs <<= 1) {
+    const long long c = ceil_div_ll(pairs * cs, slots) * (2 * 64 + (long long)ceil_div(tiles, cs) * (cs > 1 ? 80 + cs : 64));
+    if (cs == 1 || c < cost) {
+      best = cs;
+      cost = c;
+    }
+  }
+  return best;
 }
 
-inline RecParams rec_params(const dwconv_b200_sequence &s, float scale) {
+inline RecParams rec_params(const dwconv_b200_sequence &s, float scale, bool backward) {
   RecParams p;
   p.q = seq_list(s);
   p.B = s.B;
   p.groups = ceil_div(s.C, REC_GROUP);
-  p.cs = rec_cluster(s);
+  p.cs = rec_cluster(s, backward);
   p.scale = scale;
   return p;
 }
 
-inline cudaLaunchConfig_t rec_config(const RecParams &p, cudaLaunchAttribute *attr, cudaStream_t st) {
+// Launches `kernel` in clusters of p.cs CTAs.  The attributes that this takes are set once per kernel and
+// device.
+template <typename... K, typename... A>
+void rec_launch(void (*kernel)(K...), std::atomic<unsigned long long> &ready, const RecParams &p, size_t most_smem,
+                size_t smem, cudaStream_t st, A... args) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (!(ready.load(std::memory_order_acquire) & bit)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most_smem) != cudaSuccess ||
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+      return;  // the caller finds the error
+    ready.fetch_or(bit, std::memory_order_release);
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)((long long)p.groups * p.B * p.cs));
   cfg.blockDim = dim3(REC_THREADS);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
+  cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)p.cs;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = p.cs > 1 ? 1 : 0;
-  return cfg;
+  (void)cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 struct RecArgs {
@@ -628,37 +844,43 @@ struct RecArgs {
   float scale;
 };
 
-inline bool rec_vector(const RecArgs &a, size_t es) {
+// Whether all rows start on 16 bytes.
+inline bool rec_fast(const RecArgs &a, size_t es) {
+  const int E = (int)(16 / es);
   const void *ptrs[] = {a.y, a.dx, a.du, a.dv};
   for (const void *q : ptrs)
-    if (q != nullptr && !aligned_to(q, 2 * es)) return false;
-  return a.s->C % 2 == 0 && rows_vector(*a.x, 2, es) && rows_vector(*a.u, 2, es) && rows_vector(*a.v, 2, es) &&
-         (a.dy == nullptr || rows_vector(*a.dy, 2, es));
+    if (q != nullptr && !aligned_to(q, 16)) return false;
+  return a.s->C % E == 0 && rows_vector(*a.x, E, es) && rows_vector(*a.u, E, es) && rows_vector(*a.v, E, es) &&
+         (a.dy == nullptr || rows_vector(*a.dy, E, es));
 }
 
-template <typename T, bool VEC> cudaError_t launch_forward(const RecArgs &a, cudaStream_t st) {
-  const RecParams p = rec_params(*a.s, a.scale);
-  cudaLaunchAttribute attr[1];
-  const cudaLaunchConfig_t cfg = rec_config(p, attr, st);
-  return cudaLaunchKernelEx(&cfg, recurrence_forward_kernel<T, VEC>, seq_in<T>(*a.x), seq_in<T>(*a.u),
-                            seq_in<T>(*a.v), a.decay, a.initial, static_cast<T *>(a.y), a.fin, a.ckpt, p);
+template <typename T, bool FAST, bool PACKED> void launch_forward(const RecArgs &a, cudaStream_t st) {
+  static std::atomic<unsigned long long> ready{0};
+  const RecParams p = rec_params(*a.s, a.scale, false);
+  const int stage = FAST ? rec_stage_bytes<T>(3) : 0;
+  rec_launch(recurrence_forward_kernel<T, FAST, PACKED>, ready, p, rec_smem(stage, false, REC_MAX_CLUSTER),
+             rec_smem(stage, false, p.cs), st, seq_in<T>(*a.x), seq_in<T>(*a.u), seq_in<T>(*a.v), a.decay, a.initial,
+             static_cast<T *>(a.y), a.fin, a.ckpt, p);
 }
-template <typename T, bool VEC> cudaError_t launch_backward(const RecArgs &a, cudaStream_t st) {
-  const RecParams p = rec_params(*a.s, a.scale);
-  cudaLaunchAttribute attr[1];
-  const cudaLaunchConfig_t cfg = rec_config(p, attr, st);
-  return cudaLaunchKernelEx(&cfg, recurrence_backward_kernel<T, VEC>, seq_in<T>(*a.x), seq_in<T>(*a.u),
-                            seq_in<T>(*a.v), a.decay, a.initial, a.ckpt_in, seq_in<T>(*a.dy), a.dfin,
-                            static_cast<T *>(a.dx), static_cast<T *>(a.du), static_cast<T *>(a.dv), a.dinit, a.part, p);
+template <typename T, bool FAST, bool PACKED> void launch_backward(const RecArgs &a, cudaStream_t st) {
+  static std::atomic<unsigned long long> ready{0};
+  const RecParams p = rec_params(*a.s, a.scale, true);
+  const int stage = FAST ? rec_stage_bytes<T>(4) : 0;
+  rec_launch(recurrence_backward_kernel<T, FAST, PACKED>, ready, p, rec_smem(stage, true, REC_MAX_CLUSTER),
+             rec_smem(stage, true, p.cs), st, seq_in<T>(*a.x), seq_in<T>(*a.u), seq_in<T>(*a.v), a.decay, a.initial,
+             a.ckpt_in, seq_in<T>(*a.dy), a.dfin, static_cast<T *>(a.dx), static_cast<T *>(a.du),
+             static_cast<T *>(a.dv), a.dinit, a.part, p);
 }
 
 template <typename T> void forward_t(const RecArgs &a, cudaStream_t st) {
-  if (rec_vector(a, sizeof(T))) launch_forward<T, true>(a, st);
-  else launch_forward<T, false>(a, st);
+  const bool packed = a.s->offsets != nullptr;
+  if (rec_fast(a, sizeof(T))) packed ? launch_forward<T, true, true>(a, st) : launch_forward<T, true, false>(a, st);
+  else packed ? launch_forward<T, false, true>(a, st) : launch_forward<T, false, false>(a, st);
 }
 template <typename T> void backward_t(const RecArgs &a, cudaStream_t st) {
-  if (rec_vector(a, sizeof(T))) launch_backward<T, true>(a, st);
-  else launch_backward<T, false>(a, st);
+  const bool packed = a.s->offsets != nullptr;
+  if (rec_fast(a, sizeof(T))) packed ? launch_backward<T, true, true>(a, st) : launch_backward<T, true, false>(a, st);
+  else packed ? launch_backward<T, false, true>(a, st) : launch_backward<T, false, false>(a, st);
 }
 
 template <typename T>
@@ -698,7 +920,7 @@ size_t dwconv_b200_recurrence_checkpoint_bytes(const dwconv_b200_sequence *seq) 
 
 size_t dwconv_b200_recurrence_workspace_bytes(const dwconv_b200_sequence *seq) {
   if (check_recurrence(DWCONV_B200_F32, seq) != DWCONV_B200_OK) return 0;
-  const size_t n = (size_t)seq->B * rec_cluster(*seq) * seq->C * sizeof(float);
+  const size_t n = (size_t)seq->B * rec_cluster(*seq, true) * seq->C * sizeof(float);
   return (n + 15) / 16 * 16 + 16;
 }
 
@@ -756,8 +978,8 @@ int dwconv_b200_recurrence_backward(const dwconv_b200_rows *x, const dwconv_b200
   }
   e = api_launch_status();
   if (e) return e;
-  launch_column_sum(a.part, (long long)seq->B * rec_cluster(*seq), seq->C,
-                    ColumnSumOut{ddecay, nullptr, DWCONV_B200_F32, seq->C, 1, decay, scale}, st);
+  launch_column_sum(a.part, (long long)seq->B * rec_cluster(*seq, true), seq->C,
+                    ColumnSumOut{ddecay, nullptr, DWCONV_B200_F32, seq->C, 1, decay}, st);
   return api_launch_status();
 }
 
@@ -774,7 +996,7 @@ int dwconv_b200_recurrence_step(const void *x, long long x_stride, const void *u
   if (!aligned_to(x, es) || !aligned_to(u, es) || !aligned_to(v, es) || !aligned_to(decay, 4) ||
       !aligned_to(state, 4) || !aligned_to(y, es))
     return DWCONV_B200_MISALIGNED;
-  const RecParams p = rec_params(s, scale);
+  const RecParams p = rec_params(s, scale, false);
   cudaStream_t st = (cudaStream_t)stream;
   switch (dtype) {
     case DWCONV_B200_F32: step_t<float>(x, x_stride, u, u_stride, v, v_stride, decay, state, y, p, st); break;
