@@ -19,11 +19,12 @@ int rows_conv_f16_take_error();   // rows_conv_f16.cu
 int rows_conv_bf16_take_error();  // rows_conv_bf16.cu
 int tiles_tma_take_error();      // tiles_tma.cu
 int nhwc_tma_take_error();       // nhwc_tma.cu
+int seq_take_error();            // seq_recurrence.cu
 
 int rows_conv_take_error() {
   return conv_take_error_here() | rows_conv_f16_take_error() | rows_conv_bf16_take_error() |
          rows_conv_epi_take_error() | rows_bigk_take_error() |
-         tiles_tma_take_error() | nhwc_tma_take_error();
+         tiles_tma_take_error() | nhwc_tma_take_error() | seq_take_error();
 }
 
 template int rows_forward<float>(const float *, const float *, float *, const Shape &, cudaStream_t);

@@ -20,22 +20,29 @@
 // P h + H.  Pairs meet in shared memory, every warp folds those in front of it onto the state that
 // enters the tile, and walks its rows once more from registers.  Tiles follow one another along T.
 // Where there are too few (channel block, batch) pairs to fill the device evenly, a cluster of CTAs takes
-// neighbouring tiles together and passes its tiles' pairs through distributed shared memory: one
-// cluster barrier per CTAs * W * L rows, no second pass over the data for it, and the same order of
-// operations on every run.
+// neighbouring tiles together and passes its tiles' pairs on by asynchronous stores to distributed
+// shared memory, which signal the receiving CTA's barrier themselves (a cluster-wide barrier with its
+// memory fence cost a fifth of the time): no second pass over the data, and the same order of operations
+// on every run.
 //
-// A warp copies the rows of its next tile to shared memory by 16-byte asynchronous copies as soon
-// as those of the current one are in registers, so that the barriers, folds and stores run under
-// them.  Tensors without 16-byte rows are read two elements per lane instead, without copies ahead.
+// A warp has the rows of its next tile copied to shared memory by tensor copies (TMA, one box of L rows
+// by 64 channels per tensor; what lies outside the tensor arrives as zeros) as soon as those of the
+// current one are in registers, so that the barriers, folds and stores run under them.  Tensors that the
+// copy engine cannot address (rows off 16-byte boundaries) are read two elements per lane instead, without
+// copies ahead.
 //
 // The forward pass keeps the fp32 state that enters each tile (1 / (W L) of the rows); the backward
 // pass starts from it, so it reads y nowhere and its h[t-1] have not been rounded to the data's type.
 #include <atomic>
 
+#include "rows_engine.cuh"
 #include "seq_common.cuh"
+#include "tensor_map.cuh"
 
 namespace dwb {
 namespace {
+
+__device__ int g_seq_error_flag;  // raised by a wait that ran out
 
 constexpr int REC_L = 8, REC_W = 8, REC_TILE = REC_L * REC_W, REC_GROUP = 64;
 constexpr int REC_THREADS = REC_W * 32;
@@ -156,97 +163,91 @@ __device__ __forceinline__ float softplus(float v) { return v > 20.f ? v : log1p
 
 // ---- channel pairs of a lane -------------------------------------------------------------------
 
-// VEC: channels c, c + 1, one load.  Otherwise (odd C, odd strides) channels c and c + 32, one each.
+// VEC: channels c, c + 1, one load.  Otherwise (odd C, odd strides) channels c0 and c1 = c0 + 32, one each.
+// Lanes beyond the last channel work on the last one too, and store the same values to the same places:
+// no access needs a test.
+struct Chan {
+  int c0, c1;
+};
 template <typename T, bool VEC> struct Pair;
 template <typename T> struct Pair<T, true> {
   using P = Pack<T, 2>;
   using Raw = typename P::Raw;
-  static __device__ __forceinline__ int channel(int g, int lane) { return g * REC_GROUP + 2 * lane; }
+  static __device__ __forceinline__ Chan channels(int g, int lane, int C) {
+    const int c = min(g * REC_GROUP + 2 * lane, C - 2);
+    return Chan{c, c + 1};
+  }
   static __device__ __forceinline__ Raw zero() { return P::zero(); }
   static __device__ __forceinline__ Raw closed() {
     const float f[2] = {-__int_as_float(0x7f800000), -__int_as_float(0x7f800000)};
     return P::pack(f);
   }
-  static __device__ __forceinline__ Raw load(const T *p, bool on0, bool) {
-    return on0 ? P::load(p) : P::zero();
-  }
+  static __device__ __forceinline__ Raw load(const T *row, const Chan &c) { return P::load(row + c.c0); }
   static __device__ __forceinline__ float2 get(const Raw &r) {
     float f[2];
     P::unpack(r, f);
     return make_float2(f[0], f[1]);
   }
-  static __device__ __forceinline__ void store(T *p, float2 v, bool on0, bool) {
+  static __device__ __forceinline__ void store(T *row, const Chan &c, float2 v) {
     const float f[2] = {v.x, v.y};
-    if (on0) P::store(p, P::pack(f));
+    P::store(row + c.c0, P::pack(f));
   }
 };
 template <typename T> struct Pair<T, false> {
   struct Raw { T a, b; };
-  static __device__ __forceinline__ int channel(int g, int lane) { return g * REC_GROUP + lane; }
+  static __device__ __forceinline__ Chan channels(int g, int lane, int C) {
+    return Chan{min(g * REC_GROUP + lane, C - 1), min(g * REC_GROUP + lane + 32, C - 1)};
+  }
   static __device__ __forceinline__ Raw zero() { return Raw{Elem<T>::from_acc(0.f), Elem<T>::from_acc(0.f)}; }
   static __device__ __forceinline__ Raw closed() {
     const T inf = Elem<T>::from_acc(-__int_as_float(0x7f800000));
     return Raw{inf, inf};
   }
-  static __device__ __forceinline__ Raw load(const T *p, bool on0, bool on1) {
-    Raw r = zero();
-    if (on0) r.a = p[0];
-    if (on1) r.b = p[32];
-    return r;
-  }
+  static __device__ __forceinline__ Raw load(const T *row, const Chan &c) { return Raw{row[c.c0], row[c.c1]}; }
   static __device__ __forceinline__ float2 get(const Raw &r) {
     return make_float2(Elem<T>::to_acc(r.a), Elem<T>::to_acc(r.b));
   }
-  static __device__ __forceinline__ void store(T *p, float2 v, bool on0, bool on1) {
-    if (on0) p[0] = Elem<T>::from_acc(v.x);
-    if (on1) p[32] = Elem<T>::from_acc(v.y);
+  static __device__ __forceinline__ void store(T *row, const Chan &c, float2 v) {
+    row[c.c0] = Elem<T>::from_acc(v.x);
+    row[c.c1] = Elem<T>::from_acc(v.y);
   }
 };
 
 // ---- copies ahead ------------------------------------------------------------------------------
 
-// 16 bytes to shared memory, or 16 zero bytes.
-__device__ __forceinline__ void copy16(uint32_t to, const void *from, bool on) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(on ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copies_done() {
-  asm volatile("cp.async.wait_all;" ::: "memory");
-  __syncwarp();
-}
-
-// The rows of one tensor that a warp works on, [REC_L][REC_GROUP] in shared memory, copied by its lanes.
-template <typename T> struct RowCopy {
-  static constexpr int E = 16 / (int)sizeof(T), CHUNKS = REC_GROUP / E, ROWS = 32 / CHUNKS, PASSES = REC_L / ROWS;
-  const T *from;  // this lane's chunk of row `sub` of the tensor's row 0
-  long long rs;
-  uint32_t to;
-  int sub;
-  bool on;
-  __device__ __forceinline__ void init(const SeqIn<T> &in, T *stage, int b, int grp, int C, int lane) {
-    const int col = (lane % CHUNKS) * E;
-    sub = lane / CHUNKS;
-    on = grp * REC_GROUP + col < C;
-    from = in.p + (long long)b * in.bs + (on ? grp * REC_GROUP + col : 0);
-    rs = in.rs;
-    to = (uint32_t)__cvta_generic_to_shared(stage + sub * REC_GROUP + col);
-  }
-  // rows t0 .. t0 + REC_L - 1; zeros at T and behind
-  __device__ __forceinline__ void start(int t0, int T_) const {
-    const T *p = from + (long long)(t0 + sub) * rs;
-#pragma unroll
-    for (int k = 0; k < PASSES; ++k) {
-      const bool in = on && t0 + sub + k * ROWS < T_;
-      copy16(to + k * ROWS * REC_GROUP * (int)sizeof(T), in ? p + (long long)(k * ROWS) * rs : from, in);
-    }
-  }
+struct RecMaps {
+  CUtensorMap m[4];  // x, u, v (, dy) as (channel, row, batch)
 };
+__device__ __forceinline__ void rows_load(void *to, const CUtensorMap *map, int c, int t, int b, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_u32(to)),
+      "l"(map), "r"(c), "r"(t), "r"(b), "r"(smem_u32(bar))
+      : "memory");
+}
+// Bounded wait for what this CTA's and its peers' copies and stores signal.  A wait that runs out raises
+// the flag that dwconv_b200_device_status reports; the kernel goes on to its end.
+__device__ __forceinline__ void wait_or_flag(uint64_t *bar, uint32_t parity) {
+  for (unsigned n = 0; n < ROWS_WAIT_LIMIT; ++n) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(ROWS_WAIT_HINT_NS)
+        : "memory");
+    if (ok) return;
+  }
+  if ((threadIdx.x & 31) == 0) atomicExch(&g_seq_error_flag, 8);
+}
 
-// Rows at T and behind: a gate of -infinity is closed, the state passes through it.  A lane writes what
-// it reads itself.
-template <typename T> __device__ __forceinline__ void close_rows(T *gate, int rows, int lane) {
+// Rows at T and behind: a gate of -infinity is closed, the state passes through it.  Every lane
+// writes what it reads itself (the same as others that share its channels).
+template <typename T> __device__ __forceinline__ void close_rows(T *gate, int rows, int col) {
 #pragma unroll
   for (int j = 0; j < REC_L; ++j)
-    if (j >= rows) Pack<T, 2>::store(gate + j * REC_GROUP + 2 * lane, Pair<T, true>::closed());
+    if (j >= rows) Pack<T, 2>::store(gate + j * REC_GROUP + col, Pair<T, true>::closed());
 }
 
 // ---- rows of a warp ----------------------------------------------------------------------------
@@ -284,12 +285,12 @@ struct RowWalk {
   }
 };
 
-__device__ __forceinline__ float2 load_state(const float *s, long long j, int C, int c, int c1, bool on0, bool on1) {
-  return make_float2(on0 ? s[j * C + c] : 0.f, on1 ? s[j * C + c1] : 0.f);
+__device__ __forceinline__ float2 load_state(const float *s, long long j, int C, const Chan &c) {
+  return make_float2(s[j * C + c.c0], s[j * C + c.c1]);
 }
-__device__ __forceinline__ void store_state(float *s, long long j, int C, int c, int c1, bool on0, bool on1, float2 v) {
-  if (on0) s[j * C + c] = v.x;
-  if (on1) s[j * C + c1] = v.y;
+__device__ __forceinline__ void store_state(float *s, long long j, int C, const Chan &c, float2 v) {
+  s[j * C + c.c0] = v.x;
+  s[j * C + c.c1] = v.y;
 }
 
 // Folding pairs.  PACKED: a pair whose rows begin a sequence takes nothing from in front of it, whatever
@@ -307,11 +308,15 @@ template <bool PACKED> __device__ __forceinline__ float2 apply(float2 P, float2 
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ void store_peer(const void *mine, int rank, float4 v) {
-  uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
-               : "memory");
+// 16 bytes to the same place of a peer's shared memory, counted by the same barrier of the peer.
+__device__ __forceinline__ void store_peer(const void *mine, const uint64_t *bar, int rank, float4 v) {
+  uint32_t a, m;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(mine)), "r"(rank));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(m) : "r"(smem_u32(bar)), "r"(rank));
+  asm volatile(
+      "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(a), "f"(v.x),
+      "f"(v.y), "f"(v.z), "f"(v.w), "r"(m)
+      : "memory");
 }
 
 // The warp's number, known to the compiler to be the same in all its lanes.
@@ -324,88 +329,98 @@ struct RecParams {
 };
 
 // Sequences without a row: what enters leaves.
-__device__ __forceinline__ void empty_states(const RecParams &p, int warp, const float *from, float *to, int c, int c1,
-                                             bool on0, bool on1) {
+__device__ __forceinline__ void empty_states(const RecParams &p, int warp, const float *from, float *to, const Chan &c) {
   for (int j = warp; j < p.q.S; j += REC_W)
     if (seq_bound(p.q, j) >= seq_bound(p.q, j + 1))
-      store_state(to, j, p.q.C, c, c1, on0, on1, from ? load_state(from, j, p.q.C, c, c1, on0, on1) : f2(0.f));
+      store_state(to, j, p.q.C, c, from ? load_state(from, j, p.q.C, c) : f2(0.f));
 }
 
-// Shared memory of a CTA: the staged rows (FAST), the warps' pairs (twice, for one barrier per tile),
+// Shared memory of a CTA: the staged rows (FAST), barriers, the warps' pairs (twice, for one barrier per tile),
 // backward the rows' decays, the tiles' pairs of the cluster (twice).
 constexpr int REC_PAIRS = 2 * REC_W * 32 * (int)sizeof(float4);
 template <typename T> constexpr int rec_stage_bytes(int tensors) {
   return tensors * REC_TILE * REC_GROUP * (int)sizeof(T);
 }
+constexpr int REC_BARRIERS = 128;  // one per warp for its copies, two for the cluster's pairs
 constexpr int REC_DECAYS = REC_TILE * REC_GROUP * (int)sizeof(float);
 inline size_t rec_smem(int stage, bool backward, int cs) {
-  return (size_t)stage + REC_PAIRS + (backward ? REC_PAIRS / 2 + REC_DECAYS : 0) + (cs > 1 ? 2 * cs * 32 * sizeof(float4) : 0);
+  return (size_t)stage + REC_BARRIERS + REC_PAIRS + (backward ? REC_PAIRS / 2 + REC_DECAYS : 0) + (cs > 1 ? 2 * cs * 32 * sizeof(float4) : 0);
 }
 
-// FAST: 16-byte rows, copied ahead; otherwise read where they are used, channels c and c + 32 per lane.
+// FAST: rows copied ahead by tensor copies; otherwise read where they are used, channels c and c + 32 per lane.
+// Barriers of a CTA; with clusters, a peer's shared memory may be written once the peer has passed here.
+template <bool FAST> __device__ __forceinline__ void start_cta(uint64_t *bars, int cs) {
+  if (!FAST && cs == 1) return;
+  if (threadIdx.x == 0) {
+    for (int n = 0; n < REC_W + 2; ++n) mbar_init(bars + n, 1);
+    fence_barrier_init();
+  }
+  __syncthreads();
+  if (cs > 1) {
+    cluster_arrive();
+    cluster_wait();
+  }
+}
+
 template <typename T, bool FAST, bool PACKED, bool SERIES>
-__device__ __forceinline__ void forward_body(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v, const float *__restrict__ initial,
+__device__ __forceinline__ void forward_body(const RecMaps &maps, SeqIn<T> x, SeqIn<T> u, SeqIn<T> v, const float *__restrict__ initial,
              T *__restrict__ y, float *__restrict__ fin, float *__restrict__ ckpt, const RecParams &p, const Rate &k) {
   using Q = Pair<T, FAST>;
   constexpr int L = REC_L, W = REC_W, NT = 3;
-  extern __shared__ __align__(16) unsigned char smem[];
+  extern __shared__ __align__(128) unsigned char smem[];
   T *stage = reinterpret_cast<T *>(smem);
-  float4(*agg)[W][32] = reinterpret_cast<float4(*)[W][32]>(smem + (FAST ? rec_stage_bytes<T>(NT) : 0));
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (FAST ? rec_stage_bytes<T>(NT) : 0)), *met = bars + W;
+  float4(*agg)[W][32] = reinterpret_cast<float4(*)[W][32]>(reinterpret_cast<unsigned char *>(bars) + REC_BARRIERS);
   float4 *far = reinterpret_cast<float4 *>(agg + 2);  // [2][cs][32]
   const int lane = threadIdx.x & 31, warp = uniform_warp();
   const int rank = (int)(blockIdx.x % p.cs);
   const long long pair = blockIdx.x / p.cs;
   const int grp = (int)(pair % p.groups), b = (int)(pair / p.groups);
-  const int C = p.q.C, c = Q::channel(grp, lane), c1 = FAST ? c + 1 : c + 32;
-  const bool on0 = c < C, on1 = c1 < C;
+  const int C = p.q.C;
+  const Chan c = Q::channels(grp, lane, C);
   const int tiles = ceil_div(p.q.T, REC_TILE), steps = ceil_div(tiles, p.cs);
   T *mine = stage + warp * (NT * L * REC_GROUP);
-  RowCopy<T> cx, cu, cv;
+  const int col = c.c0 - grp * REC_GROUP;  // of this lane in the staged rows
   auto start_copies = [&](int tile) {
-    const int t = tile * REC_TILE + warp * L;
-    cx.start(t, p.q.T);
-    cu.start(t, p.q.T);
-    cv.start(t, p.q.T);
+    if (lane == 0) {
+      const int t = tile * REC_TILE + warp * L;
+      mbar_arrive_expect_tx(bars + warp, NT * L * REC_GROUP * (uint32_t)sizeof(T));
+#pragma unroll
+      for (int n = 0; n < NT; ++n) rows_load(mine + n * L * REC_GROUP, &maps.m[n], grp * REC_GROUP, t, b, bars + warp);
+    }
   };
-  if constexpr (FAST) {
-    cx.init(x, mine, b, grp, C, lane);
-    cu.init(u, mine + L * REC_GROUP, b, grp, C, lane);
-    cv.init(v, mine + 2 * L * REC_GROUP, b, grp, C, lane);
-    if (steps > 0) start_copies(rank);
-  }
-  if (p.cs > 1) {  // a peer's shared memory may be written once it runs
-    cluster_arrive();
-    cluster_wait();
-  }
-  if (PACKED && fin != nullptr && rank == 0) empty_states(p, warp, initial, fin, c, c1, on0, on1);
+  start_cta<FAST>(bars, p.cs);
+  if (FAST && steps > 0) start_copies(rank);
+  if (PACKED && fin != nullptr && rank == 0) empty_states(p, warp, initial, fin, c);
   RowWalk walk;
   float2 carry = f2(0.f);
-  if (!PACKED && initial != nullptr) carry = load_state(initial, b, C, c, c1, on0, on1);
+  if (!PACKED && initial != nullptr) carry = load_state(initial, b, C, c);
   for (int it = 0; it < steps; ++it) {
-    const int tile = it * p.cs + rank, t0 = tile * REC_TILE + warp * L, half = it & 1;
+    const int tile = it * p.cs + rank, t0 = tile * REC_TILE + warp * L, half = it & 1, phase = it >> 1 & 1;
     const int rows = p.q.T - t0;
+    if (p.cs > 1 && threadIdx.x == 0) mbar_arrive_expect_tx(met + half, p.cs * 512);
     RowMasks m{0u, 0u, 0u};
     if (PACKED) m = walk.masks<L>(p.q, t0);
     float2 a[L], bb[L], P = f2(1.f), H = f2(0.f);
     {
       typename Q::Raw rx[L], ru[L], rv[L];
       if constexpr (FAST) {
-        copies_done();
-        if (!PACKED && rows < L) close_rows<T>(mine + L * REC_GROUP, rows, lane);
+        wait_or_flag(bars + warp, it & 1);
+        if (!PACKED && rows < L) close_rows<T>(mine + L * REC_GROUP, rows, col);
 #pragma unroll
         for (int j = 0; j < L; ++j) {
-          rx[j] = Q::P::load(mine + j * REC_GROUP + 2 * lane);
-          ru[j] = Q::P::load(mine + (L + j) * REC_GROUP + 2 * lane);
-          rv[j] = Q::P::load(mine + (2 * L + j) * REC_GROUP + 2 * lane);
+          rx[j] = Q::P::load(mine + j * REC_GROUP + col);
+          ru[j] = Q::P::load(mine + (L + j) * REC_GROUP + col);
+          rv[j] = Q::P::load(mine + (2 * L + j) * REC_GROUP + col);
         }
       } else {
-        const T *px = x.row(b, t0) + c, *pu = u.row(b, t0) + c, *pv = v.row(b, t0) + c;
+        const T *px = x.row(b, t0), *pu = u.row(b, t0), *pv = v.row(b, t0);
 #pragma unroll
         for (int j = 0; j < L; ++j) {
-          rx[j] = Q::load(px + j * x.rs, j < rows && on0, j < rows && on1);
-          ru[j] = Q::load(pu + j * u.rs, j < rows && on0, j < rows && on1);
+          rx[j] = j < rows ? Q::load(px + j * x.rs, c) : Q::zero();
+          ru[j] = j < rows ? Q::load(pu + j * u.rs, c) : Q::zero();
           if (!PACKED && j >= rows) ru[j] = Q::closed();
-          rv[j] = Q::load(pv + j * v.rs, j < rows && on0, j < rows && on1);
+          rv[j] = j < rows ? Q::load(pv + j * v.rs, c) : Q::zero();
         }
       }
 #pragma unroll
@@ -434,7 +449,7 @@ __device__ __forceinline__ void forward_body(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v,
           H = f2(0.f);
         } else if (m.start >> j & 1u) {
           if (initial != nullptr)
-            bb[j] = fma2(a[j], load_state(initial, seq_locate(p.q, t0 + j).seq, C, c, c1, on0, on1), bb[j]);
+            bb[j] = fma2(a[j], load_state(initial, seq_locate(p.q, t0 + j).seq, C, c), bb[j]);
           P = f2(-1.f);
           H = bb[j];
         } else {
@@ -458,10 +473,9 @@ __device__ __forceinline__ void forward_body(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v,
           TH = apply<PACKED>(P2, H2, TH);
           TP = join<PACKED>(TP, P2);
         }
-        for (int peer = warp; peer < p.cs; peer += W) store_peer(there, peer, make_float4(TP.x, TP.y, TH.x, TH.y));
+        for (int peer = warp; peer < p.cs; peer += W) store_peer(there, met + half, peer, make_float4(TP.x, TP.y, TH.x, TH.y));
       }
-      cluster_arrive();
-      cluster_wait();
+      wait_or_flag(met + half, phase);
       for (int w = 0; w < p.cs; ++w) {
         if (w == rank) h = carry;
         const float4 e = far[(half * p.cs + w) * 32 + lane];
@@ -469,7 +483,7 @@ __device__ __forceinline__ void forward_body(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v,
       }
     }
     if (ckpt != nullptr && warp == 0 && tile < tiles)
-      store_state(ckpt, (long long)b * tiles + tile, C, c, c1, on0, on1, h);
+      store_state(ckpt, (long long)b * tiles + tile, C, c, h);
     float2 in = h;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
@@ -487,32 +501,33 @@ __device__ __forceinline__ void forward_body(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v,
 #pragma unroll
       for (int j = 0; j < L; ++j) {
         h = fma2(a[j], h, bb[j]);
-        Q::store(py + (unsigned)(j * C + c), h, on0, on1);
+        Q::store(py + (long long)j * C, c, h);
       }
     } else {
 #pragma unroll
       for (int j = 0; j < L; ++j) {
         h = PACKED && ((m.start | m.none) >> j & 1u) ? bb[j] : fma2(a[j], h, bb[j]);
-        Q::store(py + (unsigned)(j * C + c), h, j < rows && on0, j < rows && on1);
+        if (j < rows) Q::store(py + (long long)j * C, c, h);
         if (PACKED && (m.end >> j & 1u) && fin != nullptr)
-          store_state(fin, seq_locate(p.q, t0 + j).seq, C, c, c1, on0, on1, h);
+          store_state(fin, seq_locate(p.q, t0 + j).seq, C, c, h);
       }
     }
   }
-  if (!PACKED && fin != nullptr && rank == 0 && warp == 0) store_state(fin, b, C, c, c1, on0, on1, carry);
+  if (!PACKED && fin != nullptr && rank == 0 && warp == 0) store_state(fin, b, C, c, carry);
 }
 
 template <typename T, bool FAST, bool PACKED, bool SERIES>
-__device__ __forceinline__ void backward_body(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v, const float *__restrict__ initial,
+__device__ __forceinline__ void backward_body(const RecMaps &maps, SeqIn<T> x, SeqIn<T> u, SeqIn<T> v, const float *__restrict__ initial,
               const float *__restrict__ ckpt, SeqIn<T> dy, const float *__restrict__ dfin, T *__restrict__ dx,
               T *__restrict__ du, T *__restrict__ dv, float *__restrict__ dinit, float *__restrict__ part,
               const RecParams &p, const Rate &k) {
   using Q = Pair<T, FAST>;
   constexpr int L = REC_L, W = REC_W, NT = 4;
-  extern __shared__ __align__(16) unsigned char smem[];
+  extern __shared__ __align__(128) unsigned char smem[];
   T *stage = reinterpret_cast<T *>(smem);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (FAST ? rec_stage_bytes<T>(NT) : 0)), *met = bars + W;
   // P, H of each warp's rows, and what leaves them towards earlier rows
-  float4(*agg)[W][32] = reinterpret_cast<float4(*)[W][32]>(smem + (FAST ? rec_stage_bytes<T>(NT) : 0));
+  float4(*agg)[W][32] = reinterpret_cast<float4(*)[W][32]>(reinterpret_cast<unsigned char *>(bars) + REC_BARRIERS);
   float2(*aggq)[W][32] = reinterpret_cast<float2(*)[W][32]>(agg + 2);
   float2(*keep)[32] = reinterpret_cast<float2(*)[32]>(aggq + 2) + uniform_warp() * L;  // a of this warp's rows
   float4 *far = reinterpret_cast<float4 *>(reinterpret_cast<float2(*)[32]>(aggq + 2) + W * L);  // [2][cs][32]
@@ -520,64 +535,58 @@ __device__ __forceinline__ void backward_body(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v
   const int rank = (int)(blockIdx.x % p.cs);
   const long long pair = blockIdx.x / p.cs;
   const int grp = (int)(pair % p.groups), b = (int)(pair / p.groups);
-  const int C = p.q.C, c = Q::channel(grp, lane), c1 = FAST ? c + 1 : c + 32;
-  const bool on0 = c < C, on1 = c1 < C;
+  const int C = p.q.C;
+  const Chan c = Q::channels(grp, lane, C);
   const int tiles = ceil_div(p.q.T, REC_TILE), steps = ceil_div(tiles, p.cs);
   T *mine = stage + warp * (NT * L * REC_GROUP);
-  RowCopy<T> cx, cu, cv, cg;
+  const int col = c.c0 - grp * REC_GROUP;  // of this lane in the staged rows
   auto start_copies = [&](int tile) {
-    const int t = tile * REC_TILE + warp * L;
-    cx.start(t, p.q.T);
-    cu.start(t, p.q.T);
-    cv.start(t, p.q.T);
-    cg.start(t, p.q.T);
+    if (lane == 0) {
+      const int t = tile * REC_TILE + warp * L;
+      mbar_arrive_expect_tx(bars + warp, NT * L * REC_GROUP * (uint32_t)sizeof(T));
+#pragma unroll
+      for (int n = 0; n < NT; ++n) rows_load(mine + n * L * REC_GROUP, &maps.m[n], grp * REC_GROUP, t, b, bars + warp);
+    }
   };
-  if constexpr (FAST) {
-    cx.init(x, mine, b, grp, C, lane);
-    cu.init(u, mine + L * REC_GROUP, b, grp, C, lane);
-    cv.init(v, mine + 2 * L * REC_GROUP, b, grp, C, lane);
-    cg.init(dy, mine + 3 * L * REC_GROUP, b, grp, C, lane);
-    if (steps > 0) start_copies((steps - 1) * p.cs + rank);
-  }
-  if (p.cs > 1) {
-    cluster_arrive();
-    cluster_wait();
-  }
-  if (PACKED && dinit != nullptr && rank == 0) empty_states(p, warp, dfin, dinit, c, c1, on0, on1);
+  start_cta<FAST>(bars, p.cs);
+  if (FAST && steps > 0) start_copies((steps - 1) * p.cs + rank);
+  if (PACKED && dinit != nullptr && rank == 0) empty_states(p, warp, dfin, dinit, c);
   RowWalk walk;
   float2 carry = f2(0.f), ddecay = f2(0.f);
-  if (!PACKED && dfin != nullptr) carry = load_state(dfin, b, C, c, c1, on0, on1);
+  if (!PACKED && dfin != nullptr) carry = load_state(dfin, b, C, c);
   for (int it = steps - 1; it >= 0; --it) {
-    const int tile = it * p.cs + rank, t0 = tile * REC_TILE + warp * L, half = it & 1;
+    const int n = steps - 1 - it, half = n & 1, phase = n >> 1 & 1;
+    const int tile = it * p.cs + rank, t0 = tile * REC_TILE + warp * L;
     const int rows = p.q.T - t0;
+    if (p.cs > 1 && threadIdx.x == 0) mbar_arrive_expect_tx(met + half, p.cs * 512);
     RowMasks mk{0u, 0u, 0u};
     if (PACKED) mk = walk.masks<L>(p.q, t0);
     const unsigned special = mk.start | mk.none;
     float2 h = f2(0.f);
-    if (tile < tiles) h = load_state(ckpt, (long long)b * tiles + tile, C, c, c1, on0, on1);
+    if (tile < tiles) h = load_state(ckpt, (long long)b * tiles + tile, C, c);
     typename Q::Raw rx[L];
     float2 t[L], i[L], g[L];
     {
       typename Q::Raw ru[L], rv[L], rg[L];
       if constexpr (FAST) {
-        copies_done();
-        if (!PACKED && rows < L) close_rows<T>(mine + L * REC_GROUP, rows, lane);
+        wait_or_flag(bars + warp, n & 1);
+        if (!PACKED && rows < L) close_rows<T>(mine + L * REC_GROUP, rows, col);
 #pragma unroll
         for (int j = 0; j < L; ++j) {
-          rx[j] = Q::P::load(mine + j * REC_GROUP + 2 * lane);
-          ru[j] = Q::P::load(mine + (L + j) * REC_GROUP + 2 * lane);
-          rv[j] = Q::P::load(mine + (2 * L + j) * REC_GROUP + 2 * lane);
-          rg[j] = Q::P::load(mine + (3 * L + j) * REC_GROUP + 2 * lane);
+          rx[j] = Q::P::load(mine + j * REC_GROUP + col);
+          ru[j] = Q::P::load(mine + (L + j) * REC_GROUP + col);
+          rv[j] = Q::P::load(mine + (2 * L + j) * REC_GROUP + col);
+          rg[j] = Q::P::load(mine + (3 * L + j) * REC_GROUP + col);
         }
       } else {
-        const T *px = x.row(b, t0) + c, *pu = u.row(b, t0) + c, *pv = v.row(b, t0) + c, *pg = dy.row(b, t0) + c;
+        const T *px = x.row(b, t0), *pu = u.row(b, t0), *pv = v.row(b, t0), *pg = dy.row(b, t0);
 #pragma unroll
         for (int j = 0; j < L; ++j) {
-          rx[j] = Q::load(px + j * x.rs, j < rows && on0, j < rows && on1);
-          ru[j] = Q::load(pu + j * u.rs, j < rows && on0, j < rows && on1);
+          rx[j] = j < rows ? Q::load(px + j * x.rs, c) : Q::zero();
+          ru[j] = j < rows ? Q::load(pu + j * u.rs, c) : Q::zero();
           if (!PACKED && j >= rows) ru[j] = Q::closed();
-          rv[j] = Q::load(pv + j * v.rs, j < rows && on0, j < rows && on1);
-          rg[j] = Q::load(pg + j * dy.rs, j < rows && on0, j < rows && on1);
+          rv[j] = j < rows ? Q::load(pv + j * v.rs, c) : Q::zero();
+          rg[j] = j < rows ? Q::load(pg + j * dy.rs, c) : Q::zero();
         }
       }
 #pragma unroll
@@ -589,6 +598,7 @@ __device__ __forceinline__ void backward_body(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v
       }
     }
     if constexpr (FAST) {
+      if (!PACKED && rows < L) fence_proxy_async_smem();  // rows closed by plain stores
       __syncwarp();
       if (it > 0) start_copies(tile - p.cs);
     }
@@ -596,7 +606,7 @@ __device__ __forceinline__ void backward_body(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v
 #pragma unroll
       for (int j = 0; j < L; ++j)
         if (mk.end >> j & 1u)
-          g[j] = add2(g[j], load_state(dfin, seq_locate(p.q, t0 + j).seq, C, c, c1, on0, on1));
+          g[j] = add2(g[j], load_state(dfin, seq_locate(p.q, t0 + j).seq, C, c));
     }
     // what the rows do to a state going down (P, H), and what they pass to a gradient going up
     // (G = sum_j a[0] .. a[j] g[j], up to the first row that begins a sequence)
@@ -609,7 +619,7 @@ __device__ __forceinline__ void backward_body(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v
       if (PACKED && (special >> j & 1u)) {
         if (mk.none >> j & 1u) bb = f2(0.f);
         else if (initial != nullptr)
-          bb = fma2(a, load_state(initial, seq_locate(p.q, t0 + j).seq, C, c, c1, on0, on1), bb);
+          bb = fma2(a, load_state(initial, seq_locate(p.q, t0 + j).seq, C, c), bb);
         P = f2(-1.f);
         H = bb;
       } else {
@@ -638,10 +648,9 @@ __device__ __forceinline__ void backward_body(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v
           TG = apply<PACKED>(P2, aggq[half][w][lane], TG);
           TP = join<PACKED>(TP, P2);
         }
-        for (int peer = warp; peer < p.cs; peer += W) store_peer(there, peer, make_float4(TP.x, TP.y, TG.x, TG.y));
+        for (int peer = warp; peer < p.cs; peer += W) store_peer(there, met + half, peer, make_float4(TP.x, TP.y, TG.x, TG.y));
       }
-      cluster_arrive();
-      cluster_wait();
+      wait_or_flag(met + half, phase);
       for (int w = p.cs - 1; w >= 0; --w) {
         if (w == rank) q = carry;
         const float4 e = far[(half * p.cs + w) * 32 + lane];
@@ -670,7 +679,7 @@ __device__ __forceinline__ void backward_body(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v
       q = mul2(keep[j][lane], g[j]);
       if (PACKED && (special >> j & 1u)) {
         if ((mk.start >> j & 1u) && dinit != nullptr)
-          store_state(dinit, seq_locate(p.q, t0 + j).seq, C, c, c1, on0, on1, q);
+          store_state(dinit, seq_locate(p.q, t0 + j).seq, C, c, q);
         q = f2(0.f);
       }
     }
@@ -685,7 +694,7 @@ __device__ __forceinline__ void backward_body(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v
       if (PACKED && (special >> j & 1u)) {
         h = f2(0.f);
         if ((mk.start >> j & 1u) && initial != nullptr)
-          h = load_state(initial, seq_locate(p.q, t0 + j).seq, C, c, c1, on0, on1);
+          h = load_state(initial, seq_locate(p.q, t0 + j).seq, C, c);
         if (mk.none >> j & 1u) g[j] = f2(0.f);
       }
       const float2 ddx = mul2(g[j], mul2(beta, i[j]));
@@ -694,15 +703,15 @@ __device__ __forceinline__ void backward_body(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v
       const float2 ddu = mul2(dzz, one_minus2(r));
       sum = add2(sum, dzz);
       h = fma2(a, h, mul2(beta, ix));
-      const bool live = j < rows;
-      const unsigned o = (unsigned)(j * C + c);
-      Q::store(px + o, ddx, live && on0, live && on1);
-      Q::store(pu + o, ddu, live && on0, live && on1);
-      Q::store(pv + o, ddv, live && on0, live && on1);
+      if (j < rows) {
+        Q::store(px + (long long)j * C, c, ddx);
+        Q::store(pu + (long long)j * C, c, ddu);
+        Q::store(pv + (long long)j * C, c, ddv);
+      }
     }
     ddecay = add2(ddecay, sum);
   }
-  if (!PACKED && dinit != nullptr && rank == 0 && warp == 0) store_state(dinit, b, C, c, c1, on0, on1, carry);
+  if (!PACKED && dinit != nullptr && rank == 0 && warp == 0) store_state(dinit, b, C, c, carry);
   // this CTA's part of ddecay: the warps' sums in order
   __syncthreads();
   aggq[0][warp][lane] = ddecay;
@@ -711,45 +720,43 @@ __device__ __forceinline__ void backward_body(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v
     float2 s = aggq[0][0][lane];
 #pragma unroll
     for (int w = 1; w < W; ++w) s = add2(s, aggq[0][w][lane]);
-    store_state(part, (long long)b * p.cs + rank, C, c, c1, on0, on1, s);
+    store_state(part, (long long)b * p.cs + rank, C, c, s);
   }
 }
 
-// Of this lane's channels, 0 beyond the last.
-__device__ __forceinline__ Rate rate_of(const float *decay, float scale, int c, int c1, bool on0, bool on1) {
-  const float2 k = make_float2(on0 ? scale * softplus(decay[c]) : 0.f, on1 ? scale * softplus(decay[c1]) : 0.f);
+__device__ __forceinline__ Rate rate_of(const float *decay, float scale, const Chan &c) {
+  const float2 k = make_float2(scale * softplus(decay[c.c0]), scale * softplus(decay[c.c1]));
   return Rate{make_float2(-k.x, -k.y), make_float2(sqrtf(2.f * k.x), sqrtf(2.f * k.y))};
 }
 template <typename T, bool FAST> __device__ __forceinline__ Rate cta_rate(const float *decay, const RecParams &p) {
-  const int grp = (int)(blockIdx.x / p.cs % p.groups), c = Pair<T, FAST>::channel(grp, threadIdx.x & 31);
-  const int c1 = FAST ? c + 1 : c + 32;
-  return rate_of(decay, p.scale, c, c1, c < p.q.C, c1 < p.q.C);
+  const int grp = (int)(blockIdx.x / p.cs % p.groups);
+  return rate_of(decay, p.scale, Pair<T, FAST>::channels(grp, threadIdx.x & 31, p.q.C));
 }
 
 template <typename T, bool FAST, bool PACKED>
 __global__ void __launch_bounds__(REC_THREADS, 3)
-recurrence_forward_kernel(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v, const float *__restrict__ decay,
+recurrence_forward_kernel(const __grid_constant__ RecMaps maps, SeqIn<T> x, SeqIn<T> u, SeqIn<T> v, const float *__restrict__ decay,
                           const float *__restrict__ initial, T *__restrict__ y, float *__restrict__ fin,
                           float *__restrict__ ckpt, RecParams p) {
   const Rate k = cta_rate<T, FAST>(decay, p);
   // the same in every warp of the CTA: they have its channels in common
   if (__all_sync(0xffffffffu, k.ks.x >= -REC_SERIES && k.ks.y >= -REC_SERIES))
-    forward_body<T, FAST, PACKED, true>(x, u, v, initial, y, fin, ckpt, p, k);
+    forward_body<T, FAST, PACKED, true>(maps, x, u, v, initial, y, fin, ckpt, p, k);
   else
-    forward_body<T, FAST, PACKED, false>(x, u, v, initial, y, fin, ckpt, p, k);
+    forward_body<T, FAST, PACKED, false>(maps, x, u, v, initial, y, fin, ckpt, p, k);
 }
 
 template <typename T, bool FAST, bool PACKED>
 __global__ void __launch_bounds__(REC_THREADS, 2)
-recurrence_backward_kernel(SeqIn<T> x, SeqIn<T> u, SeqIn<T> v, const float *__restrict__ decay,
+recurrence_backward_kernel(const __grid_constant__ RecMaps maps, SeqIn<T> x, SeqIn<T> u, SeqIn<T> v, const float *__restrict__ decay,
                            const float *__restrict__ initial, const float *__restrict__ ckpt, SeqIn<T> dy,
                            const float *__restrict__ dfin, T *__restrict__ dx, T *__restrict__ du, T *__restrict__ dv,
                            float *__restrict__ dinit, float *__restrict__ part, RecParams p) {
   const Rate k = cta_rate<T, FAST>(decay, p);
   if (__all_sync(0xffffffffu, k.ks.x >= -REC_SERIES && k.ks.y >= -REC_SERIES))
-    backward_body<T, FAST, PACKED, true>(x, u, v, initial, ckpt, dy, dfin, dx, du, dv, dinit, part, p, k);
+    backward_body<T, FAST, PACKED, true>(maps, x, u, v, initial, ckpt, dy, dfin, dx, du, dv, dinit, part, p, k);
   else
-    backward_body<T, FAST, PACKED, false>(x, u, v, initial, ckpt, dy, dfin, dx, du, dv, dinit, part, p, k);
+    backward_body<T, FAST, PACKED, false>(maps, x, u, v, initial, ckpt, dy, dfin, dx, du, dv, dinit, part, p, k);
 }
 
 template <typename T, bool VEC>
@@ -763,17 +770,17 @@ recurrence_step_kernel(const T *__restrict__ x, long long xs, const T *__restric
   if (pair >= (long long)p.groups * p.B) return;
   const int grp = (int)(pair % p.groups);
   const long long b = pair / p.groups;
-  const int C = p.q.C, c = Q::channel(grp, lane), c1 = VEC ? c + 1 : c + 32;
-  const bool on0 = c < C, on1 = c1 < C;
-  const typename Q::Raw rx = Q::load(x + b * xs + c, on0, on1), ru = Q::load(u + b * us + c, on0, on1),
-                        rv = Q::load(v + b * vs + c, on0, on1);
-  const float2 h0 = load_state(state, b, C, c, c1, on0, on1);
-  const Rate k = rate_of(decay, p.scale, c, c1, on0, on1);
+  const int C = p.q.C;
+  const Chan c = Q::channels(grp, lane, C);
+  const typename Q::Raw rx = Q::load(x + b * xs, c), ru = Q::load(u + b * us, c), rv = Q::load(v + b * vs, c);
+  const float2 h0 = load_state(state, b, C, c);
+  const Rate k = rate_of(decay, p.scale, c);
   const float2 t = root_sigmoid2(Q::get(ru)), sz = mul2(k.ks, mul2(t, t));
   const float2 bb = mul2(beta2<false>(t, sz, k), mul2(sigmoid2(Q::get(rv)), Q::get(rx)));
   const float2 h = fma2(keep2<false>(sz), h0, bb);
-  store_state(state, b, C, c, c1, on0, on1, h);
-  Q::store(y + b * C + c, h, on0, on1);
+  __syncwarp();  // lanes that share a channel have all read its state
+  store_state(state, b, C, c, h);
+  Q::store(y + b * C, c, h);
 }
 
 // ---- host --------------------------------------------------------------------------------------
@@ -844,43 +851,59 @@ struct RecArgs {
   float scale;
 };
 
-// Whether all rows start on 16 bytes.
-inline bool rec_fast(const RecArgs &a, size_t es) {
-  const int E = (int)(16 / es);
+// One operand as the copy engine sees it; false where it cannot.
+template <typename T> bool rows_map(CUtensorMap *map, const dwconv_b200_rows &r, const dwconv_b200_sequence &s) {
+  constexpr int E = 16 / (int)sizeof(T);
+  // the stride of an extent of one is never used: any valid one will do
+  const long long rs = s.T > 1 ? r.row_stride : E, bs = s.B > 1 ? r.batch_stride : E;
+  if (!aligned_to(r.data, 16) || rs <= 0 || bs <= 0 || rs % E != 0 || bs % E != 0) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)s.C, (cuuint64_t)s.T, (cuuint64_t)s.B};
+  const cuuint64_t strides[2] = {(cuuint64_t)rs * sizeof(T), (cuuint64_t)bs * sizeof(T)};
+  const cuuint32_t box[3] = {(cuuint32_t)REC_GROUP, (cuuint32_t)REC_L, 1u};
+  return encode_tensor_map<T>(map, static_cast<const T *>(r.data), 3, dims, strides, box);
+}
+template <typename T> bool rec_maps(const RecArgs &a, RecMaps &maps) {
+  if (a.s->T == 0 || a.s->C % 2 != 0) return false;
   const void *ptrs[] = {a.y, a.dx, a.du, a.dv};
   for (const void *q : ptrs)
-    if (q != nullptr && !aligned_to(q, 16)) return false;
-  return a.s->C % E == 0 && rows_vector(*a.x, E, es) && rows_vector(*a.u, E, es) && rows_vector(*a.v, E, es) &&
-         (a.dy == nullptr || rows_vector(*a.dy, E, es));
+    if (q != nullptr && !aligned_to(q, 2 * sizeof(T))) return false;
+  return rows_map<T>(&maps.m[0], *a.x, *a.s) && rows_map<T>(&maps.m[1], *a.u, *a.s) &&
+         rows_map<T>(&maps.m[2], *a.v, *a.s) && (a.dy == nullptr || rows_map<T>(&maps.m[3], *a.dy, *a.s));
 }
 
-template <typename T, bool FAST, bool PACKED> void launch_forward(const RecArgs &a, cudaStream_t st) {
+template <typename T, bool FAST, bool PACKED> void launch_forward(const RecArgs &a, const RecMaps &maps, cudaStream_t st) {
   static std::atomic<unsigned long long> ready{0};
   const RecParams p = rec_params(*a.s, a.scale, false);
   const int stage = FAST ? rec_stage_bytes<T>(3) : 0;
   rec_launch(recurrence_forward_kernel<T, FAST, PACKED>, ready, p, rec_smem(stage, false, REC_MAX_CLUSTER),
-             rec_smem(stage, false, p.cs), st, seq_in<T>(*a.x), seq_in<T>(*a.u), seq_in<T>(*a.v), a.decay, a.initial,
+             rec_smem(stage, false, p.cs), st, maps, seq_in<T>(*a.x), seq_in<T>(*a.u), seq_in<T>(*a.v), a.decay, a.initial,
              static_cast<T *>(a.y), a.fin, a.ckpt, p);
 }
-template <typename T, bool FAST, bool PACKED> void launch_backward(const RecArgs &a, cudaStream_t st) {
+template <typename T, bool FAST, bool PACKED> void launch_backward(const RecArgs &a, const RecMaps &maps, cudaStream_t st) {
   static std::atomic<unsigned long long> ready{0};
   const RecParams p = rec_params(*a.s, a.scale, true);
   const int stage = FAST ? rec_stage_bytes<T>(4) : 0;
   rec_launch(recurrence_backward_kernel<T, FAST, PACKED>, ready, p, rec_smem(stage, true, REC_MAX_CLUSTER),
-             rec_smem(stage, true, p.cs), st, seq_in<T>(*a.x), seq_in<T>(*a.u), seq_in<T>(*a.v), a.decay, a.initial,
+             rec_smem(stage, true, p.cs), st, maps, seq_in<T>(*a.x), seq_in<T>(*a.u), seq_in<T>(*a.v), a.decay, a.initial,
              a.ckpt_in, seq_in<T>(*a.dy), a.dfin, static_cast<T *>(a.dx), static_cast<T *>(a.du),
              static_cast<T *>(a.dv), a.dinit, a.part, p);
 }
 
 template <typename T> void forward_t(const RecArgs &a, cudaStream_t st) {
   const bool packed = a.s->offsets != nullptr;
-  if (rec_fast(a, sizeof(T))) packed ? launch_forward<T, true, true>(a, st) : launch_forward<T, true, false>(a, st);
-  else packed ? launch_forward<T, false, true>(a, st) : launch_forward<T, false, false>(a, st);
+  RecMaps maps{};
+  if (rec_maps<T>(a, maps))
+    packed ? launch_forward<T, true, true>(a, maps, st) : launch_forward<T, true, false>(a, maps, st);
+  else
+    packed ? launch_forward<T, false, true>(a, maps, st) : launch_forward<T, false, false>(a, maps, st);
 }
 template <typename T> void backward_t(const RecArgs &a, cudaStream_t st) {
   const bool packed = a.s->offsets != nullptr;
-  if (rec_fast(a, sizeof(T))) packed ? launch_backward<T, true, true>(a, st) : launch_backward<T, true, false>(a, st);
-  else packed ? launch_backward<T, false, true>(a, st) : launch_backward<T, false, false>(a, st);
+  RecMaps maps{};
+  if (rec_maps<T>(a, maps))
+    packed ? launch_backward<T, true, true>(a, maps, st) : launch_backward<T, true, false>(a, maps, st);
+  else
+    packed ? launch_backward<T, false, true>(a, maps, st) : launch_backward<T, false, false>(a, maps, st);
 }
 
 template <typename T>
@@ -906,6 +929,21 @@ int check_recurrence(int dtype, const dwconv_b200_sequence *s) {
 }
 
 }  // namespace
+
+// Reads and clears this translation unit's error flag (bit 3).
+int seq_take_error() {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_seq_error_flag, sizeof(int)) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return 0;
+  }
+  if (v != 0) {
+    const int zero = 0;
+    (void)cudaMemcpyToSymbol(g_seq_error_flag, &zero, sizeof(int));
+  }
+  return v;
+}
+
 }  // namespace dwb
 
 using namespace dwb;
