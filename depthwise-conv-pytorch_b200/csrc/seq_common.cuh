@@ -66,6 +66,91 @@ template <typename T, int V> struct Pack {
   }
 };
 
+// ---- channels of a lane ------------------------------------------------------------------------
+
+// Arithmetic on pairs of channels: one instruction for two fp32 operations.
+__device__ __forceinline__ float2 f2(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 one_minus2(float2 v) { return fma2(v, f2(-1.f), f2(1.f)); }
+
+__device__ __forceinline__ float ex2f(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rcpf(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rsqf(float v) {
+  float r;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+// 1 + exp(-v)
+__device__ __forceinline__ float2 one_plus_exp2(float2 v) {
+  const float2 e = mul2(v, f2(-LOG2E));
+  return add2(make_float2(ex2f(e.x), ex2f(e.y)), f2(1.f));
+}
+// sigmoid; an overflowing exponential gives 0
+__device__ __forceinline__ float2 sigmoid2(float2 v) {
+  const float2 s = one_plus_exp2(v);
+  return make_float2(rcpf(s.x), rcpf(s.y));
+}
+
+// H pairs of channels per lane.  VEC: 2 H adjacent ones, one load; otherwise (odd C, odd strides; H = 1)
+// channels c and d = c + 32, one load each.  Lanes beyond the last channel work on the last ones too, and
+// store the same values to the same places: no access needs a test.
+template <typename T, int H, bool VEC> struct Lanes;
+template <typename T, int H> struct Lanes<T, H, true> {
+  static constexpr int GROUP = 64 * H;  // channels of a warp
+  using P = Pack<T, 2 * H>;
+  using Raw = typename P::Raw;
+  int c;
+  __device__ __forceinline__ Lanes(int group, int lane, int C) : c(min(group * GROUP + 2 * H * lane, C - 2 * H)) {}
+  __device__ __forceinline__ int channel(int i) const { return c + i; }
+  __device__ __forceinline__ Raw load(const T *row) const { return P::load(row + c); }
+  __device__ __forceinline__ void store(T *row, const float2 (&v)[H]) const {
+    float f[2 * H];
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      f[2 * h] = v[h].x;
+      f[2 * h + 1] = v[h].y;
+    }
+    P::store(row + c, P::pack(f));
+  }
+  static __device__ __forceinline__ Raw zero() { return P::zero(); }
+  static __device__ __forceinline__ void get(const Raw &r, float2 (&v)[H]) {
+    float f[2 * H];
+    P::unpack(r, f);
+#pragma unroll
+    for (int h = 0; h < H; ++h) v[h] = make_float2(f[2 * h], f[2 * h + 1]);
+  }
+};
+template <typename T> struct Lanes<T, 1, false> {
+  static constexpr int GROUP = 64;
+  struct Raw { T a, b; };
+  int c, d;
+  __device__ __forceinline__ Lanes(int group, int lane, int C)
+      : c(min(group * GROUP + lane, C - 1)), d(min(group * GROUP + lane + 32, C - 1)) {}
+  __device__ __forceinline__ int channel(int i) const { return i ? d : c; }
+  __device__ __forceinline__ Raw load(const T *row) const { return Raw{row[c], row[d]}; }
+  __device__ __forceinline__ void store(T *row, const float2 (&v)[1]) const {
+    row[c] = Elem<T>::from_acc(v[0].x);
+    row[d] = Elem<T>::from_acc(v[0].y);
+  }
+  static __device__ __forceinline__ Raw zero() { return Raw{Elem<T>::from_acc(0.f), Elem<T>::from_acc(0.f)}; }
+  static __device__ __forceinline__ void get(const Raw &r, float2 (&v)[1]) {
+    v[0] = make_float2(Elem<T>::to_acc(r.a), Elem<T>::to_acc(r.b));
+  }
+};
+
 // ---- packed sequences --------------------------------------------------------------------------
 
 // The list of packed sequences, or (offsets null) one sequence per batch element.

@@ -28,26 +28,28 @@ struct Conv1dParams {
   int act;
 };
 
-__device__ __forceinline__ float sigmoid_f(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
-
-__device__ __forceinline__ float act_f(float p, int act) {
+__device__ __forceinline__ float2 act2(float2 p, int act) {
   if (act == DWCONV_B200_ACT_NONE) return p;
-  if (act == DWCONV_B200_ACT_SILU) return p * sigmoid_f(p);
-  return apply_activation<float>(p, act);
+  if (act == DWCONV_B200_ACT_SILU) return mul2(p, sigmoid2(p));
+  return make_float2(apply_activation<float>(p.x, act), apply_activation<float>(p.y, act));
 }
 
-// act'(p)
-__device__ __forceinline__ float act_slope(float p, int act) {
+__device__ __forceinline__ float slope(float p, int act) {
   switch (act) {
-    case DWCONV_B200_ACT_SILU: {
-      const float s = sigmoid_f(p);
-      return s * fmaf(p, 1.f - s, 1.f);
-    }
     case DWCONV_B200_ACT_RELU: return p > 0.f ? 1.f : 0.f;
     case DWCONV_B200_ACT_RELU6: return p > 0.f && p < 6.f ? 1.f : 0.f;
     case DWCONV_B200_ACT_HARDSWISH: return p <= -3.f ? 0.f : (p >= 3.f ? 1.f : (2.f * p + 3.f) / 6.f);
     default: return 1.f;
   }
+}
+// g act'(p)
+__device__ __forceinline__ float2 act_back2(float2 g, float2 p, int act) {
+  if (act == DWCONV_B200_ACT_NONE) return g;
+  if (act == DWCONV_B200_ACT_SILU) {
+    const float2 s = sigmoid2(p);
+    return mul2(mul2(g, s), fma2(p, one_minus2(s), f2(1.f)));
+  }
+  return mul2(g, make_float2(slope(p.x, act), slope(p.y, act)));
 }
 
 __device__ __forceinline__ SeqSpan conv_span(const SeqList &q, int b, int t) {
@@ -56,22 +58,50 @@ __device__ __forceinline__ SeqSpan conv_span(const SeqList &q, int b, int t) {
 }
 
 // The K-1 rows in front of row t, oldest first: rows of the sequence, or of its initial state.
-template <typename T, int V, int K>
-__device__ __forceinline__ void fill_window(float (&win)[K][V], const SeqIn<T> &x, const T *initial, int C, int b,
-                                            int t, const SeqSpan &sp, int c, bool on) {
-  using P = Pack<T, V>;
+template <typename T, int H, bool VEC, int K>
+__device__ __forceinline__ void fill_window(float2 (&win)[K][H], const Lanes<T, H, VEC> &ln, const SeqIn<T> &x,
+                                            const T *initial, int C, int b, int t, const SeqSpan &sp) {
 #pragma unroll
   for (int j = 0; j < K - 1; ++j) {
     const int row = t - (K - 1) + j;
-    typename P::Raw raw = P::zero();
-    if (on) {
-      if (row >= sp.begin) raw = P::load(x.row(b, row) + c);
-      else if (initial != nullptr && sp.seq >= 0)
-        raw = P::load(initial + ((long long)sp.seq * (K - 1) + (row - sp.begin + K - 1)) * C + c);
-    }
-    P::unpack(raw, win[j]);
+    typename Lanes<T, H, VEC>::Raw raw = ln.zero();
+    if (row >= sp.begin) raw = ln.load(x.row(b, row));
+    else if (initial != nullptr && sp.seq >= 0)
+      raw = ln.load(initial + ((long long)sp.seq * (K - 1) + (row - sp.begin + K - 1)) * C);
+    ln.get(raw, win[j]);
   }
 }
+
+template <int H, int K> __device__ __forceinline__ void shift(float2 (&a)[K][H]) {
+#pragma unroll
+  for (int k = 0; k + 1 < K; ++k)
+#pragma unroll
+    for (int h = 0; h < H; ++h) a[k][h] = a[k + 1][h];
+}
+
+// The taps (and bias) of a lane's channels.
+template <typename T, int H, bool VEC, int K> struct Taps {
+  float2 w[K][H], b[H];
+  __device__ __forceinline__ Taps(const Lanes<T, H, VEC> &ln, const T *wt, const T *bias) {
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      const int c = ln.channel(2 * h), d = ln.channel(2 * h + 1);
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        w[k][h] = make_float2(read(wt + (long long)c * K + k), read(wt + (long long)d * K + k));
+      b[h] = bias != nullptr ? make_float2(read(bias + c), read(bias + d)) : f2(0.f);
+    }
+  }
+  // the sum over a window, taps in order
+  __device__ __forceinline__ void apply(const float2 (&win)[K][H], float2 (&o)[H]) const {
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      o[h] = b[h];
+#pragma unroll
+      for (int k = 0; k < K; ++k) o[h] = fma2(w[k][h], win[k][h], o[h]);
+    }
+  }
+};
 
 // The last K-1 rows of each sequence.
 template <typename T, int K>
@@ -94,76 +124,72 @@ __device__ void final_rows(const SeqIn<T> &x, const T *initial, T *fin, const Se
   }
 }
 
-template <typename T, int V, int K>
-__global__ void __launch_bounds__(CONV_WARPS * 32)
+template <typename T, int H, bool VEC, int K>
+__global__ void __launch_bounds__(CONV_WARPS * 32, K <= 4 ? 3 : 2)
 conv1d_forward_kernel(SeqIn<T> x, const T *__restrict__ w, const T *__restrict__ bias, const T *__restrict__ initial,
                       T *__restrict__ y, T *__restrict__ fin, Conv1dParams p) {
-  using P = Pack<T, V>;
-  constexpr int U = 8;  // rows loaded together
+  using Ln = Lanes<T, H, VEC>;
+  constexpr int U = sizeof(T) == 4 ? 4 : 8;  // rows loaded together
   if (blockIdx.x >= p.main) {
     if constexpr (K > 1) final_rows<T, K>(x, initial, fin, p.q, (int)(blockIdx.x - p.main), (int)(gridDim.x - p.main));
     return;
   }
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
   const int cb = (int)(blockIdx.x % p.cblocks);
   const long long rest = blockIdx.x / p.cblocks;
   const int rb = (int)(rest % p.rblocks), b = (int)(rest / p.rblocks);
-  const int C = p.q.C, c = (cb * 32 + lane) * V;
-  const bool on = c < C;
+  const int C = p.q.C;
   const long long first = ((long long)rb * CONV_WARPS + warp) * p.R;
   if (first >= p.q.T) return;
   const int t0 = (int)first, t1 = min(t0 + p.R, p.q.T);
-  float wk[K][V], bv[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) wk[k][i] = on ? read(w + (long long)(c + i) * K + k) : 0.f;
-    bv[i] = on && bias ? read(bias + c + i) : 0.f;
-  }
+  const Ln ln(cb, threadIdx.x & 31, C);
+  const Taps<T, H, VEC, K> taps(ln, w, bias);
   SeqSpan sp = conv_span(p.q, b, t0);
-  float win[K][V];
-  fill_window<T, V, K>(win, x, initial, C, b, t0, sp, c, on);
-  for (int t = t0; t < t1; t += U) {
-    typename P::Raw raw[U];
-    const T *xr = x.row(b, t) + c;
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-      raw[j] = P::zero();
-      if (on && t + j < t1) raw[j] = P::load(xr + j * x.rs);
+  float2 win[K][H];
+  fill_window(win, ln, x, initial, C, b, t0, sp);
+  int t = t0;
+  while (t < t1) {
+    if (t == sp.next) {
+      sp = conv_span(p.q, b, t);
+      fill_window(win, ln, x, initial, C, b, t, sp);
     }
-    T *yr = y + ((long long)b * p.q.T + t) * C + c;
+    const T *xr = x.row(b, t);
+    T *yr = y + ((long long)b * p.q.T + t) * C;
+    if (t + U <= t1 && t + U <= sp.next && sp.seq >= 0) {
+      typename Ln::Raw raw[U];
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-      if (t + j >= t1) break;
-      if (t + j == sp.next) {
-        sp = conv_span(p.q, b, t + j);
-        fill_window<T, V, K>(win, x, initial, C, b, t + j, sp, c, on);
+      for (int j = 0; j < U; ++j) raw[j] = ln.load(xr + j * x.rs);
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        float2 o[H];
+        ln.get(raw[j], win[K - 1]);
+        taps.apply(win, o);
+#pragma unroll
+        for (int h = 0; h < H; ++h) o[h] = act2(o[h], p.act);
+        ln.store(yr + (long long)j * C, o);
+        shift(win);
       }
-      P::unpack(raw[j], win[K - 1]);
-      float o[V];
+      t += U;
+    } else {
+      float2 o[H];
+      ln.get(ln.load(xr), win[K - 1]);
+      taps.apply(win, o);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        o[i] = bv[i];
-#pragma unroll
-        for (int k = 0; k < K; ++k) o[i] = fmaf(wk[k][i], win[k][i], o[i]);
-        o[i] = sp.seq >= 0 ? act_f(o[i], p.act) : 0.f;
-      }
-      if (on) P::store(yr + (long long)j * C, P::pack(o));
-#pragma unroll
-      for (int k = 0; k + 1 < K; ++k)
-#pragma unroll
-        for (int i = 0; i < V; ++i) win[k][i] = win[k + 1][i];
+      for (int h = 0; h < H; ++h) o[h] = sp.seq >= 0 ? act2(o[h], p.act) : f2(0.f);
+      ln.store(yr, o);
+      shift(win);
+      ++t;
     }
   }
 }
 
 // dx, the initial rows' gradient, and this CTA's part of dw and db: part[block of runs][K + 1][C].
-template <typename T, int V, int K>
-__global__ void __launch_bounds__(CONV_WARPS * 32)
+template <typename T, int H, bool VEC, int K>
+__global__ void __launch_bounds__(CONV_WARPS * 32, 2)
 conv1d_backward_kernel(SeqIn<T> x, const T *__restrict__ w, const T *__restrict__ bias, const T *__restrict__ initial,
                        SeqIn<T> dy, const T *__restrict__ dfin, T *__restrict__ dx, T *__restrict__ dinit,
                        float *__restrict__ part, Conv1dParams p) {
-  using P = Pack<T, V>;
+  using Ln = Lanes<T, H, VEC>;
   if (blockIdx.x >= p.main) {  // sequences without a row: their state passes through
     const long long each = (long long)(K - 1) * p.q.C;
     for (int j = (int)(blockIdx.x - p.main); j < p.q.S; j += (int)(gridDim.x - p.main)) {
@@ -174,80 +200,65 @@ conv1d_backward_kernel(SeqIn<T> x, const T *__restrict__ w, const T *__restrict_
     }
     return;
   }
-  __shared__ float sum[(K + 1) * V * 32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ float2 sum[(K + 1) * H][32];
+  const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
   const int cb = (int)(blockIdx.x % p.cblocks);
   const long long rest = blockIdx.x / p.cblocks;
   const int rb = (int)(rest % p.rblocks), b = (int)(rest / p.rblocks);
-  const int C = p.q.C, c = (cb * 32 + lane) * V;
-  const bool on = c < C;
+  const int C = p.q.C;
+  const Ln ln(cb, lane, C);
   const long long first = ((long long)rb * CONV_WARPS + warp) * p.R;
-  float dwk[K][V], db[V];
+  float2 dwk[K][H], db[H];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    db[i] = 0.f;
+  for (int h = 0; h < H; ++h) {
+    db[h] = f2(0.f);
 #pragma unroll
-    for (int k = 0; k < K; ++k) dwk[k][i] = 0.f;
+    for (int k = 0; k < K; ++k) dwk[k][h] = f2(0.f);
   }
   if (first < p.q.T) {
     const int t0 = (int)first, t1 = min(t0 + p.R, p.q.T);
-    float wk[K][V], bv[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-#pragma unroll
-      for (int k = 0; k < K; ++k) wk[k][i] = on ? read(w + (long long)(c + i) * K + k) : 0.f;
-      bv[i] = on && bias ? read(bias + c + i) : 0.f;
-    }
-    float win[K][V], dpw[K][V];  // rows t-(K-1) .. t of x and of dp, oldest first; t's place is free between rows
+    const Taps<T, H, VEC, K> taps(ln, w, bias);
+    float2 win[K][H], dpw[K][H];  // rows t-(K-1) .. t of x and of dp, oldest first; t's place is free between rows
     SeqSpan sp = conv_span(p.q, b, t0);
-    fill_window<T, V, K>(win, x, initial, C, b, t0, sp, c, on);
+    fill_window(win, ln, x, initial, C, b, t0, sp);
+    auto clear = [&]() {
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+      for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < V; ++i) dpw[k][i] = 0.f;
-
-    // the gradient of row t - (K-1), complete once dp[t] is in the window (oldest dp: tap K-1)
-    auto gradient = [&](float (&o)[V]) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        o[i] = 0.f;
-#pragma unroll
-        for (int k = 0; k < K; ++k) o[i] = fmaf(wk[k][i], dpw[K - 1 - k][i], o[i]);
-      }
+        for (int h = 0; h < H; ++h) dpw[k][h] = f2(0.f);
     };
-    auto shift = [&](float (&a)[K][V]) {
+    clear();
+    // the gradient of row t - (K-1), complete once dp[t] is in the window (oldest dp: tap K-1)
+    auto gradient = [&](float2 (&o)[H]) {
 #pragma unroll
-      for (int k = 0; k + 1 < K; ++k)
+      for (int h = 0; h < H; ++h) {
+        o[h] = mul2(taps.w[0][h], dpw[K - 1][h]);
 #pragma unroll
-        for (int i = 0; i < V; ++i) a[k][i] = a[k + 1][i];
+        for (int k = 1; k < K; ++k) o[h] = fma2(taps.w[k][h], dpw[K - 1 - k][h], o[h]);
+      }
     };
     // a row's gradient to where it belongs: dx, or the initial rows of a sequence that starts here
-    auto emit = [&](int row, const float (&o)[V]) {
-      if (!on) return;
+    auto emit = [&](int row, const float2 (&o)[H]) {
       if (row >= sp.begin) {
-        if (row >= t0 && row < t1) P::store(dx + ((long long)b * p.q.T + row) * C + c, P::pack(o));
+        if (row >= t0 && row < t1) ln.store(dx + ((long long)b * p.q.T + row) * C, o);
       } else if (dinit != nullptr && sp.seq >= 0 && sp.begin >= t0 && sp.begin < t1) {
-        P::store(dinit + ((long long)sp.seq * (K - 1) + (row - sp.begin + K - 1)) * C + c, P::pack(o));
+        ln.store(dinit + ((long long)sp.seq * (K - 1) + (row - sp.begin + K - 1)) * C, o);
       }
     };
-    auto take = [&](const typename P::Raw &rx, const typename P::Raw &rg) {
-      float g[V];
-      P::unpack(rx, win[K - 1]);
-      P::unpack(rg, g);
+    auto take = [&](const typename Ln::Raw &rx, const typename Ln::Raw &rg) {
+      float2 g[H], s[H];
+      ln.get(rx, win[K - 1]);
+      ln.get(rg, g);
+      taps.apply(win, s);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float s = bv[i];
-#pragma unroll
-        for (int k = 0; k < K; ++k) s = fmaf(wk[k][i], win[k][i], s);
-        dpw[K - 1][i] = g[i] * act_slope(s, p.act);
-      }
+      for (int h = 0; h < H; ++h) dpw[K - 1][h] = act_back2(g[h], s[h], p.act);
     };
     auto count = [&]() {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        db[i] += dpw[K - 1][i];
+      for (int h = 0; h < H; ++h) {
+        db[h] = add2(db[h], dpw[K - 1][h]);
 #pragma unroll
-        for (int k = 0; k < K; ++k) dwk[k][i] = fmaf(dpw[K - 1][i], win[k][i], dwk[k][i]);
+        for (int k = 0; k < K; ++k) dwk[k][h] = fma2(dpw[K - 1][h], win[k][h], dwk[k][h]);
       }
     };
 
@@ -259,65 +270,60 @@ conv1d_backward_kernel(SeqIn<T> x, const T *__restrict__ w, const T *__restrict_
         // the sequence ends: its last K-1 rows take no more products, but are its final state
 #pragma unroll
         for (int f = 0; f < K - 1; ++f) {
-          float o[V];
+          float2 o[H];
 #pragma unroll
-          for (int i = 0; i < V; ++i) dpw[K - 1][i] = 0.f;
+          for (int h = 0; h < H; ++h) dpw[K - 1][h] = f2(0.f);
           gradient(o);
-          if (dfin != nullptr && sp.seq >= 0 && on) {
-            float d[V];
-            P::unpack(P::load(dfin + ((long long)sp.seq * (K - 1) + f) * C + c), d);
+          if (dfin != nullptr && sp.seq >= 0) {
+            float2 d[H];
+            ln.get(ln.load(dfin + ((long long)sp.seq * (K - 1) + f) * C), d);
 #pragma unroll
-            for (int i = 0; i < V; ++i) o[i] += d[i];
+            for (int h = 0; h < H; ++h) o[h] = add2(o[h], d[h]);
           }
           emit(t + f - (K - 1), o);
           shift(dpw);
         }
         if (t >= t1) break;
         sp = conv_span(p.q, b, t);
-        fill_window<T, V, K>(win, x, initial, C, b, t, sp, c, on);
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-          for (int i = 0; i < V; ++i) dpw[k][i] = 0.f;
+        fill_window(win, ln, x, initial, C, b, t, sp);
+        clear();
       }
       const int lead = t - (K - 1);
       if (lead >= t0 && lead >= sp.begin && t + U <= t1 && t + U <= sp.next && sp.seq >= 0) {
         // U rows inside the run and the sequence
-        typename P::Raw rx[U], rg[U];
-        const T *xr = x.row(b, t) + c, *gr = dy.row(b, t) + c;
+        typename Ln::Raw rx[U], rg[U];
+        const T *xr = x.row(b, t), *gr = dy.row(b, t);
+        T *dr = dx + ((long long)b * p.q.T + lead) * C;
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-          rx[j] = rg[j] = P::zero();
-          if (on) {
-            rx[j] = P::load(xr + j * x.rs);
-            rg[j] = P::load(gr + j * dy.rs);
-          }
+          rx[j] = ln.load(xr + j * x.rs);
+          rg[j] = ln.load(gr + j * dy.rs);
         }
 #pragma unroll
         for (int j = 0; j < U; ++j) {
+          float2 o[H];
           take(rx[j], rg[j]);
           count();
-          float o[V];
           gradient(o);
-          if (on) P::store(dx + ((long long)b * p.q.T + lead + j) * C + c, P::pack(o));
+          ln.store(dr + (long long)j * C, o);
           shift(win);
           shift(dpw);
         }
         t += U;
       } else {
-        typename P::Raw rx = P::zero(), rg = P::zero();
-        if (on && sp.seq >= 0) {
-          rx = P::load(x.row(b, t) + c);
-          rg = P::load(dy.row(b, t) + c);
+        typename Ln::Raw rx = ln.zero(), rg = ln.zero();
+        if (sp.seq >= 0) {
+          rx = ln.load(x.row(b, t));
+          rg = ln.load(dy.row(b, t));
         }
         take(rx, rg);
         if (sp.seq < 0) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) dpw[K - 1][i] = 0.f;
+          for (int h = 0; h < H; ++h) dpw[K - 1][h] = f2(0.f);
         } else if (t < t1) {
           count();
         }
-        float o[V];
+        float2 o[H];
         gradient(o);
         emit(lead, o);
         shift(win);
@@ -326,58 +332,54 @@ conv1d_backward_kernel(SeqIn<T> x, const T *__restrict__ w, const T *__restrict_
       }
     }
   }
-  if (part == nullptr) return;
-  for (int k = 0; k < CONV_WARPS; ++k) {  // warp after warp, in order
-    if (warp == k) {
+  for (int n = 0; n < CONV_WARPS; ++n) {  // warp after warp, in order
+    if (warp == n) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
+      for (int h = 0; h < H; ++h) {
 #pragma unroll
         for (int m = 0; m <= K; ++m) {
-          float *s = sum + (m * V + i) * 32 + lane;
-          const float v = m < K ? dwk[m < K ? m : 0][i] : db[i];
-          *s = k ? *s + v : v;
+          float2 *s = &sum[m * H + h][lane];
+          const float2 v = m < K ? dwk[m < K ? m : 0][h] : db[h];
+          *s = n ? add2(*s, v) : v;
         }
       }
     }
     __syncthreads();
   }
   float *mine = part + rest * (K + 1) * C;
-  for (int m = threadIdx.x; m < (K + 1) * V * 32; m += blockDim.x) {
-    const int ch = cb * 32 * V + m % (32 * V), k = m / (32 * V);  // consecutive threads, consecutive channels
-    const int i = (m % V), l = (m % (32 * V)) / V;
-    if (ch < C) mine[(long long)k * C + ch] = sum[(k * V + i) * 32 + l];
+  for (int m = threadIdx.x; m < (K + 1) * Ln::GROUP; m += blockDim.x) {  // consecutive threads, consecutive channels
+    const int n = m % Ln::GROUP, k = m / Ln::GROUP, ch = cb * Ln::GROUP + n;
+    const int l = VEC ? n / (2 * H) : n % 32, i = VEC ? n % (2 * H) : n / 32;
+    const float2 v = sum[k * H + i / 2][l];
+    if (ch < C) mine[(long long)k * C + ch] = i & 1 ? v.y : v.x;
   }
 }
 
-template <typename T, int V, int K>
+template <typename T, int H, bool VEC, int K>
 __global__ void __launch_bounds__(128)
 conv1d_step_kernel(const T *__restrict__ x, long long xs, const T *__restrict__ w, const T *__restrict__ bias,
-                   T *__restrict__ state, T *__restrict__ y, long long n, int C, int act) {
-  using P = Pack<T, V>;
-  const long long at = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * V;
-  if (at >= n) return;
-  const int c = (int)(at % C);
-  const long long b = at / C;
-  T *st = state + b * (K - 1) * C + c;
-  typename P::Raw raw[K];
+                   T *__restrict__ state, T *__restrict__ y, long long units, int groups, int C, int act) {
+  using Ln = Lanes<T, H, VEC>;
+  const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);  // a group of channels of a batch element
+  if (unit >= units) return;
+  const Ln ln((int)(unit % groups), threadIdx.x & 31, C);
+  const long long b = unit / groups;
+  T *st = state + b * (K - 1) * C;
+  typename Ln::Raw raw[K];
 #pragma unroll
-  for (int k = 0; k < K - 1; ++k) raw[k] = P::load(st + (long long)k * C);
-  raw[K - 1] = P::load(x + b * xs + c);
-  float o[V];
+  for (int k = 0; k < K - 1; ++k) raw[k] = ln.load(st + (long long)k * C);
+  raw[K - 1] = ln.load(x + b * xs);
+  const Taps<T, H, VEC, K> taps(ln, w, bias);
+  float2 win[K][H], o[H];
 #pragma unroll
-  for (int i = 0; i < V; ++i) o[i] = bias ? read(bias + c + i) : 0.f;
+  for (int k = 0; k < K; ++k) ln.get(raw[k], win[k]);
+  taps.apply(win, o);
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    float f[V];
-    P::unpack(raw[k], f);
+  for (int h = 0; h < H; ++h) o[h] = act2(o[h], act);
+  ln.store(y + b * C, o);
+  __syncwarp();  // lanes that share channels have all read their state
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = fmaf(read(w + (long long)(c + i) * K + k), f[i], o[i]);
-  }
-#pragma unroll
-  for (int i = 0; i < V; ++i) o[i] = act_f(o[i], act);
-  P::store(y + at, P::pack(o));
-#pragma unroll
-  for (int k = 0; k < K - 1; ++k) P::store(st + (long long)k * C, raw[k + 1]);
+  for (int k = 0; k < K - 1; ++k) ln.store(st + (long long)k * C, win[k + 1]);
 }
 
 // ---- host --------------------------------------------------------------------------------------
@@ -392,11 +394,11 @@ inline int conv_run(int B, int T, int C) {
   return R;
 }
 
-inline Conv1dParams conv_params(const dwconv_b200_sequence &s, int V, int act) {
+inline Conv1dParams conv_params(const dwconv_b200_sequence &s, int group, int act) {
   Conv1dParams p;
   p.q = seq_list(s);
   p.R = conv_run(s.B, s.T, s.C);
-  p.cblocks = ceil_div(s.C, 32 * V);
+  p.cblocks = ceil_div(s.C, group);
   p.rblocks = ceil_div(ceil_div(s.T, p.R), CONV_WARPS);
   p.main = (long long)p.cblocks * p.rblocks * s.B;
   p.act = act;
@@ -430,31 +432,30 @@ struct ConvArgs {
   int taps, act;
 };
 
-template <typename T, int V> void launch_forward(const ConvArgs &a, cudaStream_t st) {
-  const Conv1dParams p = conv_params(*a.s, V, a.act);
+template <typename T, int H, bool VEC> void launch_forward(const ConvArgs &a, cudaStream_t st) {
+  const Conv1dParams p = conv_params(*a.s, Lanes<T, H, VEC>::GROUP, a.act);
   long long extra = 0;
   if (a.fin != nullptr && a.taps > 1) {
     extra = ceil_div_ll((long long)p.q.S * (a.taps - 1) * p.q.C, CONV_WARPS * 32);
     if (extra > STATE_BLOCKS) extra = STATE_BLOCKS;
   }
   if (p.main + extra == 0) return;
-  DWB_TAPS(a.taps, (conv1d_forward_kernel<T, V, TAPS><<<(unsigned)(p.main + extra), CONV_WARPS * 32, 0, st>>>(
+  DWB_TAPS(a.taps, (conv1d_forward_kernel<T, H, VEC, TAPS><<<(unsigned)(p.main + extra), CONV_WARPS * 32, 0, st>>>(
                        seq_in<T>(*a.x), (const T *)a.w, (const T *)a.bias, (const T *)a.initial, (T *)a.y,
                        (T *)a.fin, p)))
 }
 
 // Register windows of x, dp, w and dw: four channels per lane for up to four taps, two above.
-template <typename T, int V> void launch_backward(const ConvArgs &a, cudaStream_t st) {
-  const Conv1dParams p = conv_params(*a.s, a.taps > 4 && V > 2 ? 2 : V, a.act);
+template <typename T, int H, bool VEC> void launch_backward(const ConvArgs &a, cudaStream_t st) {
+  const Conv1dParams p = conv_params(*a.s, a.taps > 4 ? 64 : Lanes<T, H, VEC>::GROUP, a.act);
   long long extra = 0;
   if (a.dinit != nullptr && a.taps > 1 && (a.s->offsets != nullptr || a.s->T == 0))
     extra = p.q.S < STATE_BLOCKS ? p.q.S : STATE_BLOCKS;
   if (p.main + extra == 0) return;
-  DWB_TAPS(a.taps,
-           (conv1d_backward_kernel<T, (TAPS > 4 && V > 2 ? 2 : V), TAPS>
-            <<<(unsigned)(p.main + extra), CONV_WARPS * 32, 0, st>>>(
-                seq_in<T>(*a.x), (const T *)a.w, (const T *)a.bias, (const T *)a.initial, seq_in<T>(*a.dy),
-                (const T *)a.dfin, (T *)a.dx, (T *)a.dinit, a.part, p)))
+  DWB_TAPS(a.taps, (conv1d_backward_kernel<T, (TAPS > 4 ? 1 : H), VEC, TAPS>
+                    <<<(unsigned)(p.main + extra), CONV_WARPS * 32, 0, st>>>(
+                        seq_in<T>(*a.x), (const T *)a.w, (const T *)a.bias, (const T *)a.initial, seq_in<T>(*a.dy),
+                        (const T *)a.dfin, (T *)a.dx, (T *)a.dinit, a.part, p)))
 }
 
 // Whether everything that moves V channels at a time may.
@@ -466,21 +467,22 @@ inline bool conv_vector(const ConvArgs &a, int V, size_t es) {
 }
 
 template <typename T> void forward_t(const ConvArgs &a, cudaStream_t st) {
-  if (conv_vector(a, 4, sizeof(T))) launch_forward<T, 4>(a, st);
-  else launch_forward<T, 1>(a, st);
+  if (conv_vector(a, 4, sizeof(T))) launch_forward<T, 2, true>(a, st);
+  else launch_forward<T, 1, false>(a, st);
 }
 template <typename T> void backward_t(const ConvArgs &a, cudaStream_t st) {
-  if (conv_vector(a, 4, sizeof(T))) launch_backward<T, 4>(a, st);
-  else launch_backward<T, 1>(a, st);
+  if (conv_vector(a, 4, sizeof(T))) launch_backward<T, 2, true>(a, st);
+  else launch_backward<T, 1, false>(a, st);
 }
 
-template <typename T, int V>
+template <typename T, int H, bool VEC>
 void launch_step(const void *x, long long xs, const void *w, const void *bias, void *state, void *y, int B, int C,
                  int taps, int act, cudaStream_t st) {
-  const long long n = (long long)B * C;
-  const unsigned grid = (unsigned)ceil_div_ll(n / V, 128);
-  DWB_TAPS(taps, (conv1d_step_kernel<T, V, TAPS><<<grid, 128, 0, st>>>(
-                     (const T *)x, xs, (const T *)w, (const T *)bias, (T *)state, (T *)y, n, C, act)))
+  const int groups = ceil_div(C, Lanes<T, H, VEC>::GROUP);
+  const long long units = (long long)B * groups;
+  const unsigned grid = (unsigned)ceil_div_ll(units, 4);
+  DWB_TAPS(taps, (conv1d_step_kernel<T, H, VEC, TAPS><<<grid, 128, 0, st>>>(
+                     (const T *)x, xs, (const T *)w, (const T *)bias, (T *)state, (T *)y, units, groups, C, act)))
 }
 
 template <typename T>
@@ -488,9 +490,9 @@ void step_t(const void *x, long long xs, const void *w, const void *bias, void *
             int taps, int act, cudaStream_t st) {
   if (C % 4 == 0 && xs % 4 == 0 && aligned_to(x, 4 * sizeof(T)) && aligned_to(state, 4 * sizeof(T)) &&
       aligned_to(y, 4 * sizeof(T)))
-    launch_step<T, 4>(x, xs, w, bias, state, y, B, C, taps, act, st);
+    launch_step<T, 2, true>(x, xs, w, bias, state, y, B, C, taps, act, st);
   else
-    launch_step<T, 1>(x, xs, w, bias, state, y, B, C, taps, act, st);
+    launch_step<T, 1, false>(x, xs, w, bias, state, y, B, C, taps, act, st);
 }
 
 int check_conv(int dtype, const dwconv_b200_sequence *s, int taps) {

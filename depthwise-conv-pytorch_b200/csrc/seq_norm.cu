@@ -4,8 +4,10 @@
 //   with xh = (x - m) s and q = dy w:   dx = s (q - mean(q) - xh mean(q xh)),
 //   dw = sum over rows of dy xh,  db = sum over rows of dy.
 //
-// Both directions read each row once: `tpr` threads own a row (a power of two, up to a whole CTA) and
-// keep its values in registers, NV vectors of V elements per thread.  The variance is the sum of
+// Bound by memory (forward: x in, y out; backward: x, dy in, dx out), which a row's two sums interrupt.  Both
+// directions read each row once: `tpr` threads own a row (a power of two, up to 512) and keep its values
+// in registers as they came, NV vectors of V elements per thread, and the next row is on its way
+// meanwhile.  CTAs stay for many rows (backward: with w in registers).  The variance is the sum of
 // squares around the mean (warps' sums are merged by the parallel-variance formula, so that one
 // exchange through shared memory gives both moments), never a difference of large sums.
 #include "seq_common.cuh"
@@ -19,14 +21,8 @@ struct NormParams {
   float eps;
 };
 
-constexpr int NORM_WARPS = 32;
-constexpr int NORM_ROW_THREADS = 128;  // threads of a CTA that holds several rows
-
-// Most threads that share a row whose threads hold `per` values each: what the registers of one SM
-// allow (forward: the values; backward: x, dy, w and the two running sums).
-__host__ __device__ constexpr int norm_max_tpr(int per, bool backward) {
-  return backward ? (per <= 4 ? 1024 : per <= 16 ? 512 : 256) : (per <= 16 ? 1024 : 512);
-}
+constexpr int NORM_ROW_THREADS = 128;  // threads of a CTA whose rows lie within warps
+constexpr int NORM_CTA = 512;          // of one whose rows span warps
 
 // Sum over the `width` adjacent lanes (a power of two up to 32) that share a row.
 __device__ __forceinline__ float lanes_sum(float v, int width) {
@@ -34,7 +30,12 @@ __device__ __forceinline__ float lanes_sum(float v, int width) {
   return v;
 }
 
-// Valid elements among the vectors that the 32 lanes of warp w hold.
+// Barrier of the tpr threads (a multiple of 32) that share a row.
+__device__ __forceinline__ void row_sync(int slot, int tpr) {
+  asm volatile("bar.sync %0, %1;" ::"r"(slot + 1), "r"(tpr) : "memory");
+}
+
+// Valid elements among the vectors that the 32 lanes of a row's warp w hold.
 template <int V, int NV> __device__ __forceinline__ float warp_count(int C, int tpr, int w) {
   int n = 0;
 #pragma unroll
@@ -45,205 +46,208 @@ template <int V, int NV> __device__ __forceinline__ float warp_count(int C, int 
   return (float)(n * V);
 }
 
-// BLOCK: a CTA of tpr > 32 threads per row; otherwise 32 / tpr rows per warp.
-template <typename T, int V, int NV, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? norm_max_tpr(V *NV, false) : NORM_ROW_THREADS)
-norm_forward_kernel(const T *__restrict__ x, const T *__restrict__ w,
-                                    const T *__restrict__ b, T *__restrict__ y, float2 *stats, NormParams p) {
+// A thread's part of a row: NV vectors, tpr vectors apart.
+template <typename T, int V, int NV> struct RowPart {
   using P = Pack<T, V>;
-  __shared__ float2 red[2][BLOCK ? NORM_WARPS : 1];
-  const int tid = threadIdx.x, lane = tid & (p.tpr - 1);
-  const int slots = BLOCK ? 1 : blockDim.x / p.tpr;
-  const int slot = BLOCK ? 0 : tid / p.tpr;
+  typename P::Raw raw[NV];
+  __device__ __forceinline__ void load(const T *row, int lane, int tpr, int C, bool live) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * tpr + lane) * V;
+      raw[j] = P::zero();
+      if (live && c < C) raw[j] = P::load(row + c);
+    }
+  }
+  __device__ __forceinline__ void get(int j, float (&f)[V]) const { P::unpack(raw[j], f); }
+};
+
+// BLOCK: rows of tpr > 32 threads, blockDim / tpr of them at a time; otherwise 32 / tpr rows per warp.
+template <typename T, int V, int NV, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? NORM_CTA : NORM_ROW_THREADS, BLOCK ? 2 : 6)
+norm_forward_kernel(const T *__restrict__ x, const T *__restrict__ w, const T *__restrict__ b, T *__restrict__ y,
+                    float2 *stats, NormParams p) {
+  using P = Pack<T, V>;
+  __shared__ float2 red[2][NORM_CTA / 32];
+  const int tpr = p.tpr, lane = threadIdx.x & (tpr - 1), slot = threadIdx.x / tpr, slots = blockDim.x / tpr;
+  RowPart<T, V, NV> next;
+  const float inv = 1.f / (float)p.C;
+  const long long step = (long long)gridDim.x * slots;
   int phase = 0;
-  for (long long r0 = (long long)blockIdx.x * slots; r0 < p.rows; r0 += (long long)gridDim.x * slots) {
-    const long long r = r0 + slot;
+  long long r = (long long)blockIdx.x * slots + slot;
+  next.load(x + r * p.xs, lane, tpr, p.C, r < p.rows);
+  // the rows of a warp go on together (shuffles); those of different warps need not
+  for (long long r0 = BLOCK ? r : (long long)blockIdx.x * slots; r0 < p.rows; r0 += step, r += step) {
     const bool live = r < p.rows;
-    float f[NV][V];
+    const RowPart<T, V, NV> cur = next;
+    next.load(x + (r + step) * p.xs, lane, tpr, p.C, r + step < p.rows);
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (j * p.tpr + lane) * V;
-      typename P::Raw raw = P::zero();
-      if (live && c < p.C) raw = P::load(x + r * p.xs + c);
-      P::unpack(raw, f[j]);
+      float f[V];
+      cur.get(j, f);
 #pragma unroll
-      for (int i = 0; i < V; ++i) sum += f[j][i];
+      for (int i = 0; i < V; ++i) sum += f[i];
     }
-    float mean, rstd;
-    if constexpr (!BLOCK) {
-      mean = lanes_sum(sum, p.tpr) / (float)p.C;
-      float sq = 0.f;
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-        if ((j * p.tpr + lane) * V < p.C) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) sq += (f[j][i] - mean) * (f[j][i] - mean);
-        }
-      rstd = rsqrtf(lanes_sum(sq, p.tpr) / (float)p.C + p.eps);
-    } else {
-      const int wid = tid >> 5, nw = p.tpr >> 5;
-      const float n = warp_count<V, NV>(p.C, p.tpr, wid);
-      const float wm = n > 0.f ? lanes_sum(sum, 32) / n : 0.f;
-      float sq = 0.f;
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-        if ((j * p.tpr + lane) * V < p.C) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) sq += (f[j][i] - wm) * (f[j][i] - wm);
-        }
-      sq = lanes_sum(sq, 32);
-      if ((tid & 31) == 0) red[phase][wid] = make_float2(wm, sq);
-      __syncthreads();
-      float m = 0.f, m2 = 0.f;
-      for (int i = 0; i < nw; ++i) m += warp_count<V, NV>(p.C, p.tpr, i) * red[phase][i].x;
-      m /= (float)p.C;
-      for (int i = 0; i < nw; ++i) {
-        const float d = red[phase][i].x - m;
-        m2 += red[phase][i].y + warp_count<V, NV>(p.C, p.tpr, i) * d * d;
-      }
-      mean = m;
-      rstd = rsqrtf(m2 / (float)p.C + p.eps);
-      phase ^= 1;  // the other half: a fast warp may be a row ahead, never two
-    }
-    if (stats != nullptr && live && lane == 0) stats[r] = make_float2(mean, rstd);
+    float mean, rstd, centre, sq = 0.f;
+    const int wid = lane >> 5;
+    const float n = BLOCK ? warp_count<V, NV>(p.C, tpr, wid) : (float)p.C;
+    sum = lanes_sum(sum, BLOCK ? 32 : tpr);
+    centre = BLOCK ? (n > 0.f ? sum / n : 0.f) : sum * inv;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (j * p.tpr + lane) * V;
+      float f[V];
+      cur.get(j, f);
+      if ((j * tpr + lane) * V < p.C) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) sq = fmaf(f[i] - centre, f[i] - centre, sq);
+      }
+    }
+    sq = lanes_sum(sq, BLOCK ? 32 : tpr);
+    if constexpr (!BLOCK) {
+      mean = centre;
+    } else {
+      const int nw = tpr >> 5;
+      float2 *mine = red[phase] + slot * nw;
+      if ((threadIdx.x & 31) == 0) mine[wid] = make_float2(centre, sq);
+      row_sync(slot, tpr);
+      float m = 0.f;
+      for (int i = 0; i < nw; ++i) m = fmaf(warp_count<V, NV>(p.C, tpr, i), mine[i].x, m);
+      mean = m * inv;
+      sq = 0.f;
+      for (int i = 0; i < nw; ++i) {
+        const float d = mine[i].x - mean;
+        sq += mine[i].y + warp_count<V, NV>(p.C, tpr, i) * d * d;
+      }
+      phase ^= 1;  // the other half: a fast warp may be a row ahead, never two
+    }
+    rstd = rsqrtf(sq * inv + p.eps);
+    if (stats != nullptr && live && lane == 0) stats[r] = make_float2(mean, rstd);
+    T *yr = y + r * p.C;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * tpr + lane) * V;
       if (!live || c >= p.C) continue;
-      float wv[V], bv[V];
-      if (w) P::unpack(P::load(w + c), wv);
+      float f[V], wv[V], bv[V];
+      cur.get(j, f);
+      if (w) P::unpack(P::load(w + c), wv);  // out of L1
       if (b) P::unpack(P::load(b + c), bv);
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        f[j][i] = fmaf((f[j][i] - mean) * rstd, w ? wv[i] : 1.f, b ? bv[i] : 0.f);
-      P::store(y + r * p.C + c, P::pack(f[j]));
+      for (int i = 0; i < V; ++i) f[i] = fmaf((f[i] - mean) * rstd, w ? wv[i] : 1.f, b ? bv[i] : 0.f);
+      P::store(yr + c, P::pack(f));
     }
   }
 }
 
-// dx, and this CTA's part of dw and db: part[blockIdx.x][2][C].
+// dx, and this CTA's part of dw and db: part[blockIdx.x][2][C].  Shared memory: [2][NV * tpr * V] floats.
 template <typename T, int V, int NV, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? norm_max_tpr(V *NV, true) : NORM_ROW_THREADS)
-norm_backward_kernel(const T *__restrict__ x, const T *__restrict__ w,
-                                     const float2 *__restrict__ stats, const T *__restrict__ dy,
-                                     T *__restrict__ dx, float *__restrict__ part, NormParams p) {
+__global__ void __launch_bounds__(BLOCK ? NORM_CTA : NORM_ROW_THREADS, BLOCK ? 1 : 4)
+norm_backward_kernel(const T *__restrict__ x, const T *__restrict__ w, const float2 *__restrict__ stats,
+                     const T *__restrict__ dy, T *__restrict__ dx, float *__restrict__ part, NormParams p) {
   using P = Pack<T, V>;
-  __shared__ float2 red[2][BLOCK ? NORM_WARPS : 1];
-  extern __shared__ float acc_s[];  // !BLOCK: [2][NV * tpr * V]
-  const int tid = threadIdx.x, lane = tid & (p.tpr - 1);
-  const int slots = BLOCK ? 1 : blockDim.x / p.tpr;
-  const int slot = BLOCK ? 0 : tid / p.tpr;
-  float dw[NV][V], db[NV][V], wv[NV][V];
+  __shared__ float2 red[2][NORM_CTA / 32];
+  extern __shared__ float acc_s[];
+  const int tpr = p.tpr, lane = threadIdx.x & (tpr - 1), slot = threadIdx.x / tpr, slots = blockDim.x / tpr;
+  float dw[NV][V], db[NV][V];
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int c = (j * p.tpr + lane) * V;
-    typename P::Raw raw = P::zero();
-    if (w && c < p.C) raw = P::load(w + c);
-    P::unpack(raw, wv[j]);
+  for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      dw[j][i] = db[j][i] = 0.f;
-      if (!w) wv[j][i] = 1.f;
-    }
-  }
+    for (int i = 0; i < V; ++i) dw[j][i] = db[j][i] = 0.f;
+  RowPart<T, V, NV> nx, ng, wr;
+  if (w) wr.load(w, lane, tpr, p.C, true);
   const float inv = 1.f / (float)p.C;
+  const long long step = (long long)gridDim.x * slots;
   int phase = 0;
-  for (long long r0 = (long long)blockIdx.x * slots; r0 < p.rows; r0 += (long long)gridDim.x * slots) {
-    const long long r = r0 + slot;
-    const bool live = r < p.rows;
-    const float2 st = live ? stats[r] : make_float2(0.f, 0.f);
-    float xh[NV][V], g[NV][V];
+  long long r = (long long)blockIdx.x * slots + slot;
+  nx.load(x + r * p.xs, lane, tpr, p.C, r < p.rows);
+  ng.load(dy + r * p.dys, lane, tpr, p.C, r < p.rows);
+  float2 ns = r < p.rows ? stats[r] : make_float2(0.f, 0.f);
+  for (long long r0 = BLOCK ? r : (long long)blockIdx.x * slots; r0 < p.rows; r0 += step, r += step) {
+    const bool live = r < p.rows, more = r + step < p.rows;
+    const RowPart<T, V, NV> cx = nx, cg = ng;
+    const float2 st = ns;
+    nx.load(x + (r + step) * p.xs, lane, tpr, p.C, more);
+    ng.load(dy + (r + step) * p.dys, lane, tpr, p.C, more);
+    ns = more ? stats[r + step] : make_float2(0.f, 0.f);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (j * p.tpr + lane) * V;
-      typename P::Raw rx = P::zero(), rg = P::zero();
-      const bool on = live && c < p.C;
-      if (on) {
-        rx = P::load(x + r * p.xs + c);
-        rg = P::load(dy + r * p.dys + c);
-      }
-      P::unpack(rx, xh[j]);
-      P::unpack(rg, g[j]);
+      float xv[V], g[V], wv[V];
+      cx.get(j, xv);
+      cg.get(j, g);  // zeros beyond the row: they count nowhere
+      if (w) wr.get(j, wv);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        xh[j][i] = on ? (xh[j][i] - st.x) * st.y : 0.f;
-        const float q = g[j][i] * wv[j][i];
+        const float xh = (xv[i] - st.x) * st.y, q = w ? g[i] * wv[i] : g[i];
         s1 += q;
-        s2 = fmaf(q, xh[j][i], s2);
-        dw[j][i] = fmaf(g[j][i], xh[j][i], dw[j][i]);
-        db[j][i] += g[j][i];
+        s2 = fmaf(q, xh, s2);
+        dw[j][i] = fmaf(g[i], xh, dw[j][i]);
+        db[j][i] += g[i];
       }
     }
-    if constexpr (!BLOCK) {
-      s1 = lanes_sum(s1, p.tpr);
-      s2 = lanes_sum(s2, p.tpr);
-    } else {
-      s1 = lanes_sum(s1, 32);
-      s2 = lanes_sum(s2, 32);
-      if ((tid & 31) == 0) red[phase][tid >> 5] = make_float2(s1, s2);
-      __syncthreads();
+    s1 = lanes_sum(s1, BLOCK ? 32 : tpr);
+    s2 = lanes_sum(s2, BLOCK ? 32 : tpr);
+    if constexpr (BLOCK) {
+      const int nw = tpr >> 5;
+      float2 *mine = red[phase] + slot * nw;
+      if ((threadIdx.x & 31) == 0) mine[lane >> 5] = make_float2(s1, s2);
+      row_sync(slot, tpr);
       s1 = s2 = 0.f;
-      for (int i = 0; i < (p.tpr >> 5); ++i) {
-        s1 += red[phase][i].x;
-        s2 += red[phase][i].y;
+      for (int i = 0; i < nw; ++i) {
+        s1 += mine[i].x;
+        s2 += mine[i].y;
       }
       phase ^= 1;
     }
     s1 *= inv;
     s2 *= inv;
+    T *dr = dx + r * p.C;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (j * p.tpr + lane) * V;
+      const int c = (j * tpr + lane) * V;
       if (!live || c >= p.C) continue;
-      float o[V];
+      float xv[V], g[V], wv[V];
+      cx.get(j, xv);
+      cg.get(j, g);
+      if (w) wr.get(j, wv);
 #pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = st.y * (g[j][i] * wv[j][i] - s1 - xh[j][i] * s2);
-      P::store(dx + r * p.C + c, P::pack(o));
+      for (int i = 0; i < V; ++i) {
+        const float xh = (xv[i] - st.x) * st.y, q = w ? g[i] * wv[i] : g[i];
+        xv[i] = st.y * (q - s1 - xh * s2);
+      }
+      P::store(dr + c, P::pack(xv));
     }
   }
   if (part == nullptr) return;
-  float *mine = part + (long long)blockIdx.x * 2 * p.C;
-  if constexpr (BLOCK) {
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * p.tpr + lane) * V;
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (c + i < p.C) {
-          mine[c + i] = dw[j][i];
-          mine[p.C + c + i] = db[j][i];
-        }
-    }
-  } else {
-    // rows of a warp by shuffles, then warp after warp in order
-    const int cols = NV * p.tpr * V;
+  // rows of a warp by shuffles, then slot after slot (warp after warp) in order
+  const int cols = NV * tpr * V, turns = BLOCK ? slots : (int)(blockDim.x >> 5);
+  const int turn = BLOCK ? slot : (int)(threadIdx.x >> 5);
+  if constexpr (!BLOCK) {
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        for (int o = p.tpr; o < 32; o <<= 1) {
+        for (int o = tpr; o < 32; o <<= 1) {
           dw[j][i] += __shfl_xor_sync(0xffffffffu, dw[j][i], o);
           db[j][i] += __shfl_xor_sync(0xffffffffu, db[j][i], o);
         }
-    for (int k = 0; k < (int)(blockDim.x >> 5); ++k) {
-      if ((tid >> 5) == k && (tid & 31) < p.tpr) {
+  }
+  for (int k = 0; k < turns; ++k) {
+    if (turn == k && (BLOCK || (threadIdx.x & 31) < tpr)) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+      for (int j = 0; j < NV; ++j)
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const int c = (j * p.tpr + lane) * V + i;
-            acc_s[c] = (k ? acc_s[c] : 0.f) + dw[j][i];
-            acc_s[cols + c] = (k ? acc_s[cols + c] : 0.f) + db[j][i];
-          }
-      }
-      __syncthreads();
+        for (int i = 0; i < V; ++i) {
+          const int c = (j * tpr + lane) * V + i;
+          acc_s[c] = (k ? acc_s[c] : 0.f) + dw[j][i];
+          acc_s[cols + c] = (k ? acc_s[cols + c] : 0.f) + db[j][i];
+        }
     }
-    for (int c = tid; c < p.C; c += blockDim.x) {
-      mine[c] = acc_s[c];
-      mine[p.C + c] = acc_s[cols + c];
-    }
+    __syncthreads();
+  }
+  float *mine = part + (long long)blockIdx.x * 2 * p.C;
+  for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
+    mine[c] = acc_s[c];
+    mine[p.C + c] = acc_s[cols + c];
   }
 }
 
@@ -331,83 +335,76 @@ inline int pow2_at_least(int v) {
   return p;
 }
 
-// The split of a row with the fewest idle places; among equals the one with most values per thread
-// (fewer steps in the row's sums).
-inline NormShape norm_shape(int C, int V, bool backward) {
-  static const int nv16[] = {1, 2, 3, 0}, nv8[] = {1, 2, 3, 4, 0}, nv1[] = {1, 2, 4, 8, 16, 0};
-  const int *nv = V == 8 ? nv16 : V == 4 ? nv8 : nv1;
-  NormShape best{V, 0, 0};
+// The split of a row among threads that hold at most 16 values (8 in vectors of one element) with the
+// fewest idle places; among equals the one with most values per thread (fewer steps in the row's sums).
+// `es`: bytes of an element, 0: vectors of one element only.
+inline NormShape norm_shape(int C, int es) {
+  static const NormShape choices[] = {{8, 1, 0}, {8, 2, 0}, {4, 1, 0}, {4, 2, 0}, {4, 3, 0}, {4, 4, 0}, {1, 1, 0}, {1, 2, 0}, {1, 4, 0}, {1, 8, 0}};
+  NormShape best{1, 0, 0};
   long long cost = 0;
-  for (; *nv; ++nv) {
-    const int tpr = pow2_at_least(ceil_div(C / V, *nv));
-    if (tpr > norm_max_tpr(V * *nv, backward)) continue;
-    if (best.tpr == 0 || (long long)tpr * *nv <= cost) {
-      best = NormShape{V, *nv, tpr};
-      cost = (long long)tpr * *nv;
+  for (const NormShape &n : choices) {
+    if (n.V != 1 ? (es == 0 || n.V * es > 16 || C % n.V != 0) : es != 0) continue;
+    const int tpr = pow2_at_least(ceil_div(C / n.V, n.NV));
+    if (tpr > NORM_CTA) continue;
+    const long long places = (long long)tpr * n.NV * n.V;
+    if (best.tpr == 0 || places < cost || (places == cost && n.V * n.NV > best.V * best.NV)) {
+      best = NormShape{n.V, n.NV, tpr};
+      cost = places;
     }
   }
   return best;
 }
 
-inline int norm_forward_grid(long long rows, int slots) {
-  const long long g = ceil_div_ll(rows, slots), cap = 148ll * 64;
-  return (int)(g < cap ? g : cap);
+// CTAs: enough to fill every SM, each staying for many rows.
+inline int norm_grid(long long rows, int slots, int per_sm) {
+  const long long g = ceil_div_ll(rows, slots), most = 148ll * per_sm;
+  return (int)(g < most ? g : most);
 }
-// CTAs of the backward kernels, one part of the weight gradient each.
-inline int norm_backward_parts(long long rows) { return (int)(rows < 148 * 4 ? rows : 148 * 4); }
+constexpr int NORM_PARTS = 148 * 4;  // most CTAs of the backward kernels, one part of the weight gradient each
 
 template <typename T, int V, int NV>
 void launch_forward(const T *x, const T *w, const T *b, T *y, float2 *stats, const NormParams &p, cudaStream_t st) {
   if (p.tpr > 32)
-    norm_forward_kernel<T, V, NV, true><<<norm_forward_grid(p.rows, 1), p.tpr, 0, st>>>(x, w, b, y, stats, p);
+    norm_forward_kernel<T, V, NV, true>
+        <<<norm_grid(p.rows, NORM_CTA / p.tpr, 2), NORM_CTA, 0, st>>>(x, w, b, y, stats, p);
   else
     norm_forward_kernel<T, V, NV, false>
-        <<<norm_forward_grid(p.rows, NORM_ROW_THREADS / p.tpr), NORM_ROW_THREADS, 0, st>>>(x, w, b, y, stats, p);
+        <<<norm_grid(p.rows, NORM_ROW_THREADS / p.tpr, 12), NORM_ROW_THREADS, 0, st>>>(x, w, b, y, stats, p);
 }
 
 template <typename T, int V, int NV>
-void launch_backward(const T *x, const T *w, const float2 *stats, const T *dy, T *dx, float *part, int parts,
-                     const NormParams &p, cudaStream_t st) {
-  if (p.tpr > 32)
-    norm_backward_kernel<T, V, NV, true><<<parts, p.tpr, 0, st>>>(x, w, stats, dy, dx, part, p);
-  else
-    norm_backward_kernel<T, V, NV, false><<<parts, NORM_ROW_THREADS, 2 * NV * p.tpr * V * sizeof(float), st>>>(
-        x, w, stats, dy, dx, part, p);
+int launch_backward(const T *x, const T *w, const float2 *stats, const T *dy, T *dx, float *part,
+                    const NormParams &p, cudaStream_t st) {
+  const size_t smem = part ? 2 * NV * p.tpr * V * sizeof(float) : 0;
+  const int grid = p.tpr > 32 ? norm_grid(p.rows, NORM_CTA / p.tpr, 1) : norm_grid(p.rows, NORM_ROW_THREADS / p.tpr, 4);
+  if (p.tpr > 32) {
+    if (smem > 40 * 1024)
+      (void)cudaFuncSetAttribute(norm_backward_kernel<T, V, NV, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 2 * NV * NORM_CTA * V * (int)sizeof(float));
+    norm_backward_kernel<T, V, NV, true><<<grid, NORM_CTA, smem, st>>>(x, w, stats, dy, dx, part, p);
+  } else {
+    norm_backward_kernel<T, V, NV, false><<<grid, NORM_ROW_THREADS, smem, st>>>(x, w, stats, dy, dx, part, p);
+  }
+  return grid;
 }
 
-#define DWB_NORM_SWITCH(FN, ...)                                        \
-  switch (sh.V * 100 + sh.NV) {                                         \
-    case 101: FN<T, 1, 1>(__VA_ARGS__); break;                          \
-    case 102: FN<T, 1, 2>(__VA_ARGS__); break;                          \
-    case 104: FN<T, 1, 4>(__VA_ARGS__); break;                          \
-    case 108: FN<T, 1, 8>(__VA_ARGS__); break;                          \
-    case 116: FN<T, 1, 16>(__VA_ARGS__); break;                         \
-    default: FN##_vec<T, 16 / (int)sizeof(T)>(__VA_ARGS__, sh.NV); break; \
+// FN<T, V, NV>(...) for the shape `sh`
+#define DWB_NORM_SWITCH(FN, ...)                            \
+  switch (sh.V * 100 + sh.NV) {                             \
+    case 101: FN<T, 1, 1>(__VA_ARGS__); break;              \
+    case 102: FN<T, 1, 2>(__VA_ARGS__); break;              \
+    case 104: FN<T, 1, 4>(__VA_ARGS__); break;              \
+    case 108: FN<T, 1, 8>(__VA_ARGS__); break;              \
+    case 401: FN<T, 4, 1>(__VA_ARGS__); break;              \
+    case 402: FN<T, 4, 2>(__VA_ARGS__); break;              \
+    case 403: FN<T, 4, 3>(__VA_ARGS__); break;              \
+    case 404: FN<T, 4, 4>(__VA_ARGS__); break;              \
+    default:                                                \
+      if constexpr (sizeof(T) == 2) {                       \
+        if (sh.NV == 1) FN<T, 8, 1>(__VA_ARGS__);           \
+        else FN<T, 8, 2>(__VA_ARGS__);                      \
+      }                                                     \
   }
-
-
-template <typename T, int V>
-void launch_forward_vec(const T *x, const T *w, const T *b, T *y, float2 *stats, const NormParams &p,
-                        cudaStream_t st, int nv) {
-  switch (nv) {
-    case 1: launch_forward<T, V, 1>(x, w, b, y, stats, p, st); break;
-    case 2: launch_forward<T, V, 2>(x, w, b, y, stats, p, st); break;
-    case 3: launch_forward<T, V, 3>(x, w, b, y, stats, p, st); break;
-    default:
-      if constexpr (V == 4) launch_forward<T, V, 4>(x, w, b, y, stats, p, st);
-  }
-}
-template <typename T, int V>
-void launch_backward_vec(const T *x, const T *w, const float2 *stats, const T *dy, T *dx, float *part, int parts,
-                         const NormParams &p, cudaStream_t st, int nv) {
-  switch (nv) {
-    case 1: launch_backward<T, V, 1>(x, w, stats, dy, dx, part, parts, p, st); break;
-    case 2: launch_backward<T, V, 2>(x, w, stats, dy, dx, part, parts, p, st); break;
-    case 3: launch_backward<T, V, 3>(x, w, stats, dy, dx, part, parts, p, st); break;
-    default:
-      if constexpr (V == 4) launch_backward<T, V, 4>(x, w, stats, dy, dx, part, parts, p, st);
-  }
-}
 
 template <typename T>
 void forward_t(const void *xv, const void *wv, const void *bv, void *yv, float *stats, NormParams p, cudaStream_t st) {
@@ -417,7 +414,7 @@ void forward_t(const void *xv, const void *wv, const void *bv, void *yv, float *
   constexpr int V = 16 / sizeof(T);
   const bool vec = p.C % V == 0 && p.xs % V == 0 && aligned_to(x, 16) && aligned_to(y, 16) &&
                    (!w || aligned_to(w, 16)) && (!b || aligned_to(b, 16));
-  const NormShape sh = norm_shape(p.C, vec ? V : 1, false);
+  const NormShape sh = norm_shape(p.C, vec ? (int)sizeof(T) : 0);
   p.tpr = sh.tpr;
   if (sh.tpr == 0) {
     const int grid = (int)(p.rows < 148 * 2 ? p.rows : 148 * 2);
@@ -427,22 +424,25 @@ void forward_t(const void *xv, const void *wv, const void *bv, void *yv, float *
   DWB_NORM_SWITCH(launch_forward, x, w, b, y, s2, p, st)
 }
 
+// Returns the parts of the weight gradient.
 template <typename T>
-void backward_t(const void *xv, const void *wv, const float *stats, const void *dyv, void *dxv, float *part,
-                int parts, NormParams p, cudaStream_t st) {
+int backward_t(const void *xv, const void *wv, const float *stats, const void *dyv, void *dxv, float *part,
+               NormParams p, cudaStream_t st) {
   const T *x = static_cast<const T *>(xv), *w = static_cast<const T *>(wv), *dy = static_cast<const T *>(dyv);
   T *dx = static_cast<T *>(dxv);
   const float2 *s2 = reinterpret_cast<const float2 *>(stats);
   constexpr int V = 16 / sizeof(T);
   const bool vec = p.C % V == 0 && p.xs % V == 0 && p.dys % V == 0 && aligned_to(x, 16) && aligned_to(dy, 16) &&
                    aligned_to(dx, 16) && (!w || aligned_to(w, 16));
-  const NormShape sh = norm_shape(p.C, vec ? V : 1, true);
+  const NormShape sh = norm_shape(p.C, vec ? (int)sizeof(T) : 0);
   p.tpr = sh.tpr;
+  int parts = (int)(p.rows < 148 * 2 ? p.rows : 148 * 2);
   if (sh.tpr == 0) {
     norm_backward_wide_kernel<T><<<parts, WIDE_THREADS, 0, st>>>(x, w, s2, dy, dx, part, p);
-    return;
+    return parts;
   }
-  DWB_NORM_SWITCH(launch_backward, x, w, s2, dy, dx, part, parts, p, st)
+  DWB_NORM_SWITCH(parts = launch_backward, x, w, s2, dy, dx, part, p, st)
+  return parts;
 }
 
 int check_norm(int dtype, long long rows, int C) {
@@ -481,7 +481,7 @@ int dwconv_b200_layer_norm(const void *x, long long x_stride, const void *w, con
 
 size_t dwconv_b200_layer_norm_workspace_bytes(int dtype, long long rows, int C) {
   if (check_norm(dtype, rows, C) != DWCONV_B200_OK) return 0;
-  const size_t n = (size_t)norm_backward_parts(rows) * 2 * C * sizeof(float);
+  const size_t n = (size_t)(rows < NORM_PARTS ? rows : NORM_PARTS) * 2 * C * sizeof(float);
   return (n + 15) / 16 * 16 + 16;
 }
 
@@ -504,12 +504,12 @@ int dwconv_b200_layer_norm_backward(const void *x, long long x_stride, const voi
   const NormParams p{rows, x_stride, dy_stride, C, 0, 0.f};
   cudaStream_t st = (cudaStream_t)stream;
   float *part = params ? static_cast<float *>(workspace) : nullptr;
-  const int parts = norm_backward_parts(rows);
+  int parts = 0;
   if (rows > 0) {
     switch (dtype) {
-      case DWCONV_B200_F32: backward_t<float>(x, w, stats, dy, dx, part, parts, p, st); break;
-      case DWCONV_B200_F16: backward_t<__half>(x, w, stats, dy, dx, part, parts, p, st); break;
-      default: backward_t<__nv_bfloat16>(x, w, stats, dy, dx, part, parts, p, st); break;
+      case DWCONV_B200_F32: parts = backward_t<float>(x, w, stats, dy, dx, part, p, st); break;
+      case DWCONV_B200_F16: parts = backward_t<__half>(x, w, stats, dy, dx, part, p, st); break;
+      default: parts = backward_t<__nv_bfloat16>(x, w, stats, dy, dx, part, p, st); break;
     }
     e = api_launch_status();
     if (e) return e;

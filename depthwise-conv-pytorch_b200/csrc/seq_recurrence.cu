@@ -52,47 +52,14 @@ constexpr float REC_SERIES = 0.125f;
 
 // ---- arithmetic on channel pairs ---------------------------------------------------------------
 
-__device__ __forceinline__ float2 f2(float v) { return make_float2(v, v); }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
-__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
 // The same value, of which the compiler does not know that: what is computed from it again is not kept in
 // a register meanwhile.
 __device__ __forceinline__ void forget(float2 &v) { asm volatile("" : "+f"(v.x), "+f"(v.y)); }
 
-__device__ __forceinline__ float ex2f(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-__device__ __forceinline__ float rcpf(float v) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-__device__ __forceinline__ float rsqf(float v) {
-  float r;
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-
-constexpr float LOG2E = 1.4426950408889634f;
-
-// 1 + exp(-v)
-__device__ __forceinline__ float2 one_plus_exp2(float2 v) {
-  const float2 e = mul2(v, f2(-LOG2E));
-  return add2(make_float2(ex2f(e.x), ex2f(e.y)), f2(1.f));
-}
-// sigmoid and its square root; an overflowing exponential gives 0
-__device__ __forceinline__ float2 sigmoid2(float2 v) {
-  const float2 s = one_plus_exp2(v);
-  return make_float2(rcpf(s.x), rcpf(s.y));
-}
 __device__ __forceinline__ float2 root_sigmoid2(float2 v) {
   const float2 s = one_plus_exp2(v);
   return make_float2(rsqf(s.x), rsqf(s.y));
 }
-__device__ __forceinline__ float2 one_minus2(float2 v) { return fma2(v, f2(-1.f), f2(1.f)); }
 
 __device__ __forceinline__ float2 horner2(float2 p, float2 s, float c) { return fma2(p, s, f2(c)); }
 // exp(s) - 1, p(-s) and 1 / p(-s) for -REC_SERIES <= s <= 0, from the Taylor expansions of
