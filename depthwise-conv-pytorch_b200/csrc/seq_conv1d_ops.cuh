@@ -1,0 +1,70 @@
+// What the translation units of the causal depthwise convolution share: its arguments, and how a
+// problem is cut into runs of rows.
+#pragma once
+
+#include "seq_common.cuh"
+
+namespace dwb {
+
+constexpr int CONV_WARPS = 8;
+
+struct Conv1dParams {
+  SeqList q;
+  int R;           // rows of a run
+  int cblocks;     // channel blocks
+  int rblocks;     // blocks of CONV_WARPS runs per batch element
+  long long main;  // CTAs that walk rows; those behind them fill the states
+  int act;
+};
+
+struct ConvArgs {
+  const dwconv_b200_rows *x, *dy;
+  const void *w, *bias, *initial, *dfin;
+  void *y, *fin, *dx, *dinit;
+  float *part;
+  const dwconv_b200_sequence *s;
+  int taps, act;
+};
+
+// Rows of a run: the choice whose rounds of resident warps (24 per SM forward, 16 backward), each a run and
+// what it costs beside its rows, take least.  That cost is worth 5 rows forward (the filter, the K-1 rows
+// in front) and 12 backward (those on both sides, the sums at the end).  Measured on 4 x 4096 rows of 2560
+// channels in bf16, four taps, with runs of 16 / 32 / 48 / 64 / 128 rows: forward 46 / 44 / 44 / 47 / 49 us,
+// backward 134 / 107 / 99 / 105 / 118 us; the rule takes 48 for both.
+inline int conv_run(const dwconv_b200_sequence &s, int group, bool backward) {
+  static const int runs[] = {8, 16, 24, 32, 48, 64, 96, 128};
+  const long long slots = 148 * (backward ? 16 : 24), per_row = (long long)s.B * ceil_div(s.C, group);
+  int best = runs[0];
+  long long cost = 0;
+  for (int R : runs) {
+    const long long c = ceil_div_ll(per_row * ceil_div(s.T, R), slots) * (R + (backward ? 12 : 5));
+    if (R == runs[0] || c < cost) {
+      best = R;
+      cost = c;
+    }
+  }
+  return best;
+}
+
+inline Conv1dParams conv_params(const dwconv_b200_sequence &s, int group, int act, bool backward) {
+  Conv1dParams p;
+  p.q = seq_list(s);
+  p.R = conv_run(s, group, backward);
+  p.cblocks = ceil_div(s.C, group);
+  p.rblocks = ceil_div(ceil_div(s.T, p.R), CONV_WARPS);
+  p.main = (long long)p.cblocks * p.rblocks * s.B;
+  p.act = act;
+  return p;
+}
+
+constexpr int STATE_BLOCKS = 64;  // most CTAs that fill the states
+
+// One translation unit per element type (seq_conv1d_f32.cu, seq_conv1d_f16.cu, seq_conv1d_bf16.cu).
+template <typename T> void conv1d_forward(const ConvArgs &a, cudaStream_t st);
+// Returns the parts of the filter's gradient.
+template <typename T> long long conv1d_backward(const ConvArgs &a, cudaStream_t st);
+template <typename T>
+void conv1d_step(const void *x, long long xs, const void *w, const void *bias, void *state, void *y, int B, int C,
+                 int taps, int act, cudaStream_t st);
+
+}  // namespace dwb
