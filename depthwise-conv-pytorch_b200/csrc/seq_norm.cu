@@ -46,9 +46,12 @@ template <int V, int NV> __device__ __forceinline__ float warp_count(int C, int 
   return (float)(n * V);
 }
 
-// A thread's part of a row: NV vectors, tpr vectors apart.
+// A thread's part of a row: NV vectors of V elements, tpr vectors apart, zeros beyond the row.
 template <typename T, int V, int NV> struct RowPart {
   using P = Pack<T, V>;
+  // the values of one vector, two to an instruction; the second half of a vector of one element is a zero
+  // that no sum takes in
+  static constexpr int H = (V + 1) / 2;
   typename P::Raw raw[NV];
   __device__ __forceinline__ void load(const T *row, int lane, int tpr, int C, bool live) {
 #pragma unroll
@@ -58,7 +61,23 @@ template <typename T, int V, int NV> struct RowPart {
       if (live && c < C) raw[j] = P::load(row + c);
     }
   }
-  __device__ __forceinline__ void get(int j, float (&f)[V]) const { P::unpack(raw[j], f); }
+  __device__ __forceinline__ void get(int j, float2 (&v)[H]) const { unpack(raw[j], v); }
+  static __device__ __forceinline__ void unpack(const typename P::Raw &r, float2 (&v)[H]) {
+    float f[V];
+    P::unpack(r, f);
+#pragma unroll
+    for (int h = 0; h < H; ++h) v[h] = make_float2(f[2 * h], V > 1 ? f[(2 * h + 1) % V] : 0.f);
+  }
+  static __device__ __forceinline__ typename P::Raw pack(const float2 (&v)[H]) {
+    float f[V];
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      f[2 * h] = v[h].x;
+      if (V > 1) f[(2 * h + 1) % V] = v[h].y;
+    }
+    return P::pack(f);
+  }
+  static __device__ __forceinline__ float total(float2 v) { return V > 1 ? v.x + v.y : v.x; }
 };
 
 // BLOCK: rows of tpr > 32 threads, blockDim / tpr of them at a time; otherwise 32 / tpr rows per warp.
@@ -66,11 +85,18 @@ template <typename T, int V, int NV, bool BLOCK>
 __global__ void __launch_bounds__(BLOCK ? NORM_CTA : NORM_ROW_THREADS, BLOCK ? 2 : 6)
 norm_forward_kernel(const T *__restrict__ x, const T *__restrict__ w, const T *__restrict__ b, T *__restrict__ y,
                     float2 *stats, NormParams p) {
-  using P = Pack<T, V>;
+  using R = RowPart<T, V, NV>;
+  using P = typename R::P;
+  constexpr int H = R::H;
   __shared__ float2 red[2][NORM_CTA / 32];
   const int tpr = p.tpr, lane = threadIdx.x & (tpr - 1), slot = threadIdx.x / tpr, slots = blockDim.x / tpr;
-  RowPart<T, V, NV> next;
+  R next;
   const float inv = 1.f / (float)p.C;
+  const int nw = tpr >> 5, wid = lane >> 5, other = BLOCK ? threadIdx.x & (nw - 1) : 0;
+  // this warp's elements, and those of the warp whose moments this lane folds
+  const float mine_n = BLOCK ? warp_count<V, NV>(p.C, tpr, wid) : 0.f;
+  const float mine_inv = mine_n > 0.f ? 1.f / mine_n : 0.f;
+  const float other_n = BLOCK ? warp_count<V, NV>(p.C, tpr, other) : 0.f;
   const long long step = (long long)gridDim.x * slots;
   int phase = 0;
   long long r = (long long)blockIdx.x * slots + slot;
@@ -78,62 +104,55 @@ norm_forward_kernel(const T *__restrict__ x, const T *__restrict__ w, const T *_
   // the rows of a warp go on together (shuffles); those of different warps need not
   for (long long r0 = BLOCK ? r : (long long)blockIdx.x * slots; r0 < p.rows; r0 += step, r += step) {
     const bool live = r < p.rows;
-    const RowPart<T, V, NV> cur = next;
+    float2 f[NV][H];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) next.get(j, f[j]);
     next.load(x + (r + step) * p.xs, lane, tpr, p.C, r + step < p.rows);
-    float sum = 0.f;
+    float2 sum2 = f2(0.f), sq2 = f2(0.f);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      float f[V];
-      cur.get(j, f);
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int i = 0; i < V; ++i) sum += f[i];
-    }
-    float mean, rstd, centre, sq = 0.f;
-    const int wid = lane >> 5;
-    const float n = BLOCK ? warp_count<V, NV>(p.C, tpr, wid) : (float)p.C;
-    sum = lanes_sum(sum, BLOCK ? 32 : tpr);
-    centre = BLOCK ? (n > 0.f ? sum / n : 0.f) : sum * inv;
+      for (int h = 0; h < H; ++h) sum2 = add2(sum2, f[j][h]);
+    const float sum = lanes_sum(R::total(sum2), BLOCK ? 32 : tpr);
+    float mean = sum * (BLOCK ? mine_inv : inv);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      float f[V];
-      cur.get(j, f);
+    for (int j = 0; j < NV; ++j)
       if ((j * tpr + lane) * V < p.C) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) sq = fmaf(f[i] - centre, f[i] - centre, sq);
+        for (int h = 0; h < H; ++h) {
+          const float2 d = add2(f[j][h], f2(-mean));
+          sq2 = fma2(d, d, sq2);
+        }
       }
-    }
-    sq = lanes_sum(sq, BLOCK ? 32 : tpr);
-    if constexpr (!BLOCK) {
-      mean = centre;
-    } else {
-      const int nw = tpr >> 5;
+    float sq = lanes_sum(R::total(sq2), BLOCK ? 32 : tpr);
+    if constexpr (BLOCK) {
       float2 *mine = red[phase] + slot * nw;
-      if ((threadIdx.x & 31) == 0) mine[wid] = make_float2(centre, sq);
+      if ((threadIdx.x & 31) == 0) mine[wid] = make_float2(mean, sq);
       row_sync(slot, tpr);
-      float m = 0.f;
-      for (int i = 0; i < nw; ++i) m = fmaf(warp_count<V, NV>(p.C, tpr, i), mine[i].x, m);
-      mean = m * inv;
-      sq = 0.f;
-      for (int i = 0; i < nw; ++i) {
-        const float d = mine[i].x - mean;
-        sq += mine[i].y + warp_count<V, NV>(p.C, tpr, i) * d * d;
-      }
+      const float2 o = mine[other];
+      mean = lanes_sum(other_n * o.x, nw) * inv;
+      const float d = o.x - mean;
+      sq = lanes_sum(fmaf(other_n * d, d, o.y), nw);
       phase ^= 1;  // the other half: a fast warp may be a row ahead, never two
     }
-    rstd = rsqrtf(sq * inv + p.eps);
+    const float rstd = rsqrtf(sq * inv + p.eps);
     if (stats != nullptr && live && lane == 0) stats[r] = make_float2(mean, rstd);
     T *yr = y + r * p.C;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * tpr + lane) * V;
       if (!live || c >= p.C) continue;
-      float f[V], wv[V], bv[V];
-      cur.get(j, f);
-      if (w) P::unpack(P::load(w + c), wv);  // out of L1
-      if (b) P::unpack(P::load(b + c), bv);
+      float2 wv[H], bv[H];  // out of L1
 #pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = fmaf((f[i] - mean) * rstd, w ? wv[i] : 1.f, b ? bv[i] : 0.f);
-      P::store(yr + c, P::pack(f));
+      for (int h = 0; h < H; ++h) {
+        wv[h] = f2(1.f);
+        bv[h] = f2(0.f);
+      }
+      if (w) R::unpack(P::load(w + c), wv);
+      if (b) R::unpack(P::load(b + c), bv);
+#pragma unroll
+      for (int h = 0; h < H; ++h) f[j][h] = fma2(mul2(add2(f[j][h], f2(-mean)), f2(rstd)), wv[h], bv[h]);
+      P::store(yr + c, R::pack(f[j]));
     }
   }
 }
@@ -143,18 +162,21 @@ template <typename T, int V, int NV, bool BLOCK>
 __global__ void __launch_bounds__(BLOCK ? NORM_CTA : NORM_ROW_THREADS, BLOCK ? 1 : 4)
 norm_backward_kernel(const T *__restrict__ x, const T *__restrict__ w, const float2 *__restrict__ stats,
                      const T *__restrict__ dy, T *__restrict__ dx, float *__restrict__ part, NormParams p) {
-  using P = Pack<T, V>;
+  using R = RowPart<T, V, NV>;
+  using P = typename R::P;
+  constexpr int H = R::H;
   __shared__ float2 red[2][NORM_CTA / 32];
   extern __shared__ float acc_s[];
   const int tpr = p.tpr, lane = threadIdx.x & (tpr - 1), slot = threadIdx.x / tpr, slots = blockDim.x / tpr;
-  float dw[NV][V], db[NV][V];
+  float2 dw[NV][H], db[NV][H];
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int i = 0; i < V; ++i) dw[j][i] = db[j][i] = 0.f;
-  RowPart<T, V, NV> nx, ng, wr;
+    for (int h = 0; h < H; ++h) dw[j][h] = db[j][h] = f2(0.f);
+  R nx, ng, wr;
   if (w) wr.load(w, lane, tpr, p.C, true);
   const float inv = 1.f / (float)p.C;
+  const int nw = tpr >> 5;
   const long long step = (long long)gridDim.x * slots;
   int phase = 0;
   long long r = (long long)blockIdx.x * slots + slot;
@@ -163,85 +185,79 @@ norm_backward_kernel(const T *__restrict__ x, const T *__restrict__ w, const flo
   float2 ns = r < p.rows ? stats[r] : make_float2(0.f, 0.f);
   for (long long r0 = BLOCK ? r : (long long)blockIdx.x * slots; r0 < p.rows; r0 += step, r += step) {
     const bool live = r < p.rows, more = r + step < p.rows;
-    const RowPart<T, V, NV> cx = nx, cg = ng;
     const float2 st = ns;
+    float2 xh[NV][H], g[NV][H];  // dy is zero beyond the row: what stands there counts nowhere
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      nx.get(j, xh[j]);
+      ng.get(j, g[j]);
+    }
     nx.load(x + (r + step) * p.xs, lane, tpr, p.C, more);
     ng.load(dy + (r + step) * p.dys, lane, tpr, p.C, more);
     ns = more ? stats[r + step] : make_float2(0.f, 0.f);
-    float s1 = 0.f, s2 = 0.f;
+    float2 a1 = f2(0.f), a2 = f2(0.f);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      float xv[V], g[V], wv[V];
-      cx.get(j, xv);
-      cg.get(j, g);  // zeros beyond the row: they count nowhere
+      float2 wv[H];
       if (w) wr.get(j, wv);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float xh = (xv[i] - st.x) * st.y, q = w ? g[i] * wv[i] : g[i];
-        s1 += q;
-        s2 = fmaf(q, xh, s2);
-        dw[j][i] = fmaf(g[i], xh, dw[j][i]);
-        db[j][i] += g[i];
+      for (int h = 0; h < H; ++h) {
+        xh[j][h] = mul2(add2(xh[j][h], f2(-st.x)), f2(st.y));
+        dw[j][h] = fma2(g[j][h], xh[j][h], dw[j][h]);
+        db[j][h] = add2(db[j][h], g[j][h]);
+        if (w) g[j][h] = mul2(g[j][h], wv[h]);  // q from here on
+        a1 = add2(a1, g[j][h]);
+        a2 = fma2(g[j][h], xh[j][h], a2);
       }
     }
-    s1 = lanes_sum(s1, BLOCK ? 32 : tpr);
-    s2 = lanes_sum(s2, BLOCK ? 32 : tpr);
+    float s1 = lanes_sum(R::total(a1), BLOCK ? 32 : tpr), s2 = lanes_sum(R::total(a2), BLOCK ? 32 : tpr);
     if constexpr (BLOCK) {
-      const int nw = tpr >> 5;
       float2 *mine = red[phase] + slot * nw;
       if ((threadIdx.x & 31) == 0) mine[lane >> 5] = make_float2(s1, s2);
       row_sync(slot, tpr);
-      s1 = s2 = 0.f;
-      for (int i = 0; i < nw; ++i) {
-        s1 += mine[i].x;
-        s2 += mine[i].y;
-      }
+      const float2 o = mine[threadIdx.x & (nw - 1)];
+      s1 = lanes_sum(o.x, nw);
+      s2 = lanes_sum(o.y, nw);
       phase ^= 1;
     }
-    s1 *= inv;
-    s2 *= inv;
+    s1 *= inv * st.y;
+    s2 *= inv * st.y;
     T *dr = dx + r * p.C;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * tpr + lane) * V;
       if (!live || c >= p.C) continue;
-      float xv[V], g[V], wv[V];
-      cx.get(j, xv);
-      cg.get(j, g);
-      if (w) wr.get(j, wv);
+      // rstd (q - mean(q) - xh mean(q xh))
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float xh = (xv[i] - st.x) * st.y, q = w ? g[i] * wv[i] : g[i];
-        xv[i] = st.y * (q - s1 - xh * s2);
-      }
-      P::store(dr + c, P::pack(xv));
+      for (int h = 0; h < H; ++h) g[j][h] = fma2(g[j][h], f2(st.y), fma2(xh[j][h], f2(-s2), f2(-s1)));
+      P::store(dr + c, R::pack(g[j]));
     }
   }
   if (part == nullptr) return;
   // rows of a warp by shuffles, then slot after slot (warp after warp) in order
   const int cols = NV * tpr * V, turns = BLOCK ? slots : (int)(blockDim.x >> 5);
   const int turn = BLOCK ? slot : (int)(threadIdx.x >> 5);
-  if constexpr (!BLOCK) {
+  auto each = [&](auto &&body) {  // body(value of dw, value of db, column)
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        for (int o = tpr; o < 32; o <<= 1) {
-          dw[j][i] += __shfl_xor_sync(0xffffffffu, dw[j][i], o);
-          db[j][i] += __shfl_xor_sync(0xffffffffu, db[j][i], o);
-        }
-  }
+        body(i & 1 ? dw[j][i / 2].y : dw[j][i / 2].x, i & 1 ? db[j][i / 2].y : db[j][i / 2].x,
+             (j * tpr + lane) * V + i);
+  };
+  if constexpr (!BLOCK)
+    each([&](float &v, float &u, int) {
+      for (int o = tpr; o < 32; o <<= 1) {
+        v += __shfl_xor_sync(0xffffffffu, v, o);
+        u += __shfl_xor_sync(0xffffffffu, u, o);
+      }
+    });
   for (int k = 0; k < turns; ++k) {
-    if (turn == k && (BLOCK || (threadIdx.x & 31) < tpr)) {
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int c = (j * tpr + lane) * V + i;
-          acc_s[c] = (k ? acc_s[c] : 0.f) + dw[j][i];
-          acc_s[cols + c] = (k ? acc_s[cols + c] : 0.f) + db[j][i];
-        }
-    }
+    if (turn == k && (BLOCK || (threadIdx.x & 31) < tpr))
+      each([&](float &v, float &u, int c) {
+        acc_s[c] = (k ? acc_s[c] : 0.f) + v;
+        acc_s[cols + c] = (k ? acc_s[cols + c] : 0.f) + u;
+      });
     __syncthreads();
   }
   float *mine = part + (long long)blockIdx.x * 2 * p.C;

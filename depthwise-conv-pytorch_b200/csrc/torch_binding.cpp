@@ -14,6 +14,11 @@
 // fused kernel).
 #include <torch/extension.h>
 
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
+
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
@@ -659,6 +664,200 @@ std::tuple<at::Tensor, OptTensor, OptTensor> layer_norm_backward(const at::Tenso
   return {dx, dw, db};
 }
 
+// ---- autograd nodes ---------------------------------------------------------------------
+// What the Python functions call: checks, the forward call and, where something wants a gradient, a node
+// of the autograd graph, without a trip through the interpreter in either direction.  Gradients are
+// first-order only (the message is the one of torch.autograd.function.once_differentiable).
+
+using torch::autograd::SavedVariable;
+using torch::autograd::variable_list;
+
+at::Tensor or_undefined(const OptTensor &t) { return t.has_value() ? *t : at::Tensor(); }
+OptTensor or_none(const at::Tensor &t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
+template <typename... T> bool wants_grad(const T &...t) {
+  return at::GradMode::is_enabled() && ((t.defined() && t.requires_grad()) || ...);
+}
+
+struct OnceNode : torch::autograd::Node {
+  variable_list apply(variable_list &&grads) override {
+    bool twice = false, any = false;
+    for (const at::Tensor &g : grads) {
+      any = any || g.defined();
+      twice = twice || (g.defined() && g.requires_grad());
+    }
+    variable_list out(num_outputs());
+    if (!any) return out;
+    {
+      at::AutoGradMode no_grad(false);
+      backward(grads, out);
+    }
+    if (at::GradMode::is_enabled() && twice) {
+      auto error = std::make_shared<torch::autograd::DelayedError>(
+          "trying to differentiate twice a function that was marked with @once_differentiable", (int64_t)out.size());
+      for (at::Tensor &t : out)
+        if (t.defined()) t = t.detach().requires_grad_(true);
+      out = (*error)(std::move(out));
+    }
+    return out;
+  }
+  virtual void backward(const variable_list &grads, variable_list &out) = 0;
+  at::Tensor saved(SavedVariable &v) { return v.unpack(shared_from_this()); }
+  OptTensor saved_or_none(SavedVariable &v) { return or_none(v.unpack(shared_from_this())); }
+};
+
+template <typename N, typename... T> std::shared_ptr<N> new_node(const T &...inputs) {
+  std::shared_ptr<N> n(new N(), torch::autograd::deleteNode);
+  n->set_next_edges(torch::autograd::collect_next_edges(inputs...));
+  return n;
+}
+
+struct CausalConv1dNode : OnceNode {
+  SavedVariable input, weight, bias, initial, offsets;
+  int64_t act;
+  std::string name() const override { return "CausalConv1dBackward"; }
+  void release_variables() override {
+    for (SavedVariable *v : {&input, &weight, &bias, &initial, &offsets}) v->reset_data();
+  }
+  void backward(const variable_list &grads, variable_list &out) override {
+    auto [dx, dw, db, dinit] = conv1d_causal_backward(
+        saved(input), saved(weight), saved_or_none(bias), act, saved_or_none(initial), saved_or_none(offsets),
+        or_none(grads[0]), grads.size() > 1 ? or_none(grads[1]) : OptTensor(), task_should_compute_output(3));
+    out[0] = dx;
+    out[1] = dw;
+    out[2] = or_undefined(db);
+    out[3] = or_undefined(dinit);
+  }
+};
+
+py::object conv1d_causal_autograd(const at::Tensor &input, const at::Tensor &weight, const OptTensor &bias, int64_t act,
+                                  const OptTensor &initial, const OptTensor &offsets, bool want_state) {
+  const at::Tensor b = or_undefined(bias), h = or_undefined(initial);
+  at::Tensor y;
+  OptTensor state;
+  const bool grad = wants_grad(input, weight, b, h);
+  {
+    at::AutoGradMode no_grad(false);
+    std::tie(y, state) = conv1d_causal(input, weight, bias, act, initial, offsets, want_state);
+  }
+  if (grad) {
+    auto n = new_node<CausalConv1dNode>(input, weight, b, h);
+    n->input = SavedVariable(input, false);
+    n->weight = SavedVariable(weight, false);
+    n->bias = SavedVariable(b, false);
+    n->initial = SavedVariable(h, false);
+    n->offsets = SavedVariable(or_undefined(offsets), false);
+    n->act = act;
+    torch::autograd::set_history(y, n);
+    if (want_state) torch::autograd::set_history(*state, n);
+  }
+  if (want_state) return py::make_tuple(y, *state);
+  return py::cast(y);
+}
+
+struct RecurrenceNode : OnceNode {
+  SavedVariable input, u, v, decay, initial, offsets;
+  at::Tensor ckpt;
+  double scale;
+  std::string name() const override { return "GatedLinearRecurrenceBackward"; }
+  void release_variables() override {
+    for (SavedVariable *s : {&input, &u, &v, &decay, &initial, &offsets}) s->reset_data();
+    ckpt.reset();
+  }
+  void backward(const variable_list &grads, variable_list &out) override {
+    auto [dx, du, dv, dd, dinit] = recurrence_backward(
+        saved(input), saved(u), saved(v), saved(decay), saved_or_none(initial), saved_or_none(offsets), scale, ckpt,
+        or_none(grads[0]), grads.size() > 1 ? or_none(grads[1]) : OptTensor(), task_should_compute_output(4));
+    out[0] = dx;
+    out[1] = du;
+    out[2] = dv;
+    out[3] = dd;
+    out[4] = or_undefined(dinit);
+  }
+};
+
+py::object recurrence_autograd(const at::Tensor &input, const at::Tensor &u, const at::Tensor &v,
+                               const at::Tensor &decay, const OptTensor &initial, const OptTensor &offsets,
+                               double scale, bool want_state) {
+  const at::Tensor h = or_undefined(initial);
+  at::Tensor y;
+  OptTensor state, ckpt;
+  const bool grad = wants_grad(input, u, v, decay, h);
+  {
+    at::AutoGradMode no_grad(false);
+    std::tie(y, state, ckpt) = recurrence(input, u, v, decay, initial, offsets, scale, want_state, grad);
+  }
+  if (grad) {
+    auto n = new_node<RecurrenceNode>(input, u, v, decay, h);
+    n->input = SavedVariable(input, false);
+    n->u = SavedVariable(u, false);
+    n->v = SavedVariable(v, false);
+    n->decay = SavedVariable(decay, false);
+    n->initial = SavedVariable(h, false);
+    n->offsets = SavedVariable(or_undefined(offsets), false);
+    n->ckpt = *ckpt;
+    n->scale = scale;
+    torch::autograd::set_history(y, n);
+    if (want_state) torch::autograd::set_history(*state, n);
+  }
+  if (want_state) return py::make_tuple(y, *state);
+  return py::cast(y);
+}
+
+struct LayerNormNode : OnceNode {
+  SavedVariable input, weight;
+  at::Tensor stats;
+  std::string name() const override { return "ChannelLayerNormBackward"; }
+  void release_variables() override {
+    input.reset_data();
+    weight.reset_data();
+    stats.reset();
+  }
+  void backward(const variable_list &grads, variable_list &out) override {
+    auto [dx, dw, db] = layer_norm_backward(saved(input), saved_or_none(weight), stats, grads[0],
+                                            task_should_compute_output(1), task_should_compute_output(2));
+    out[0] = dx;
+    out[1] = or_undefined(dw);
+    out[2] = or_undefined(db);
+  }
+};
+
+at::Tensor layer_norm_autograd(const at::Tensor &input, const OptTensor &weight, const OptTensor &bias, double eps) {
+  const at::Tensor w = or_undefined(weight), b = or_undefined(bias);
+  at::Tensor y;
+  OptTensor stats;
+  const bool grad = wants_grad(input, w, b);
+  {
+    at::AutoGradMode no_grad(false);
+    std::tie(y, stats) = layer_norm(input, weight, bias, eps, grad);
+  }
+  if (grad) {
+    auto n = new_node<LayerNormNode>(input, w, b);
+    n->input = SavedVariable(input, false);
+    n->weight = SavedVariable(w, false);
+    n->stats = *stats;
+    torch::autograd::set_history(y, n);
+  }
+  return y;
+}
+
+// The steps have no gradient: what would want one is refused.
+at::Tensor conv1d_causal_step_checked(const at::Tensor &input, const at::Tensor &weight, const at::Tensor &state,
+                                      const OptTensor &bias, int64_t act) {
+  TORCH_CHECK(!wants_grad(input, weight, state, or_undefined(bias)),
+              "dwconv_b200.depthwise_conv1d_causal_step: the state is updated in place and has no gradient; use "
+              "depthwise_conv1d_causal or torch.no_grad()");
+  return conv1d_causal_step(input, weight, state, bias, act);
+}
+
+at::Tensor recurrence_step_checked(const at::Tensor &input, const at::Tensor &u, const at::Tensor &v,
+                                   const at::Tensor &decay, const at::Tensor &state, double scale) {
+  TORCH_CHECK(!wants_grad(input, u, v, decay, state),
+              "dwconv_b200.gated_linear_recurrence_step: the state is updated in place and has no gradient; use "
+              "gated_linear_recurrence or torch.no_grad()");
+  return recurrence_step(input, u, v, decay, state, scale);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -678,4 +877,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("recurrence_step", &recurrence_step);
   m.def("layer_norm", &layer_norm);
   m.def("layer_norm_backward", &layer_norm_backward);
+  m.def("conv1d_causal_autograd", &conv1d_causal_autograd);
+  m.def("conv1d_causal_step_checked", &conv1d_causal_step_checked);
+  m.def("recurrence_autograd", &recurrence_autograd);
+  m.def("recurrence_step_checked", &recurrence_step_checked);
+  m.def("layer_norm_autograd", &layer_norm_autograd);
 }

@@ -393,6 +393,16 @@ _forms = _Forms(_native)
 
 
 # ---- autograd ----------------------------------------------------------------------------------
+# The compiled module has nodes of its own (no interpreter in the backward pass); these functions are
+# what runs without it, and where the device flags are checked after every call.
+
+_nodes = _native if not _lib.CHECK_STATUS else None
+
+
+def _check_flags(what):
+    if _lib.CHECK_STATUS:
+        _lib.check_device_status(what)
+
 
 def _wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
@@ -422,6 +432,7 @@ class CausalConv1dFunction(Function):
             return (None,) * 7
         dx, dw, db, dinit = _forms.conv1d_causal_backward(
             input, weight, bias, ctx.act, initial, offsets, grad, grad_state, ctx.needs_input_grad[3])
+        _check_flags("depthwise_conv1d_causal backward")
         return dx, dw, db, dinit, None, None, None
 
 
@@ -444,6 +455,7 @@ class GatedLinearRecurrenceFunction(Function):
         dx, du, dv, dd, dinit = _forms.recurrence_backward(
             input, u, v, decay, initial, offsets, ctx.scale, ckpt, grad, grad_state,
             ctx.needs_input_grad[4])
+        _check_flags("gated_linear_recurrence backward")
         return dx, du, dv, dd, dinit, None, None, None
 
 
@@ -460,6 +472,7 @@ class LayerNormFunction(Function):
         input, weight, stats = ctx.saved_tensors
         dx, dw, db = _forms.layer_norm_backward(input, weight, stats, grad, ctx.needs_input_grad[1],
                                                 ctx.needs_input_grad[2])
+        _check_flags("layer_norm backward")
         return dx, dw, db, None
 
 
@@ -480,6 +493,8 @@ def depthwise_conv1d_causal(input, weight, bias=None, activation=None, initial_s
     Gradients flow to input, weight, bias and initial state, and from output and returned state.
     """
     act = _activation(activation)
+    if _nodes is not None:
+        return _nodes.conv1d_causal_autograd(input, weight, bias, act, initial_state, offsets, bool(return_state))
     if _wants_grad(input, weight, bias, initial_state):
         return CausalConv1dFunction.apply(input, weight, bias, initial_state, offsets, act, bool(return_state))
     y, state = _forms.conv1d_causal(input, weight, bias, act, initial_state, offsets, bool(return_state))
@@ -491,6 +506,8 @@ def depthwise_conv1d_causal_step(input, weight, state, bias=None, activation=Non
     contiguous, updated in place.  The values of ``depthwise_conv1d_causal`` with T = 1.
     Inference only."""
     act = _activation(activation)
+    if _nodes is not None:
+        return _nodes.conv1d_causal_step_checked(input, weight, state, bias, act)
     if _wants_grad(input, weight, state, bias):
         raise RuntimeError("dwconv_b200.depthwise_conv1d_causal_step: the state is updated in place and "
                            "has no gradient; use depthwise_conv1d_causal or torch.no_grad()")
@@ -513,6 +530,9 @@ def gated_linear_recurrence(input, recurrence_gate, input_gate, decay, initial_s
     Gradients flow to input, both gates, decay and initial state, and from h and returned state.
     """
     scale = float(scale)
+    if _nodes is not None:
+        return _nodes.recurrence_autograd(input, recurrence_gate, input_gate, decay, initial_state, offsets, scale,
+                                          bool(return_state))
     if _wants_grad(input, recurrence_gate, input_gate, decay, initial_state):
         return GatedLinearRecurrenceFunction.apply(input, recurrence_gate, input_gate, decay, initial_state,
                                                    offsets, scale, bool(return_state))
@@ -524,6 +544,8 @@ def gated_linear_recurrence(input, recurrence_gate, input_gate, decay, initial_s
 def gated_linear_recurrence_step(input, recurrence_gate, input_gate, decay, state, scale=8.0):
     """One row of each of B sequences: input and gates [B, C], ``state`` fp32 [B, C], contiguous,
     updated in place.  Inference only."""
+    if _nodes is not None:
+        return _nodes.recurrence_step_checked(input, recurrence_gate, input_gate, decay, state, float(scale))
     if _wants_grad(input, recurrence_gate, input_gate, decay, state):
         raise RuntimeError("dwconv_b200.gated_linear_recurrence_step: the state is updated in place and "
                            "has no gradient; use gated_linear_recurrence or torch.no_grad()")
@@ -538,6 +560,8 @@ def layer_norm(input, weight=None, bias=None, eps=1e-5):
     channels as ``layer_norm(y.permute(0, 2, 3, 1), ...)`` without a copy.
     """
     eps = float(eps)
+    if _nodes is not None:
+        return _nodes.layer_norm_autograd(input, weight, bias, eps)
     if _wants_grad(input, weight, bias):
         return LayerNormFunction.apply(input, weight, bias, eps)
     return _forms.layer_norm(input, weight, bias, eps, False)[0]
