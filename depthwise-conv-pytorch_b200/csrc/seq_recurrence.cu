@@ -44,9 +44,10 @@ namespace {
 
 __device__ int g_seq_error_flag;  // raised by a wait that ran out
 
-constexpr int REC_L = 8, REC_W = 8, REC_TILE = REC_L * REC_W, REC_GROUP = 64;
-constexpr int REC_THREADS = REC_W * 32;
-constexpr int REC_MAX_CLUSTER = 16;  // 16 needs the non-portable attribute
+constexpr int REC_L = 8;       // rows of a warp
+constexpr int REC_GROUP = 64;  // channels of a warp
+constexpr int REC_CKPT = 32;   // rows between the states that are kept for the backward pass
+constexpr int REC_MAX_CLUSTER = 16;  // more than 8 needs the non-portable attribute
 // Largest z for which the power series are used: what they omit is 5e-8 of exp(-z) - 1 and 2e-9 of p there.
 constexpr float REC_SERIES = 0.125f;
 
@@ -271,6 +272,19 @@ template <bool PACKED> __device__ __forceinline__ float2 apply(float2 P, float2 
   return PACKED && cut(P) ? H : fma2(P, h, H);
 }
 
+// (P, H) of warps from .. to - 1 of a tile, onto what stands in (P, H).
+template <bool PACKED, int W>
+__device__ __forceinline__ void fold(const float4 (&agg)[W][32], int lane, int from, int to, float2 &P, float2 &H) {
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    if (w < from || w >= to) continue;
+    const float4 e = agg[w][lane];
+    const float2 P2 = make_float2(e.x, e.y), H2 = make_float2(e.z, e.w);
+    H = apply<PACKED>(P2, H2, H);
+    P = join<PACKED>(P, P2);
+  }
+}
+
 // ---- thread-block clusters ---------------------------------------------------------------------
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
@@ -296,30 +310,27 @@ struct RecParams {
 };
 
 // Sequences without a row: what enters leaves.
+template <int W>
 __device__ __forceinline__ void empty_states(const RecParams &p, int warp, const float *from, float *to, const Chan &c) {
-  for (int j = warp; j < p.q.S; j += REC_W)
+  for (int j = warp; j < p.q.S; j += W)
     if (seq_bound(p.q, j) >= seq_bound(p.q, j + 1))
       store_state(to, j, p.q.C, c, from ? load_state(from, j, p.q.C, c) : f2(0.f));
 }
 
-// Shared memory of a CTA: the staged rows (FAST), barriers, the warps' pairs (twice, for one barrier per tile),
-// backward the rows' decays, the tiles' pairs of the cluster (twice).
-constexpr int REC_PAIRS = 2 * REC_W * 32 * (int)sizeof(float4);
-template <typename T> constexpr int rec_stage_bytes(int tensors) {
-  return tensors * REC_TILE * REC_GROUP * (int)sizeof(T);
-}
-constexpr int REC_BARRIERS = 128;  // one per warp for its copies, two for the cluster's pairs
-constexpr int REC_DECAYS = REC_TILE * REC_GROUP * (int)sizeof(float);
-inline size_t rec_smem(int stage, bool backward, int cs) {
-  return (size_t)stage + REC_BARRIERS + REC_PAIRS + (backward ? REC_PAIRS / 2 + REC_DECAYS : 0) + (cs > 1 ? 2 * cs * 32 * sizeof(float4) : 0);
+// Shared memory of a CTA of W warps: the rows of NT tensors (FAST), barriers, the pairs of the warps for two
+// tiles, backward the rows' decays, the pairs of the cluster for two tiles.
+template <typename T> constexpr int rec_stage(int W, int NT) { return W * REC_L * REC_GROUP * NT * (int)sizeof(T); }
+constexpr int REC_BARRIERS = 256;  // one per warp for its copies, two for the cluster's pairs
+constexpr int rec_smem(int W, int stage, bool backward, int cs) {
+  return stage + REC_BARRIERS + 2 * W * 32 * (backward ? 24 : 16) + (backward ? W * REC_L * REC_GROUP * 4 : 0) +
+         (cs > 1 ? 2 * cs * 32 * 16 : 0);
 }
 
-// FAST: rows copied ahead by tensor copies; otherwise read where they are used, channels c and c + 32 per lane.
 // Barriers of a CTA; with clusters, a peer's shared memory may be written once the peer has passed here.
-template <bool FAST> __device__ __forceinline__ void start_cta(uint64_t *bars, int cs) {
+template <int W, bool FAST> __device__ __forceinline__ void start_cta(uint64_t *bars, int cs) {
   if (!FAST && cs == 1) return;
   if (threadIdx.x == 0) {
-    for (int n = 0; n < REC_W + 2; ++n) mbar_init(bars + n, 1);
+    for (int n = 0; n < W + 2; ++n) mbar_init(bars + n, 1);
     fence_barrier_init();
   }
   __syncthreads();
@@ -329,14 +340,21 @@ template <bool FAST> __device__ __forceinline__ void start_cta(uint64_t *bars, i
   }
 }
 
-template <typename T, bool FAST, bool PACKED, bool SERIES>
-__device__ __forceinline__ void forward_body(const RecMaps &maps, SeqIn<T> x, SeqIn<T> u, SeqIn<T> v, const float *__restrict__ initial,
-             T *__restrict__ y, float *__restrict__ fin, float *__restrict__ ckpt, const RecParams &p, const Rate &k) {
+// FAST: rows copied ahead by tensor copies; otherwise read where they are used, channels c and c + 32 per lane.
+//
+// Pairs have two places each, for even and odd tiles: a warp writes those of tile n + 2 behind tile n + 1's
+// barrier, which every warp reaches done with tile n; a peer sends those of tile n + 2 once it has this CTA's
+// of tile n + 1, which this CTA sends behind the same barrier.
+template <typename T, int W, bool FAST, bool PACKED, bool SERIES>
+__device__ __forceinline__ void forward_body(const RecMaps &maps, SeqIn<T> x, SeqIn<T> u, SeqIn<T> v,
+                                             const float *__restrict__ initial, T *__restrict__ y,
+                                             float *__restrict__ fin, float *__restrict__ ckpt, const RecParams &p,
+                                             const Rate &k) {
   using Q = Pair<T, FAST>;
-  constexpr int L = REC_L, W = REC_W, NT = 3;
+  constexpr int L = REC_L, NT = 3, TILE = W * L;
   extern __shared__ __align__(128) unsigned char smem[];
   T *stage = reinterpret_cast<T *>(smem);
-  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (FAST ? rec_stage_bytes<T>(NT) : 0)), *met = bars + W;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (FAST ? rec_stage<T>(W, NT) : 0)), *met = bars + W;
   float4(*agg)[W][32] = reinterpret_cast<float4(*)[W][32]>(reinterpret_cast<unsigned char *>(bars) + REC_BARRIERS);
   float4 *far = reinterpret_cast<float4 *>(agg + 2);  // [2][cs][32]
   const int lane = threadIdx.x & 31, warp = uniform_warp();
@@ -345,30 +363,31 @@ __device__ __forceinline__ void forward_body(const RecMaps &maps, SeqIn<T> x, Se
   const int grp = (int)(pair % p.groups), b = (int)(pair / p.groups);
   const int C = p.q.C;
   const Chan c = Q::channels(grp, lane, C);
-  const int tiles = ceil_div(p.q.T, REC_TILE), steps = ceil_div(tiles, p.cs);
+  const int tiles = ceil_div(p.q.T, TILE), steps = ceil_div(tiles, p.cs);
   T *mine = stage + warp * (NT * L * REC_GROUP);
   const int col = c.c0 - grp * REC_GROUP;  // of this lane in the staged rows
   auto start_copies = [&](int tile) {
     if (lane == 0) {
-      const int t = tile * REC_TILE + warp * L;
+      const int t = tile * TILE + warp * L;
       mbar_arrive_expect_tx(bars + warp, NT * L * REC_GROUP * (uint32_t)sizeof(T));
 #pragma unroll
       for (int n = 0; n < NT; ++n) rows_load(mine + n * L * REC_GROUP, &maps.m[n], grp * REC_GROUP, t, b, bars + warp);
     }
   };
-  start_cta<FAST>(bars, p.cs);
+  start_cta<W, FAST>(bars, p.cs);
   if (FAST && steps > 0) start_copies(rank);
-  if (PACKED && fin != nullptr && rank == 0) empty_states(p, warp, initial, fin, c);
+  if (PACKED && fin != nullptr && rank == 0) empty_states<W>(p, warp, initial, fin, c);
   RowWalk walk;
   float2 carry = f2(0.f);
   if (!PACKED && initial != nullptr) carry = load_state(initial, b, C, c);
+
+  RowMasks next_m{0u, 0u, 0u};
+  if (PACKED && steps > 0) next_m = walk.masks<L>(p.q, rank * TILE + warp * L);
   for (int it = 0; it < steps; ++it) {
-    const int tile = it * p.cs + rank, t0 = tile * REC_TILE + warp * L, half = it & 1, phase = it >> 1 & 1;
-    const int rows = p.q.T - t0;
+    const int tile = it * p.cs + rank, t0 = tile * TILE + warp * L, rows = p.q.T - t0, half = it & 1;
     if (p.cs > 1 && threadIdx.x == 0) mbar_arrive_expect_tx(met + half, p.cs * 512);
-    RowMasks m{0u, 0u, 0u};
-    if (PACKED) m = walk.masks<L>(p.q, t0);
-    float2 a[L], bb[L], P = f2(1.f), H = f2(0.f);
+    float2 a[L], bb[L];
+    const RowMasks m = next_m;
     {
       typename Q::Raw rx[L], ru[L], rv[L];
       if constexpr (FAST) {
@@ -401,6 +420,7 @@ __device__ __forceinline__ void forward_body(const RecMaps &maps, SeqIn<T> x, Se
       __syncwarp();
       if (it + 1 < steps) start_copies(tile + p.cs);
     }
+    float2 P = f2(1.f), H = f2(0.f);
     if (!PACKED || (m.start | m.none) == 0u) {
 #pragma unroll
       for (int j = 0; j < L; ++j) {
@@ -426,43 +446,45 @@ __device__ __forceinline__ void forward_body(const RecMaps &maps, SeqIn<T> x, Se
       }
     }
     agg[half][warp][lane] = make_float4(P.x, P.y, H.x, H.y);
-    __syncthreads();
+    bool cuts = false;  // whether a sequence begins in this CTA's tile
+    if (PACKED) cuts = __syncthreads_or((int)(m.start | m.none));
+    else __syncthreads();
+    if (p.cs > 1 && warp < p.cs) {
+      // the CTA's pair, folded by each of the warps that pass it on
+      float2 TP = f2(1.f), TH = f2(0.f);
+      if (cuts) fold<PACKED, W>(agg[half], lane, 0, W, TP, TH);
+      else fold<false, W>(agg[half], lane, 0, W, TP, TH);
+      float4 *there = far + (half * p.cs + rank) * 32 + lane;
+      for (int peer = warp; peer < p.cs; peer += W) store_peer(there, met + half, peer, make_float4(TP.x, TP.y, TH.x, TH.y));
+    }
     float2 h = carry;
     if (p.cs > 1) {
-      // the CTA's pair, folded by each of the warps that pass it on
-      float4 *there = far + (half * p.cs + rank) * 32 + lane;
-      if (warp < p.cs) {
-        float2 TP = f2(1.f), TH = f2(0.f);
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-          const float4 e = agg[half][w][lane];
-          const float2 P2 = make_float2(e.x, e.y), H2 = make_float2(e.z, e.w);
-          TH = apply<PACKED>(P2, H2, TH);
-          TP = join<PACKED>(TP, P2);
-        }
-        for (int peer = warp; peer < p.cs; peer += W) store_peer(there, met + half, peer, make_float4(TP.x, TP.y, TH.x, TH.y));
-      }
-      wait_or_flag(met + half, phase);
+      // this CTA's rows in front of the warp's, while the peers' pairs are on their way
+      float2 FP = f2(1.f), FH = f2(0.f);
+      if (cuts) fold<PACKED, W>(agg[half], lane, 0, warp, FP, FH);
+      else fold<false, W>(agg[half], lane, 0, warp, FP, FH);
+      if (PACKED && it + 1 < steps) next_m = walk.masks<L>(p.q, t0 + p.cs * TILE);
+      wait_or_flag(met + half, it >> 1 & 1);
       for (int w = 0; w < p.cs; ++w) {
         if (w == rank) h = carry;
         const float4 e = far[(half * p.cs + w) * 32 + lane];
         carry = apply<PACKED>(make_float2(e.x, e.y), make_float2(e.z, e.w), carry);
       }
-    }
-    if (ckpt != nullptr && warp == 0 && tile < tiles)
-      store_state(ckpt, (long long)b * tiles + tile, C, c, h);
-    float2 in = h;
+      h = apply<PACKED>(FP, FH, h);
+    } else {
+      float2 in = h;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      if (w == warp) {
-        in = h;
-        if (p.cs > 1) break;
+      for (int w = 0; w < W; ++w) {
+        if (w == warp) in = h;
+        const float4 e = agg[half][w][lane];
+        h = apply<PACKED>(make_float2(e.x, e.y), make_float2(e.z, e.w), h);
       }
-      const float4 e = agg[half][w][lane];
-      h = apply<PACKED>(make_float2(e.x, e.y), make_float2(e.z, e.w), h);
+      carry = h;
+      h = in;
+      if (PACKED && it + 1 < steps) next_m = walk.masks<L>(p.q, t0 + TILE);
     }
-    if (p.cs == 1) carry = h;
-    h = in;
+    if (ckpt != nullptr && warp * L % REC_CKPT == 0 && rows > 0)
+      store_state(ckpt, (long long)b * ceil_div(p.q.T, REC_CKPT) + t0 / REC_CKPT, C, c, h);
     T *py = y + ((long long)b * p.q.T + t0) * C;
     if (rows >= L && (!PACKED || (m.start | m.none | m.end) == 0u)) {
 #pragma unroll
@@ -483,16 +505,18 @@ __device__ __forceinline__ void forward_body(const RecMaps &maps, SeqIn<T> x, Se
   if (!PACKED && fin != nullptr && rank == 0 && warp == 0) store_state(fin, b, C, c, carry);
 }
 
+constexpr int REC_BW = REC_CKPT / REC_L;  // warps of a backward CTA: its tile starts from a kept state
+
 template <typename T, bool FAST, bool PACKED, bool SERIES>
 __device__ __forceinline__ void backward_body(const RecMaps &maps, SeqIn<T> x, SeqIn<T> u, SeqIn<T> v, const float *__restrict__ initial,
               const float *__restrict__ ckpt, SeqIn<T> dy, const float *__restrict__ dfin, T *__restrict__ dx,
               T *__restrict__ du, T *__restrict__ dv, float *__restrict__ dinit, float *__restrict__ part,
               const RecParams &p, const Rate &k) {
   using Q = Pair<T, FAST>;
-  constexpr int L = REC_L, W = REC_W, NT = 4;
+  constexpr int L = REC_L, W = REC_BW, NT = 4, TILE = W * L;
   extern __shared__ __align__(128) unsigned char smem[];
   T *stage = reinterpret_cast<T *>(smem);
-  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (FAST ? rec_stage_bytes<T>(NT) : 0)), *met = bars + W;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (FAST ? rec_stage<T>(W, NT) : 0)), *met = bars + W;
   // P, H of each warp's rows, and what leaves them towards earlier rows
   float4(*agg)[W][32] = reinterpret_cast<float4(*)[W][32]>(reinterpret_cast<unsigned char *>(bars) + REC_BARRIERS);
   float2(*aggq)[W][32] = reinterpret_cast<float2(*)[W][32]>(agg + 2);
@@ -504,30 +528,31 @@ __device__ __forceinline__ void backward_body(const RecMaps &maps, SeqIn<T> x, S
   const int grp = (int)(pair % p.groups), b = (int)(pair / p.groups);
   const int C = p.q.C;
   const Chan c = Q::channels(grp, lane, C);
-  const int tiles = ceil_div(p.q.T, REC_TILE), steps = ceil_div(tiles, p.cs);
+  const int tiles = ceil_div(p.q.T, TILE), steps = ceil_div(tiles, p.cs);
   T *mine = stage + warp * (NT * L * REC_GROUP);
   const int col = c.c0 - grp * REC_GROUP;  // of this lane in the staged rows
   auto start_copies = [&](int tile) {
     if (lane == 0) {
-      const int t = tile * REC_TILE + warp * L;
+      const int t = tile * TILE + warp * L;
       mbar_arrive_expect_tx(bars + warp, NT * L * REC_GROUP * (uint32_t)sizeof(T));
 #pragma unroll
       for (int n = 0; n < NT; ++n) rows_load(mine + n * L * REC_GROUP, &maps.m[n], grp * REC_GROUP, t, b, bars + warp);
     }
   };
-  start_cta<FAST>(bars, p.cs);
+  start_cta<W, FAST>(bars, p.cs);
   if (FAST && steps > 0) start_copies((steps - 1) * p.cs + rank);
-  if (PACKED && dinit != nullptr && rank == 0) empty_states(p, warp, dfin, dinit, c);
+  if (PACKED && dinit != nullptr && rank == 0) empty_states<W>(p, warp, dfin, dinit, c);
   RowWalk walk;
   float2 carry = f2(0.f), ddecay = f2(0.f);
   if (!PACKED && dfin != nullptr) carry = load_state(dfin, b, C, c);
+  RowMasks next_m{0u, 0u, 0u};
+  if (PACKED && steps > 0) next_m = walk.masks<L>(p.q, ((steps - 1) * p.cs + rank) * TILE + warp * L);
   for (int it = steps - 1; it >= 0; --it) {
     const int n = steps - 1 - it, half = n & 1, phase = n >> 1 & 1;
-    const int tile = it * p.cs + rank, t0 = tile * REC_TILE + warp * L;
+    const int tile = it * p.cs + rank, t0 = tile * TILE + warp * L;
     const int rows = p.q.T - t0;
     if (p.cs > 1 && threadIdx.x == 0) mbar_arrive_expect_tx(met + half, p.cs * 512);
-    RowMasks mk{0u, 0u, 0u};
-    if (PACKED) mk = walk.masks<L>(p.q, t0);
+    const RowMasks mk = next_m;
     const unsigned special = mk.start | mk.none;
     float2 h = f2(0.f);
     if (tile < tiles) h = load_state(ckpt, (long long)b * tiles + tile, C, c);
@@ -603,6 +628,7 @@ __device__ __forceinline__ void backward_body(const RecMaps &maps, SeqIn<T> x, S
     agg[half][warp][lane] = make_float4(P.x, P.y, H.x, H.y);
     aggq[half][warp][lane] = G;
     __syncthreads();
+    if (PACKED && it > 0) next_m = walk.masks<L>(p.q, t0 - p.cs * TILE);
     float2 q = carry;
     if (p.cs > 1) {
       float4 *there = far + (half * p.cs + rank) * 32 + lane;
@@ -700,21 +726,26 @@ template <typename T, bool FAST> __device__ __forceinline__ Rate cta_rate(const 
   return rate_of(decay, p.scale, Pair<T, FAST>::channels(grp, threadIdx.x & 31, p.q.C));
 }
 
-template <typename T, bool FAST, bool PACKED>
-__global__ void __launch_bounds__(REC_THREADS, 3)
-recurrence_forward_kernel(const __grid_constant__ RecMaps maps, SeqIn<T> x, SeqIn<T> u, SeqIn<T> v, const float *__restrict__ decay,
-                          const float *__restrict__ initial, T *__restrict__ y, float *__restrict__ fin,
-                          float *__restrict__ ckpt, RecParams p) {
+// CTAs per SM that the registers are cut for.  (Eight warps with two CTAs per SM and 128 registers took 160 us
+// instead of 133 on 32768 fp32 rows of 1152 channels: clusters of 16 then leave SMs of a GPC unused.)
+constexpr int rec_forward_ctas(int W) { return W == 4 ? 8 : 3; }
+constexpr int REC_BACKWARD_CTAS = 4;
+
+template <typename T, int W, bool FAST, bool PACKED>
+__global__ void __launch_bounds__(W * 32, rec_forward_ctas(W))
+recurrence_forward_kernel(const __grid_constant__ RecMaps maps, SeqIn<T> x, SeqIn<T> u, SeqIn<T> v,
+                          const float *__restrict__ decay, const float *__restrict__ initial, T *__restrict__ y,
+                          float *__restrict__ fin, float *__restrict__ ckpt, RecParams p) {
   const Rate k = cta_rate<T, FAST>(decay, p);
   // the same in every warp of the CTA: they have its channels in common
   if (__all_sync(0xffffffffu, k.ks.x >= -REC_SERIES && k.ks.y >= -REC_SERIES))
-    forward_body<T, FAST, PACKED, true>(maps, x, u, v, initial, y, fin, ckpt, p, k);
+    forward_body<T, W, FAST, PACKED, true>(maps, x, u, v, initial, y, fin, ckpt, p, k);
   else
-    forward_body<T, FAST, PACKED, false>(maps, x, u, v, initial, y, fin, ckpt, p, k);
+    forward_body<T, W, FAST, PACKED, false>(maps, x, u, v, initial, y, fin, ckpt, p, k);
 }
 
 template <typename T, bool FAST, bool PACKED>
-__global__ void __launch_bounds__(REC_THREADS, 2)
+__global__ void __launch_bounds__(REC_BW * 32, REC_BACKWARD_CTAS)
 recurrence_backward_kernel(const __grid_constant__ RecMaps maps, SeqIn<T> x, SeqIn<T> u, SeqIn<T> v, const float *__restrict__ decay,
                            const float *__restrict__ initial, const float *__restrict__ ckpt, SeqIn<T> dy,
                            const float *__restrict__ dfin, T *__restrict__ dx, T *__restrict__ du, T *__restrict__ dv,
@@ -755,12 +786,19 @@ recurrence_step_kernel(const T *__restrict__ x, long long xs, const T *__restric
 // CTAs of a cluster along T (a power of two, never more than there are tiles): the choice whose rounds of
 // resident CTAs, each a start-up worth about two tiles and its tiles, take least; a cluster's exchange
 // counts as a quarter of a tile and what it folds.
-inline int rec_cluster(const dwconv_b200_sequence &s, bool backward) {
-  const long long pairs = (long long)ceil_div(s.C, REC_GROUP) * s.B, slots = 148 * (backward ? 2 : 3);
-  const int tiles = ceil_div(s.T, REC_TILE);
+struct RecShape {
+  int W, stage, ctas;
+  bool backward;
+  int smem(int cs) const { return rec_smem(W, stage, backward, cs); }
+};
+inline int rec_cluster(const dwconv_b200_sequence &s, const RecShape &r) {
+  const long long pairs = (long long)ceil_div(s.C, REC_GROUP) * s.B;
+  const int tiles = ceil_div(s.T, r.W * REC_L);
   int best = 1;
   long long cost = 0;
   for (int cs = 1; cs <= REC_MAX_CLUSTER && (cs == 1 || cs <= tiles); cs <<= 1) {
+    const int fit = 227 * 1024 / (r.smem(cs) + 1024);
+    const long long slots = 148ll * (fit < r.ctas ? fit : r.ctas);
     const long long c = ceil_div_ll(pairs * cs, slots) * (2 * 64 + (long long)ceil_div(tiles, cs) * (cs > 1 ? 80 + cs : 64));
     if (cs == 1 || c < cost) {
       best = cs;
@@ -770,12 +808,12 @@ inline int rec_cluster(const dwconv_b200_sequence &s, bool backward) {
   return best;
 }
 
-inline RecParams rec_params(const dwconv_b200_sequence &s, float scale, bool backward) {
+inline RecParams rec_params(const dwconv_b200_sequence &s, float scale, int cs) {
   RecParams p;
   p.q = seq_list(s);
   p.B = s.B;
   p.groups = ceil_div(s.C, REC_GROUP);
-  p.cs = rec_cluster(s, backward);
+  p.cs = cs;
   p.scale = scale;
   return p;
 }
@@ -783,21 +821,21 @@ inline RecParams rec_params(const dwconv_b200_sequence &s, float scale, bool bac
 // Launches `kernel` in clusters of p.cs CTAs.  The attributes that this takes are set once per kernel and
 // device.
 template <typename... K, typename... A>
-void rec_launch(void (*kernel)(K...), std::atomic<unsigned long long> &ready, const RecParams &p, size_t most_smem,
-                size_t smem, cudaStream_t st, A... args) {
+void rec_launch(void (*kernel)(K...), std::atomic<unsigned long long> &ready, const RecParams &p, const RecShape &r,
+                cudaStream_t st, A... args) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return;
   const unsigned long long bit = 1ull << (dev & 63);
   if (!(ready.load(std::memory_order_acquire) & bit)) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most_smem) != cudaSuccess ||
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, r.smem(REC_MAX_CLUSTER)) != cudaSuccess ||
         cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
       return;  // the caller finds the error
     ready.fetch_or(bit, std::memory_order_release);
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)((long long)p.groups * p.B * p.cs));
-  cfg.blockDim = dim3(REC_THREADS);
-  cfg.dynamicSmemBytes = smem;
+  cfg.blockDim = dim3(r.W * 32);
+  cfg.dynamicSmemBytes = r.smem(p.cs);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -838,39 +876,50 @@ template <typename T> bool rec_maps(const RecArgs &a, RecMaps &maps) {
          rows_map<T>(&maps.m[2], *a.v, *a.s) && (a.dy == nullptr || rows_map<T>(&maps.m[3], *a.dy, *a.s));
 }
 
-template <typename T, bool FAST, bool PACKED> void launch_forward(const RecArgs &a, const RecMaps &maps, cudaStream_t st) {
+template <typename T, int W, bool FAST, bool PACKED>
+void launch_forward(const RecArgs &a, const RecMaps &maps, cudaStream_t st) {
   static std::atomic<unsigned long long> ready{0};
-  const RecParams p = rec_params(*a.s, a.scale, false);
-  const int stage = FAST ? rec_stage_bytes<T>(3) : 0;
-  rec_launch(recurrence_forward_kernel<T, FAST, PACKED>, ready, p, rec_smem(stage, false, REC_MAX_CLUSTER),
-             rec_smem(stage, false, p.cs), st, maps, seq_in<T>(*a.x), seq_in<T>(*a.u), seq_in<T>(*a.v), a.decay, a.initial,
-             static_cast<T *>(a.y), a.fin, a.ckpt, p);
+  const RecShape r{W, FAST ? rec_stage<T>(W, 3) : 0, rec_forward_ctas(W), false};
+  const RecParams p = rec_params(*a.s, a.scale, rec_cluster(*a.s, r));
+  rec_launch(recurrence_forward_kernel<T, W, FAST, PACKED>, ready, p, r, st, maps, seq_in<T>(*a.x),
+             seq_in<T>(*a.u), seq_in<T>(*a.v), a.decay, a.initial, static_cast<T *>(a.y), a.fin, a.ckpt, p);
 }
-template <typename T, bool FAST, bool PACKED> void launch_backward(const RecArgs &a, const RecMaps &maps, cudaStream_t st) {
+template <typename T, bool FAST, bool PACKED>
+int launch_backward(const RecArgs &a, const RecMaps &maps, cudaStream_t st) {
   static std::atomic<unsigned long long> ready{0};
-  const RecParams p = rec_params(*a.s, a.scale, true);
-  const int stage = FAST ? rec_stage_bytes<T>(4) : 0;
-  rec_launch(recurrence_backward_kernel<T, FAST, PACKED>, ready, p, rec_smem(stage, true, REC_MAX_CLUSTER),
-             rec_smem(stage, true, p.cs), st, maps, seq_in<T>(*a.x), seq_in<T>(*a.u), seq_in<T>(*a.v), a.decay, a.initial,
-             a.ckpt_in, seq_in<T>(*a.dy), a.dfin, static_cast<T *>(a.dx), static_cast<T *>(a.du),
-             static_cast<T *>(a.dv), a.dinit, a.part, p);
+  const RecShape r{REC_BW, FAST ? rec_stage<T>(REC_BW, 4) : 0, REC_BACKWARD_CTAS, true};
+  const RecParams p = rec_params(*a.s, a.scale, rec_cluster(*a.s, r));
+  rec_launch(recurrence_backward_kernel<T, FAST, PACKED>, ready, p, r, st, maps, seq_in<T>(*a.x), seq_in<T>(*a.u),
+             seq_in<T>(*a.v), a.decay, a.initial, a.ckpt_in, seq_in<T>(*a.dy), a.dfin, static_cast<T *>(a.dx),
+             static_cast<T *>(a.du), static_cast<T *>(a.dv), a.dinit, a.part, p);
+  return p.cs;
 }
 
+// Whether the largest clusters of CTAs of four warps could fill the device.  If so they are used, with the
+// cheapest barriers (8 x 8192 rows of 4096 channels in bf16: 445 us, with eight warps 492); otherwise eight
+// warps, whose clusters take twice the rows between two exchanges (one sequence of 32768 fp32 rows of 1152
+// channels: 133 us, with four warps 148).
+inline bool rec_fills(const dwconv_b200_sequence &s) {
+  return (long long)ceil_div(s.C, REC_GROUP) * s.B * REC_MAX_CLUSTER >= 148 * rec_forward_ctas(4);
+}
+
+template <typename T, bool FAST, bool PACKED> void forward_v(const RecArgs &a, const RecMaps &maps, cudaStream_t st) {
+  if (rec_fills(*a.s)) launch_forward<T, 4, FAST, PACKED>(a, maps, st);
+  else launch_forward<T, 8, FAST, PACKED>(a, maps, st);
+}
 template <typename T> void forward_t(const RecArgs &a, cudaStream_t st) {
   const bool packed = a.s->offsets != nullptr;
   RecMaps maps{};
-  if (rec_maps<T>(a, maps))
-    packed ? launch_forward<T, true, true>(a, maps, st) : launch_forward<T, true, false>(a, maps, st);
-  else
-    packed ? launch_forward<T, false, true>(a, maps, st) : launch_forward<T, false, false>(a, maps, st);
+  if (rec_maps<T>(a, maps)) packed ? forward_v<T, true, true>(a, maps, st) : forward_v<T, true, false>(a, maps, st);
+  else packed ? forward_v<T, false, true>(a, maps, st) : forward_v<T, false, false>(a, maps, st);
 }
-template <typename T> void backward_t(const RecArgs &a, cudaStream_t st) {
+// Returns the CTAs of a cluster: each left a part of the decay's gradient.
+template <typename T> int backward_t(const RecArgs &a, cudaStream_t st) {
   const bool packed = a.s->offsets != nullptr;
   RecMaps maps{};
   if (rec_maps<T>(a, maps))
-    packed ? launch_backward<T, true, true>(a, maps, st) : launch_backward<T, true, false>(a, maps, st);
-  else
-    packed ? launch_backward<T, false, true>(a, maps, st) : launch_backward<T, false, false>(a, maps, st);
+    return packed ? launch_backward<T, true, true>(a, maps, st) : launch_backward<T, true, false>(a, maps, st);
+  return packed ? launch_backward<T, false, true>(a, maps, st) : launch_backward<T, false, false>(a, maps, st);
 }
 
 template <typename T>
@@ -919,13 +968,13 @@ extern "C" {
 
 size_t dwconv_b200_recurrence_checkpoint_bytes(const dwconv_b200_sequence *seq) {
   if (check_recurrence(DWCONV_B200_F32, seq) != DWCONV_B200_OK) return 0;
-  const size_t n = (size_t)seq->B * ceil_div(seq->T, REC_TILE) * seq->C * sizeof(float);
+  const size_t n = (size_t)seq->B * ceil_div(seq->T, REC_CKPT) * seq->C * sizeof(float);
   return (n + 15) / 16 * 16 + 16;
 }
 
 size_t dwconv_b200_recurrence_workspace_bytes(const dwconv_b200_sequence *seq) {
   if (check_recurrence(DWCONV_B200_F32, seq) != DWCONV_B200_OK) return 0;
-  const size_t n = (size_t)seq->B * rec_cluster(*seq, true) * seq->C * sizeof(float);
+  const size_t n = (size_t)seq->B * REC_MAX_CLUSTER * seq->C * sizeof(float);
   return (n + 15) / 16 * 16 + 16;
 }
 
@@ -976,14 +1025,15 @@ int dwconv_b200_recurrence_backward(const dwconv_b200_rows *x, const dwconv_b200
   a.ckpt_in = checkpoints; a.dx = dx; a.du = du; a.dv = dv; a.dinit = dinitial;
   a.part = static_cast<float *>(workspace); a.s = seq; a.scale = scale;
   cudaStream_t st = (cudaStream_t)stream;
+  int cs = 1;
   switch (dtype) {
-    case DWCONV_B200_F32: backward_t<float>(a, st); break;
-    case DWCONV_B200_F16: backward_t<__half>(a, st); break;
-    default: backward_t<__nv_bfloat16>(a, st); break;
+    case DWCONV_B200_F32: cs = backward_t<float>(a, st); break;
+    case DWCONV_B200_F16: cs = backward_t<__half>(a, st); break;
+    default: cs = backward_t<__nv_bfloat16>(a, st); break;
   }
   e = api_launch_status();
   if (e) return e;
-  launch_column_sum(a.part, (long long)seq->B * rec_cluster(*seq, true), seq->C,
+  launch_column_sum(a.part, (long long)seq->B * cs, seq->C,
                     ColumnSumOut{ddecay, nullptr, DWCONV_B200_F32, seq->C, 1, decay}, st);
   return api_launch_status();
 }
@@ -1001,7 +1051,12 @@ int dwconv_b200_recurrence_step(const void *x, long long x_stride, const void *u
   if (!aligned_to(x, es) || !aligned_to(u, es) || !aligned_to(v, es) || !aligned_to(decay, 4) ||
       !aligned_to(state, 4) || !aligned_to(y, es))
     return DWCONV_B200_MISALIGNED;
-  const RecParams p = rec_params(s, scale, false);
+  RecParams p{};
+  p.q = seq_list(s);
+  p.B = B;
+  p.groups = ceil_div(C, REC_GROUP);
+  p.cs = 1;
+  p.scale = scale;
   cudaStream_t st = (cudaStream_t)stream;
   switch (dtype) {
     case DWCONV_B200_F32: step_t<float>(x, x_stride, u, u_stride, v, v_stride, decay, state, y, p, st); break;
