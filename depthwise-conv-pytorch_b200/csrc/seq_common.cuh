@@ -206,7 +206,7 @@ struct ColumnSumOut {
   const float *decay;   // non-null: the sum of column c times sigmoid(decay[c]) / softplus(decay[c])
 };
 
-constexpr int COLSUM_LANES = 32, COLSUM_WARPS = 8;
+constexpr int COLSUM_LANES = 32, COLSUM_WARPS = 32;
 
 __device__ __forceinline__ void store_as(void *p, long long i, float v, int dtype) {
   if (dtype == DWCONV_B200_F32) static_cast<float *>(p)[i] = v;
@@ -214,7 +214,7 @@ __device__ __forceinline__ void store_as(void *p, long long i, float v, int dtyp
   else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
 }
 
-// Every column is added in the same order on every run: warp w takes parts w, w + 8, ...
+// Every column is added in the same order on every run: warp w takes parts w, w + 32, ..., four at a time.
 static __global__ void __launch_bounds__(COLSUM_LANES *COLSUM_WARPS)
 column_sum_kernel(const float *__restrict__ part, long long parts, int M, ColumnSumOut out) {
   __shared__ float s[COLSUM_WARPS][COLSUM_LANES];
@@ -222,13 +222,31 @@ column_sum_kernel(const float *__restrict__ part, long long parts, int M, Column
   const int m = blockIdx.x * COLSUM_LANES + lane;
   float acc = 0.f;
   if (m < M)
-    for (long long p = w; p < parts; p += COLSUM_WARPS) acc += part[p * M + m];
+    for (long long p = w; p < parts; p += 4 * COLSUM_WARPS) {
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const long long q = p + i * COLSUM_WARPS;
+        v[i] = q < parts ? part[q * M + m] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc += v[i];
+    }
   s[w][lane] = acc;
+  __syncthreads();
+  // eight warps add four of the sums each, one warp theirs
+  if (w < 8) {
+    acc = s[w][lane];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) acc += s[w + 8 * i][lane];
+  }
+  __syncthreads();
+  if (w < 8) s[w][lane] = acc;
   __syncthreads();
   if (w != 0 || m >= M) return;
   float v = 0.f;
 #pragma unroll
-  for (int i = 0; i < COLSUM_WARPS; ++i) v += s[i][lane];
+  for (int i = 0; i < 8; ++i) v += s[i][lane];
   const int split = out.C * out.K;
   if (out.decay != nullptr && m < split) {
     const float d = out.decay[m];

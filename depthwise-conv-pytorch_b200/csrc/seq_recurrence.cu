@@ -193,21 +193,12 @@ __device__ __forceinline__ void rows_load(void *to, const CUtensorMap *map, int 
       "l"(map), "r"(c), "r"(t), "r"(b), "r"(smem_u32(bar))
       : "memory");
 }
-// Bounded wait for what this CTA's and its peers' copies and stores signal.  A wait that runs out raises
-// the flag that dwconv_b200_device_status reports; the kernel goes on to its end.
+// Bounded wait for what this CTA's copies and its peers' stores signal.  A wait that runs out raises the
+// flag that dwconv_b200_device_status reports; the kernel goes on to its end.  (The wait acquires at CTA
+// scope: what it waits for lies in this CTA's shared memory, counted by the barrier as it arrives.  At
+// cluster scope every poll would throw the L1 cache away as well.)
 __device__ __forceinline__ void wait_or_flag(uint64_t *bar, uint32_t parity) {
-  for (unsigned n = 0; n < ROWS_WAIT_LIMIT; ++n) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(ROWS_WAIT_HINT_NS)
-        : "memory");
-    if (ok) return;
-  }
-  if ((threadIdx.x & 31) == 0) atomicExch(&g_seq_error_flag, 8);
+  if (!mbar_wait_bounded(bar, parity) && (threadIdx.x & 31) == 0) atomicExch(&g_seq_error_flag, 8);
 }
 
 // Rows at T and behind: a gate of -infinity is closed, the state passes through it.  Every lane
@@ -221,37 +212,46 @@ template <typename T> __device__ __forceinline__ void close_rows(T *gate, int ro
 // ---- rows of a warp ----------------------------------------------------------------------------
 
 // Which of a warp's L rows begin a sequence, end one, or belong to none (bit j: row t0 + j).
+// start_seq, end_seq: the sequence of the last row of each kind.
 struct RowMasks {
   unsigned start, end, none;
+  int start_seq, end_seq;
 };
 
-// For packed sequences.
+// For packed sequences: spans one after the other, starting from the one that the warp's last tile ended in.
 struct RowWalk {
   SeqSpan sp{-1, 0, 0};
   template <int L> __device__ __forceinline__ RowMasks masks(const SeqList &q, int t0) {
-    RowMasks m{0u, 0u, 0u};
-    if (sp.seq >= 0 && t0 >= sp.begin && t0 + L <= sp.next) {
-      if (t0 == sp.begin) m.start = 1u;
-      if (sp.next == t0 + L) m.end = 1u << (L - 1);
-      return m;
-    }
-    for (int j = 0; j < L; ++j) {
-      const int t = t0 + j;
-      if (t >= q.T) {
-        m.none |= 1u << j;
-        continue;
-      }
-      if (j == 0 || t == sp.next) sp = seq_locate(q, t);
+    RowMasks m{0u, 0u, 0u, -1, -1};
+    int t = t0;
+    const int end = min(t0 + L, q.T);
+    while (t < end) {
+      if (!(t >= sp.begin && t < sp.next)) sp = seq_locate(q, t);
+      const int to = min(sp.next, end);
       if (sp.seq < 0) {
-        m.none |= 1u << j;
+        m.none |= (1u << (to - t0)) - (1u << (t - t0));
       } else {
-        if (t == sp.begin) m.start |= 1u << j;
-        if (t + 1 == sp.next) m.end |= 1u << j;
+        if (t == sp.begin) {
+          m.start |= 1u << (t - t0);
+          m.start_seq = sp.seq;
+        }
+        if (to == sp.next) {
+          m.end |= 1u << (to - 1 - t0);
+          m.end_seq = sp.seq;
+        }
       }
+      t = to;
     }
+    t = max(t, t0);
+    if (t < t0 + L) m.none |= (1u << L) - (1u << (t - t0));  // at T and behind
     return m;
   }
 };
+
+// The sequence of row t0 + j, one of those in `mask`, of which `last` is the sequence of the last one.
+__device__ __forceinline__ int seq_of(const SeqList &q, int t0, int j, unsigned mask, int last) {
+  return mask >> j == 1u ? last : seq_locate(q, t0 + j).seq;
+}
 
 __device__ __forceinline__ float2 load_state(const float *s, long long j, int C, const Chan &c) {
   return make_float2(s[j * C + c.c0], s[j * C + c.c1]);
@@ -318,12 +318,21 @@ __device__ __forceinline__ void empty_states(const RecParams &p, int warp, const
 }
 
 // Shared memory of a CTA of W warps: the rows of NT tensors (FAST), barriers, the pairs of the warps for two
-// tiles, backward the rows' decays, the pairs of the cluster for two tiles.
+// tiles, what enters the CTA's tile (two), backward the rows' decays, the pairs of the cluster for two tiles, PACKED the first offsets.
 template <typename T> constexpr int rec_stage(int W, int NT) { return W * REC_L * REC_GROUP * NT * (int)sizeof(T); }
 constexpr int REC_BARRIERS = 256;  // one per warp for its copies, two for the cluster's pairs
-constexpr int rec_smem(int W, int stage, bool backward, int cs) {
-  return stage + REC_BARRIERS + 2 * W * 32 * (backward ? 24 : 16) + (backward ? W * REC_L * REC_GROUP * 4 : 0) +
+constexpr int REC_OFFSETS = 1024;  // as many offsets of packed sequences are kept in shared memory
+constexpr int rec_smem(int W, int stage, bool backward, bool packed, int cs) {
+  return stage + (packed ? REC_OFFSETS * 4 : 0) + (backward ? 0 : 2 * 32 * 8) + REC_BARRIERS + 2 * W * 32 * (backward ? 24 : 16) + (backward ? W * REC_L * REC_GROUP * 4 : 0) +
          (cs > 1 ? 2 * cs * 32 * 16 : 0);
+}
+
+// The list's offsets in shared memory, where they fit.
+__device__ __forceinline__ void keep_offsets(SeqList &q, int *kept) {
+  if (q.S + 1 > REC_OFFSETS) return;
+  for (int j = threadIdx.x; j <= q.S; j += blockDim.x) kept[j] = q.offsets[j];
+  __syncthreads();
+  q.offsets = kept;
 }
 
 // Barriers of a CTA; with clusters, a peer's shared memory may be written once the peer has passed here.
@@ -356,7 +365,8 @@ __device__ __forceinline__ void forward_body(const RecMaps &maps, SeqIn<T> x, Se
   T *stage = reinterpret_cast<T *>(smem);
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (FAST ? rec_stage<T>(W, NT) : 0)), *met = bars + W;
   float4(*agg)[W][32] = reinterpret_cast<float4(*)[W][32]>(reinterpret_cast<unsigned char *>(bars) + REC_BARRIERS);
-  float4 *far = reinterpret_cast<float4 *>(agg + 2);  // [2][cs][32]
+  float2(*entry)[32] = reinterpret_cast<float2(*)[32]>(agg + 2);  // [2]: the state that enters the CTA's tile
+  float4 *far = reinterpret_cast<float4 *>(entry + 2);            // [2][cs][32]
   const int lane = threadIdx.x & 31, warp = uniform_warp();
   const int rank = (int)(blockIdx.x % p.cs);
   const long long pair = blockIdx.x / p.cs;
@@ -374,6 +384,11 @@ __device__ __forceinline__ void forward_body(const RecMaps &maps, SeqIn<T> x, Se
       for (int n = 0; n < NT; ++n) rows_load(mine + n * L * REC_GROUP, &maps.m[n], grp * REC_GROUP, t, b, bars + warp);
     }
   };
+  SeqList q = p.q;
+  if (PACKED) {
+    int *kept = reinterpret_cast<int *>(far + (p.cs > 1 ? 2 * p.cs * 32 : 0));
+    keep_offsets(q, kept);
+  }
   start_cta<W, FAST>(bars, p.cs);
   if (FAST && steps > 0) start_copies(rank);
   if (PACKED && fin != nullptr && rank == 0) empty_states<W>(p, warp, initial, fin, c);
@@ -381,13 +396,19 @@ __device__ __forceinline__ void forward_body(const RecMaps &maps, SeqIn<T> x, Se
   float2 carry = f2(0.f);
   if (!PACKED && initial != nullptr) carry = load_state(initial, b, C, c);
 
-  RowMasks next_m{0u, 0u, 0u};
-  if (PACKED && steps > 0) next_m = walk.masks<L>(p.q, rank * TILE + warp * L);
+  RowMasks next_m{0u, 0u, 0u, -1, -1};
+  float2 next_entry = f2(0.f);  // the state that the last sequence to begin in the warp's rows begins with
+  auto look = [&](int t) {
+    next_m = walk.masks<L>(q, t);
+    if (next_m.start != 0u && initial != nullptr) next_entry = load_state(initial, next_m.start_seq, C, c);
+  };
+  if (PACKED && steps > 0) look(rank * TILE + warp * L);
   for (int it = 0; it < steps; ++it) {
     const int tile = it * p.cs + rank, t0 = tile * TILE + warp * L, rows = p.q.T - t0, half = it & 1;
     if (p.cs > 1 && threadIdx.x == 0) mbar_arrive_expect_tx(met + half, p.cs * 512);
     float2 a[L], bb[L];
     const RowMasks m = next_m;
+    const float2 first = next_entry;
     {
       typename Q::Raw rx[L], ru[L], rv[L];
       if constexpr (FAST) {
@@ -436,7 +457,7 @@ __device__ __forceinline__ void forward_body(const RecMaps &maps, SeqIn<T> x, Se
           H = f2(0.f);
         } else if (m.start >> j & 1u) {
           if (initial != nullptr)
-            bb[j] = fma2(a[j], load_state(initial, seq_locate(p.q, t0 + j).seq, C, c), bb[j]);
+            bb[j] = fma2(a[j], (m.start >> j == 1u ? first : load_state(initial, seq_locate(q, t0 + j).seq, C, c)), bb[j]);
           P = f2(-1.f);
           H = bb[j];
         } else {
@@ -463,14 +484,17 @@ __device__ __forceinline__ void forward_body(const RecMaps &maps, SeqIn<T> x, Se
       float2 FP = f2(1.f), FH = f2(0.f);
       if (cuts) fold<PACKED, W>(agg[half], lane, 0, warp, FP, FH);
       else fold<false, W>(agg[half], lane, 0, warp, FP, FH);
-      if (PACKED && it + 1 < steps) next_m = walk.masks<L>(p.q, t0 + p.cs * TILE);
-      wait_or_flag(met + half, it >> 1 & 1);
-      for (int w = 0; w < p.cs; ++w) {
-        if (w == rank) h = carry;
-        const float4 e = far[(half * p.cs + w) * 32 + lane];
-        carry = apply<PACKED>(make_float2(e.x, e.y), make_float2(e.z, e.w), carry);
+      if (PACKED && it + 1 < steps) look(t0 + p.cs * TILE);
+      if (warp == 0) {  // one warp waits for the peers' pairs and folds them for all
+        wait_or_flag(met + half, it >> 1 & 1);
+        for (int w = 0; w < p.cs; ++w) {
+          if (w == rank) entry[half][lane] = carry;
+          const float4 e = far[(half * p.cs + w) * 32 + lane];
+          carry = apply<PACKED>(make_float2(e.x, e.y), make_float2(e.z, e.w), carry);
+        }
       }
-      h = apply<PACKED>(FP, FH, h);
+      __syncthreads();
+      h = apply<PACKED>(FP, FH, entry[half][lane]);
     } else {
       float2 in = h;
 #pragma unroll
@@ -481,7 +505,7 @@ __device__ __forceinline__ void forward_body(const RecMaps &maps, SeqIn<T> x, Se
       }
       carry = h;
       h = in;
-      if (PACKED && it + 1 < steps) next_m = walk.masks<L>(p.q, t0 + TILE);
+      if (PACKED && it + 1 < steps) look(t0 + TILE);
     }
     if (ckpt != nullptr && warp * L % REC_CKPT == 0 && rows > 0)
       store_state(ckpt, (long long)b * ceil_div(p.q.T, REC_CKPT) + t0 / REC_CKPT, C, c, h);
@@ -498,7 +522,7 @@ __device__ __forceinline__ void forward_body(const RecMaps &maps, SeqIn<T> x, Se
         h = PACKED && ((m.start | m.none) >> j & 1u) ? bb[j] : fma2(a[j], h, bb[j]);
         if (j < rows) Q::store(py + (long long)j * C, c, h);
         if (PACKED && (m.end >> j & 1u) && fin != nullptr)
-          store_state(fin, seq_locate(p.q, t0 + j).seq, C, c, h);
+          store_state(fin, seq_of(q, t0, j, m.end, m.end_seq), C, c, h);
       }
     }
   }
@@ -539,14 +563,19 @@ __device__ __forceinline__ void backward_body(const RecMaps &maps, SeqIn<T> x, S
       for (int n = 0; n < NT; ++n) rows_load(mine + n * L * REC_GROUP, &maps.m[n], grp * REC_GROUP, t, b, bars + warp);
     }
   };
+  SeqList list = p.q;
+  if (PACKED) {
+    int *kept = reinterpret_cast<int *>(far + (p.cs > 1 ? 2 * p.cs * 32 : 0));
+    keep_offsets(list, kept);
+  }
   start_cta<W, FAST>(bars, p.cs);
   if (FAST && steps > 0) start_copies((steps - 1) * p.cs + rank);
   if (PACKED && dinit != nullptr && rank == 0) empty_states<W>(p, warp, dfin, dinit, c);
   RowWalk walk;
   float2 carry = f2(0.f), ddecay = f2(0.f);
   if (!PACKED && dfin != nullptr) carry = load_state(dfin, b, C, c);
-  RowMasks next_m{0u, 0u, 0u};
-  if (PACKED && steps > 0) next_m = walk.masks<L>(p.q, ((steps - 1) * p.cs + rank) * TILE + warp * L);
+  RowMasks next_m{0u, 0u, 0u, -1, -1};
+  if (PACKED && steps > 0) next_m = walk.masks<L>(list, ((steps - 1) * p.cs + rank) * TILE + warp * L);
   for (int it = steps - 1; it >= 0; --it) {
     const int n = steps - 1 - it, half = n & 1, phase = n >> 1 & 1;
     const int tile = it * p.cs + rank, t0 = tile * TILE + warp * L;
@@ -598,7 +627,7 @@ __device__ __forceinline__ void backward_body(const RecMaps &maps, SeqIn<T> x, S
 #pragma unroll
       for (int j = 0; j < L; ++j)
         if (mk.end >> j & 1u)
-          g[j] = add2(g[j], load_state(dfin, seq_locate(p.q, t0 + j).seq, C, c));
+          g[j] = add2(g[j], load_state(dfin, seq_of(list, t0, j, mk.end, mk.end_seq), C, c));
     }
     // what the rows do to a state going down (P, H), and what they pass to a gradient going up
     // (G = sum_j a[0] .. a[j] g[j], up to the first row that begins a sequence)
@@ -611,7 +640,7 @@ __device__ __forceinline__ void backward_body(const RecMaps &maps, SeqIn<T> x, S
       if (PACKED && (special >> j & 1u)) {
         if (mk.none >> j & 1u) bb = f2(0.f);
         else if (initial != nullptr)
-          bb = fma2(a, load_state(initial, seq_locate(p.q, t0 + j).seq, C, c), bb);
+          bb = fma2(a, load_state(initial, seq_of(list, t0, j, mk.start, mk.start_seq), C, c), bb);
         P = f2(-1.f);
         H = bb;
       } else {
@@ -628,7 +657,7 @@ __device__ __forceinline__ void backward_body(const RecMaps &maps, SeqIn<T> x, S
     agg[half][warp][lane] = make_float4(P.x, P.y, H.x, H.y);
     aggq[half][warp][lane] = G;
     __syncthreads();
-    if (PACKED && it > 0) next_m = walk.masks<L>(p.q, t0 - p.cs * TILE);
+    if (PACKED && it > 0) next_m = walk.masks<L>(list, t0 - p.cs * TILE);
     float2 q = carry;
     if (p.cs > 1) {
       float4 *there = far + (half * p.cs + rank) * 32 + lane;
@@ -672,7 +701,7 @@ __device__ __forceinline__ void backward_body(const RecMaps &maps, SeqIn<T> x, S
       q = mul2(keep[j][lane], g[j]);
       if (PACKED && (special >> j & 1u)) {
         if ((mk.start >> j & 1u) && dinit != nullptr)
-          store_state(dinit, seq_locate(p.q, t0 + j).seq, C, c, q);
+          store_state(dinit, seq_of(list, t0, j, mk.start, mk.start_seq), C, c, q);
         q = f2(0.f);
       }
     }
@@ -687,7 +716,7 @@ __device__ __forceinline__ void backward_body(const RecMaps &maps, SeqIn<T> x, S
       if (PACKED && (special >> j & 1u)) {
         h = f2(0.f);
         if ((mk.start >> j & 1u) && initial != nullptr)
-          h = load_state(initial, seq_locate(p.q, t0 + j).seq, C, c);
+          h = load_state(initial, seq_of(list, t0, j, mk.start, mk.start_seq), C, c);
         if (mk.none >> j & 1u) g[j] = f2(0.f);
       }
       const float2 ddx = mul2(g[j], mul2(beta, i[j]));
@@ -788,8 +817,8 @@ recurrence_step_kernel(const T *__restrict__ x, long long xs, const T *__restric
 // counts as a quarter of a tile and what it folds.
 struct RecShape {
   int W, stage, ctas;
-  bool backward;
-  int smem(int cs) const { return rec_smem(W, stage, backward, cs); }
+  bool backward, packed;
+  int smem(int cs) const { return rec_smem(W, stage, backward, packed, cs); }
 };
 inline int rec_cluster(const dwconv_b200_sequence &s, const RecShape &r) {
   const long long pairs = (long long)ceil_div(s.C, REC_GROUP) * s.B;
@@ -879,7 +908,7 @@ template <typename T> bool rec_maps(const RecArgs &a, RecMaps &maps) {
 template <typename T, int W, bool FAST, bool PACKED>
 void launch_forward(const RecArgs &a, const RecMaps &maps, cudaStream_t st) {
   static std::atomic<unsigned long long> ready{0};
-  const RecShape r{W, FAST ? rec_stage<T>(W, 3) : 0, rec_forward_ctas(W), false};
+  const RecShape r{W, FAST ? rec_stage<T>(W, 3) : 0, rec_forward_ctas(W), false, PACKED};
   const RecParams p = rec_params(*a.s, a.scale, rec_cluster(*a.s, r));
   rec_launch(recurrence_forward_kernel<T, W, FAST, PACKED>, ready, p, r, st, maps, seq_in<T>(*a.x),
              seq_in<T>(*a.u), seq_in<T>(*a.v), a.decay, a.initial, static_cast<T *>(a.y), a.fin, a.ckpt, p);
@@ -887,7 +916,7 @@ void launch_forward(const RecArgs &a, const RecMaps &maps, cudaStream_t st) {
 template <typename T, bool FAST, bool PACKED>
 int launch_backward(const RecArgs &a, const RecMaps &maps, cudaStream_t st) {
   static std::atomic<unsigned long long> ready{0};
-  const RecShape r{REC_BW, FAST ? rec_stage<T>(REC_BW, 4) : 0, REC_BACKWARD_CTAS, true};
+  const RecShape r{REC_BW, FAST ? rec_stage<T>(REC_BW, 4) : 0, REC_BACKWARD_CTAS, true, PACKED};
   const RecParams p = rec_params(*a.s, a.scale, rec_cluster(*a.s, r));
   rec_launch(recurrence_backward_kernel<T, FAST, PACKED>, ready, p, r, st, maps, seq_in<T>(*a.x), seq_in<T>(*a.u),
              seq_in<T>(*a.v), a.decay, a.initial, a.ckpt_in, seq_in<T>(*a.dy), a.dfin, static_cast<T *>(a.dx),
