@@ -34,6 +34,7 @@
 // The forward pass keeps the fp32 state that enters each tile (1 / (W L) of the rows); the backward
 // pass starts from it, so it reads y nowhere and its h[t-1] have not been rounded to the data's type.
 #include <atomic>
+#include <cmath>
 
 #include "rows_engine.cuh"
 #include "seq_common.cuh"
@@ -812,27 +813,40 @@ recurrence_step_kernel(const T *__restrict__ x, long long xs, const T *__restric
 
 // ---- host --------------------------------------------------------------------------------------
 
-// CTAs of a cluster along T (a power of two, never more than there are tiles): the choice whose rounds of
-// resident CTAs, each a start-up worth about two tiles and its tiles, take least; a cluster's exchange
-// counts as a quarter of a tile and what it folds.
+// A kernel's CTA, and what is known about its time: a tile takes `tile` microseconds of an SM's throughput, and
+// `chain` where the SM has nothing else to do (its loads, gates, folds and exchanges follow one another).
 struct RecShape {
   int W, stage, ctas;
   bool backward, packed;
+  float tile, chain;
   int smem(int cs) const { return rec_smem(W, stage, backward, packed, cs); }
 };
-inline int rec_cluster(const dwconv_b200_sequence &s, const RecShape &r) {
+
+// CTAs of a cluster along T, and the time that goes with it in microseconds, by a model: n CTAs of an SM take
+// (tile n) and (chain) per tile, the larger nearly alone; CTAs beyond those that fit follow them; a start
+// is worth two tiles.  Measured against all sizes: one packed list of 8191 rows of 2560 channels in bf16,
+// forward, clusters of 4 / 6 / 8 / 10 / 12 / 16: 114 / 87 / 83 / 73 / 99 / 91 us (it takes 10); 8 x 8192 rows of
+// 4096, backward, 1 / 2 / 4 / 8: 980 / 900 / 947 / 982 us (it takes 2).  Odd sizes and 14 leave SMs of a
+// GPC without work and are not in the choice.
+struct RecChoice {
+  int cs;
+  float us;
+};
+inline RecChoice rec_cluster(const dwconv_b200_sequence &s, const RecShape &r) {
+  static const int sizes[] = {1, 2, 4, 6, 8, 10, 12, 16};
+  const int sms = 148, tiles = ceil_div(s.T, r.W * REC_L);
   const long long pairs = (long long)ceil_div(s.C, REC_GROUP) * s.B;
-  const int tiles = ceil_div(s.T, r.W * REC_L);
-  int best = 1;
-  long long cost = 0;
-  for (int cs = 1; cs <= REC_MAX_CLUSTER && (cs == 1 || cs <= tiles); cs <<= 1) {
-    const int fit = 227 * 1024 / (r.smem(cs) + 1024);
-    const long long slots = 148ll * (fit < r.ctas ? fit : r.ctas);
-    const long long c = ceil_div_ll(pairs * cs, slots) * (2 * 64 + (long long)ceil_div(tiles, cs) * (cs > 1 ? 80 + cs : 64));
-    if (cs == 1 || c < cost) {
-      best = cs;
-      cost = c;
-    }
+  RecChoice best{1, 0.f};
+  for (int cs : sizes) {
+    if (cs > 1 && cs > tiles) break;
+    const int fit = 227 * 1024 / (r.smem(cs) + 1024), slots = fit < r.ctas ? fit : r.ctas;
+    auto time = [&](float n) {
+      const float a = r.tile * n, b = r.chain;
+      return sqrtf(sqrtf(a * a * a * a + b * b * b * b));
+    };
+    const float n = (float)(pairs * cs) / sms, full = floorf(n / slots), rest = ceilf(n - full * slots);
+    const float us = (ceil_div(tiles, cs) + 2) * (full * time((float)slots) + (rest > 0.f ? time(rest) : 0.f));
+    if (cs == 1 || us < best.us) best = RecChoice{cs, us};
   }
   return best;
 }
@@ -905,36 +919,36 @@ template <typename T> bool rec_maps(const RecArgs &a, RecMaps &maps) {
          rows_map<T>(&maps.m[2], *a.v, *a.s) && (a.dy == nullptr || rows_map<T>(&maps.m[3], *a.dy, *a.s));
 }
 
+template <typename T, int W, bool FAST, bool PACKED> RecShape forward_shape() {
+  return RecShape{W, FAST ? rec_stage<T>(W, 3) : 0, rec_forward_ctas(W), false, PACKED, W * 0.125f, W == 4 ? 2.3f : 2.6f};
+}
 template <typename T, int W, bool FAST, bool PACKED>
-void launch_forward(const RecArgs &a, const RecMaps &maps, cudaStream_t st) {
+void launch_forward(const RecArgs &a, const RecMaps &maps, int cs, cudaStream_t st) {
   static std::atomic<unsigned long long> ready{0};
-  const RecShape r{W, FAST ? rec_stage<T>(W, 3) : 0, rec_forward_ctas(W), false, PACKED};
-  const RecParams p = rec_params(*a.s, a.scale, rec_cluster(*a.s, r));
-  rec_launch(recurrence_forward_kernel<T, W, FAST, PACKED>, ready, p, r, st, maps, seq_in<T>(*a.x),
-             seq_in<T>(*a.u), seq_in<T>(*a.v), a.decay, a.initial, static_cast<T *>(a.y), a.fin, a.ckpt, p);
+  const RecParams p = rec_params(*a.s, a.scale, cs);
+  rec_launch(recurrence_forward_kernel<T, W, FAST, PACKED>, ready, p, forward_shape<T, W, FAST, PACKED>(), st, maps,
+             seq_in<T>(*a.x), seq_in<T>(*a.u), seq_in<T>(*a.v), a.decay, a.initial, static_cast<T *>(a.y), a.fin, a.ckpt,
+             p);
 }
 template <typename T, bool FAST, bool PACKED>
 int launch_backward(const RecArgs &a, const RecMaps &maps, cudaStream_t st) {
   static std::atomic<unsigned long long> ready{0};
-  const RecShape r{REC_BW, FAST ? rec_stage<T>(REC_BW, 4) : 0, REC_BACKWARD_CTAS, true, PACKED};
-  const RecParams p = rec_params(*a.s, a.scale, rec_cluster(*a.s, r));
+  const RecShape r{REC_BW, FAST ? rec_stage<T>(REC_BW, 4) : 0, REC_BACKWARD_CTAS, true, PACKED, 1.f, 2.4f};
+  const RecParams p = rec_params(*a.s, a.scale, rec_cluster(*a.s, r).cs);
   rec_launch(recurrence_backward_kernel<T, FAST, PACKED>, ready, p, r, st, maps, seq_in<T>(*a.x), seq_in<T>(*a.u),
              seq_in<T>(*a.v), a.decay, a.initial, a.ckpt_in, seq_in<T>(*a.dy), a.dfin, static_cast<T *>(a.dx),
              static_cast<T *>(a.du), static_cast<T *>(a.dv), a.dinit, a.part, p);
   return p.cs;
 }
 
-// Whether the largest clusters of CTAs of four warps could fill the device.  If so they are used, with the
-// cheapest barriers (8 x 8192 rows of 4096 channels in bf16: 445 us, with eight warps 492); otherwise eight
-// warps, whose clusters take twice the rows between two exchanges (one sequence of 32768 fp32 rows of 1152
-// channels: 133 us, with four warps 148).
-inline bool rec_fills(const dwconv_b200_sequence &s) {
-  return (long long)ceil_div(s.C, REC_GROUP) * s.B * REC_MAX_CLUSTER >= 148 * rec_forward_ctas(4);
-}
-
+// CTAs of four warps have the cheapest barriers and pack best; those of eight take twice the rows between two
+// exchanges, which counts where there are few of them.  8 x 8192 rows of 4096 channels in bf16: 437 us with
+// four, 441 with eight; one sequence of 32768 fp32 rows of 1152: 155 and 124.
 template <typename T, bool FAST, bool PACKED> void forward_v(const RecArgs &a, const RecMaps &maps, cudaStream_t st) {
-  if (rec_fills(*a.s)) launch_forward<T, 4, FAST, PACKED>(a, maps, st);
-  else launch_forward<T, 8, FAST, PACKED>(a, maps, st);
+  const RecChoice four = rec_cluster(*a.s, forward_shape<T, 4, FAST, PACKED>());
+  const RecChoice eight = rec_cluster(*a.s, forward_shape<T, 8, FAST, PACKED>());
+  if (four.us <= eight.us) launch_forward<T, 4, FAST, PACKED>(a, maps, four.cs, st);
+  else launch_forward<T, 8, FAST, PACKED>(a, maps, eight.cs, st);
 }
 template <typename T> void forward_t(const RecArgs &a, cudaStream_t st) {
   const bool packed = a.s->offsets != nullptr;
