@@ -7,10 +7,14 @@
 // Bound by memory (forward: x in, y out; backward: x and dy in, dx out).  A warp owns 64 or 128
 // channels and a run of R rows; the rows stream through a register window, so each is read once, but for the
 // K-1 rows in front of a run (backward: behind it too), which come from L1 / L2.  The sums are in fp32.
+// Rows are copied to shared memory some chunks of rows ahead (cp.async), every lane the bytes that it will
+// read itself: no barrier, no registers for what is on its way.
 //
 // Packed sequences: a warp's row number is the same in all lanes, so a sequence's end is one uniform
 // comparison per row; there the window is filled anew from the next sequence's initial rows.
 #pragma once
+
+#include <atomic>
 
 #include "seq_conv1d_ops.cuh"
 
@@ -54,6 +58,64 @@ __device__ __forceinline__ SeqSpan conv_span(const SeqList &q, int b, int t) {
 template <int K> __host__ __device__ constexpr int ring(int at, int k) { return (at + k) % K; }
 // Rows a lane loads together: a multiple of K.
 template <int K> constexpr int conv_unroll(int most) { return K >= most ? K : most / K * K; }
+
+// Chunks of U rows of NT tensors on their way to a lane: STAGES - 1 of them while one is worked on.
+template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t to, const void *from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
+}
+template <typename T, int H, int U, int NT> struct RowPipe {
+  using Raw = typename Lanes<T, H, true>::Raw;
+  static constexpr int CHUNK = U * NT * 32 * (int)sizeof(Raw);  // bytes of a warp's chunk
+  static constexpr int FIT = 64 * 1024 / (CONV_WARPS * CHUNK);
+  static constexpr int STAGES = FIT < 2 ? 2 : (FIT > 4 ? 4 : FIT);
+  static constexpr int BYTES = CONV_WARPS * STAGES * CHUNK;     // of a CTA
+  const unsigned char *mine;
+  __device__ __forceinline__ RowPipe(unsigned char *smem, int warp, int lane)
+      : mine(smem + warp * STAGES * CHUNK + lane * (int)sizeof(Raw)) {}
+  __device__ __forceinline__ const Raw *at(int stage, int j, int n) const {
+    return reinterpret_cast<const Raw *>(mine + stage * CHUNK + (j * NT + n) * 32 * (int)sizeof(Raw));
+  }
+  // row[n]: this lane's place in the chunk's first row of tensor n, rs[n] elements between rows
+  __device__ __forceinline__ void start(int stage, const T *const (&row)[NT], const long long (&rs)[NT]) const {
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        copy_async<(int)sizeof(Raw)>((uint32_t)__cvta_generic_to_shared(at(stage, j, n)), row[n] + j * rs[n]);
+  }
+  static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  // the oldest of the chunks on their way has arrived
+  static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory"); }
+  // `chunks` chunks from the given rows on: body(chunk, stage) once chunk has arrived.
+  template <typename F>
+  __device__ __forceinline__ void run(int chunks, const T *const (&first)[NT], const long long (&rs)[NT], F &&body) const {
+    const T *row[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) row[n] = first[n];
+    auto next = [&](int i, int stage) {
+      if (i < chunks) {
+        start(stage, row, rs);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) row[n] += U * rs[n];
+      }
+      commit();
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) next(i, i);
+    int stage = 0;
+    for (int i = 0; i < chunks; ++i) {
+      wait();
+      body(i, stage);
+      next(i + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
+      stage = stage == STAGES - 1 ? 0 : stage + 1;
+    }
+  }
+};
+template <typename T, int H, bool VEC, int U, int NT> constexpr int pipe_bytes() {
+  if constexpr (VEC) return RowPipe<T, H, U, NT>::BYTES;
+  else return 0;
+}
+template <typename T, int K> constexpr int forward_unroll() { return conv_unroll<K>(4); }
 
 // The K-1 rows in front of row t, oldest first at 0: rows of the sequence, or of its initial state.
 template <typename T, int H, bool VEC, int K>
@@ -144,7 +206,8 @@ __global__ void __launch_bounds__(CONV_WARPS * 32, K <= 4 ? 3 : 2)
 conv1d_forward_kernel(SeqIn<T> x, const T *__restrict__ w, const T *__restrict__ bias, const T *__restrict__ initial,
                       T *__restrict__ y, T *__restrict__ fin, Conv1dParams p) {
   using Ln = Lanes<T, H, VEC>;
-  constexpr int U = conv_unroll<K>(sizeof(T) == 4 ? 4 : 8);
+  constexpr int U = forward_unroll<T, K>();
+  extern __shared__ __align__(16) unsigned char pipe_smem[];
   if (blockIdx.x >= p.main) {
     if constexpr (K > 1) final_rows<T, K>(x, initial, fin, p.q, (int)(blockIdx.x - p.main), (int)(gridDim.x - p.main));
     return;
@@ -170,20 +233,36 @@ conv1d_forward_kernel(SeqIn<T> x, const T *__restrict__ w, const T *__restrict__
     }
     const T *xr = x.row(b, t);
     T *yr = y + ((long long)b * p.q.T + t) * C;
-    if (t + U <= t1 && t + U <= sp.next && sp.seq >= 0) {
-      typename Ln::Raw raw[U];
+    const int chunks = sp.seq >= 0 ? (min(t1, sp.next) - t) / U : 0;
+    if (chunks > 0) {
+      auto rows = [&](const typename Ln::Raw (&raw)[U], T *out) {
 #pragma unroll
-      for (int j = 0; j < U; ++j) raw[j] = ln.load(xr + j * x.rs);
+        for (int j = 0; j < U; ++j) {
+          float2 o[H];
+          ln.get(raw[j], win[ring<K>(j, K - 1)]);
+          taps.apply(win, j, o);
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        float2 o[H];
-        ln.get(raw[j], win[ring<K>(j, K - 1)]);
-        taps.apply(win, j, o);
+          for (int h = 0; h < H; ++h) o[h] = act2<ACT>(o[h], p.act);
+          ln.store(out + (long long)j * C, o);
+        }
+      };
+      if constexpr (VEC) {
+        const RowPipe<T, H, U, 1> pipe(pipe_smem, warp, threadIdx.x & 31);
+        pipe.run(chunks, {xr + ln.channel(0)}, {x.rs}, [&](int i, int stage) {
+          typename Ln::Raw raw[U];
 #pragma unroll
-        for (int h = 0; h < H; ++h) o[h] = act2<ACT>(o[h], p.act);
-        ln.store(yr + (long long)j * C, o);
+          for (int j = 0; j < U; ++j) raw[j] = *pipe.at(stage, j, 0);
+          rows(raw, yr + (long long)i * U * C);
+        });
+      } else {
+        for (int i = 0; i < chunks; ++i) {
+          typename Ln::Raw raw[U];
+#pragma unroll
+          for (int j = 0; j < U; ++j) raw[j] = ln.load(xr + ((long long)i * U + j) * x.rs);
+          rows(raw, yr + (long long)i * U * C);
+        }
       }
-      t += U;
+      t += chunks * U;
     } else {
       float2 o[H];
       ln.get(ln.load(xr), win[K - 1]);
@@ -215,6 +294,7 @@ conv1d_backward_kernel(SeqIn<T> x, const T *__restrict__ w, const T *__restrict_
     return;
   }
   __shared__ float2 sum[(K + 1) * H][32];
+  extern __shared__ __align__(16) unsigned char pipe_smem[];
   const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
   const int cb = (int)(blockIdx.x % p.cblocks);
   const long long rest = blockIdx.x / p.cblocks;
@@ -305,25 +385,39 @@ conv1d_backward_kernel(SeqIn<T> x, const T *__restrict__ w, const T *__restrict_
         clear();
       }
       const int lead = t - (K - 1);
-      if (lead >= t0 && lead >= sp.begin && t + U <= t1 && t + U <= sp.next && sp.seq >= 0) {
-        // U rows inside the run and the sequence
-        typename Ln::Raw rx[U], rg[U];
+      const int chunks = lead >= t0 && lead >= sp.begin && sp.seq >= 0 ? (min(t1, sp.next) - t) / U : 0;
+      if (chunks > 0) {
+        // chunks of U rows inside the run and the sequence
         const T *xr = x.row(b, t), *gr = dy.row(b, t);
         T *dr = dx + ((long long)b * p.q.T + lead) * C;
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-          rx[j] = ln.load(xr + j * x.rs);
-          rg[j] = ln.load(gr + j * dy.rs);
-        }
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
+        auto row = [&](int j, const typename Ln::Raw &rx, const typename Ln::Raw &rg, T *out) {
           float2 o[H];
-          take(j, rx[j], rg[j]);
+          take(j, rx, rg);
           count(j);
           gradient(j, o);
-          ln.store(dr + (long long)j * C, o);
+          ln.store(out, o);
+        };
+        if constexpr (VEC) {
+          const RowPipe<T, H, U, 2> pipe(pipe_smem, warp, lane);
+          pipe.run(chunks, {xr + ln.channel(0), gr + ln.channel(0)}, {x.rs, dy.rs}, [&](int i, int stage) {
+            T *out = dr + (long long)i * U * C;
+#pragma unroll
+            for (int j = 0; j < U; ++j) row(j, *pipe.at(stage, j, 0), *pipe.at(stage, j, 1), out + (long long)j * C);
+          });
+        } else {
+          for (int i = 0; i < chunks; ++i) {
+            typename Ln::Raw rx[U], rg[U];
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+              rx[j] = ln.load(xr + ((long long)i * U + j) * x.rs);
+              rg[j] = ln.load(gr + ((long long)i * U + j) * dy.rs);
+            }
+            T *out = dr + (long long)i * U * C;
+#pragma unroll
+            for (int j = 0; j < U; ++j) row(j, rx[j], rg[j], out + (long long)j * C);
+          }
         }
-        t += U;
+        t += chunks * U;
       } else {
         typename Ln::Raw rx = ln.zero(), rg = ln.zero();
         if (sp.seq >= 0) {
@@ -415,6 +509,21 @@ conv1d_step_kernel(const T *__restrict__ x, long long xs, const T *__restrict__ 
   else { constexpr int ACT = ANY; CALL; }
 
 
+// One kernel with its shared memory; what that takes is set once per kernel and device.
+template <auto KERNEL, int SMEM, typename... A> void launch_rows(long long ctas, cudaStream_t st, A... args) {
+  static std::atomic<unsigned long long> ready{0};
+  if (SMEM > 32 * 1024) {  // with the static part, more than 48 KB
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (!(ready.load(std::memory_order_acquire) & bit)) {
+      if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) return;
+      ready.fetch_or(bit, std::memory_order_release);
+    }
+  }
+  KERNEL<<<(unsigned)ctas, CONV_WARPS * 32, SMEM, st>>>(args...);
+}
+
 template <typename T, int H, bool VEC> void launch_forward(const ConvArgs &a, cudaStream_t st) {
   const Conv1dParams p = conv_params(*a.s, Lanes<T, H, VEC>::GROUP, a.act, false);
   long long extra = 0;
@@ -423,11 +532,10 @@ template <typename T, int H, bool VEC> void launch_forward(const ConvArgs &a, cu
     if (extra > STATE_BLOCKS) extra = STATE_BLOCKS;
   }
   if (p.main + extra == 0) return;
-  auto go = [&](auto kernel) {
-    kernel<<<(unsigned)(p.main + extra), CONV_WARPS * 32, 0, st>>>(
-        seq_in<T>(*a.x), (const T *)a.w, (const T *)a.bias, (const T *)a.initial, (T *)a.y, (T *)a.fin, p);
-  };
-  DWB_TAPS(a.taps, DWB_ACT(a.act, go((conv1d_forward_kernel<T, H, VEC, TAPS, ACT>))))
+  DWB_TAPS(a.taps, DWB_ACT(a.act, (launch_rows<conv1d_forward_kernel<T, H, VEC, TAPS, ACT>,
+                                               pipe_bytes<T, H, VEC, forward_unroll<T, TAPS>(), 1>()>(
+                                      p.main + extra, st, seq_in<T>(*a.x), (const T *)a.w, (const T *)a.bias,
+                                      (const T *)a.initial, (T *)a.y, (T *)a.fin, p))))
 }
 
 // Register windows of x, dp, w and dw: four channels per lane for up to four taps, two above.
@@ -438,12 +546,11 @@ template <typename T, int H, bool VEC> long long launch_backward(const ConvArgs 
   if (a.dinit != nullptr && a.taps > 1 && (a.s->offsets != nullptr || a.s->T == 0))
     extra = p.q.S < STATE_BLOCKS ? p.q.S : STATE_BLOCKS;
   if (p.main + extra == 0) return 0;
-  auto go = [&](auto kernel) {
-    kernel<<<(unsigned)(p.main + extra), CONV_WARPS * 32, 0, st>>>(
-        seq_in<T>(*a.x), (const T *)a.w, (const T *)a.bias, (const T *)a.initial, seq_in<T>(*a.dy), (const T *)a.dfin,
-        (T *)a.dx, (T *)a.dinit, a.part, p);
-  };
-  DWB_TAPS(a.taps, DWB_ACT(a.act, go((conv1d_backward_kernel<T, (TAPS > 4 ? 1 : H), VEC, TAPS, ACT>))))
+  DWB_TAPS(a.taps, DWB_ACT(a.act, (launch_rows<conv1d_backward_kernel<T, (TAPS > 4 ? 1 : H), VEC, TAPS, ACT>,
+                                               pipe_bytes<T, (TAPS > 4 ? 1 : H), VEC, conv_unroll<TAPS>(4), 2>()>(
+                                      p.main + extra, st, seq_in<T>(*a.x), (const T *)a.w, (const T *)a.bias,
+                                      (const T *)a.initial, seq_in<T>(*a.dy), (const T *)a.dfin, (T *)a.dx,
+                                      (T *)a.dinit, a.part, p))))
   return (long long)p.rblocks * a.s->B;
 }
 
