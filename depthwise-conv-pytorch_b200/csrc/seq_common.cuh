@@ -221,6 +221,7 @@ column_sum_kernel(const float *__restrict__ part, long long parts, int M, Column
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int m = blockIdx.x * COLSUM_LANES + lane;
   float acc = 0.f;
+  pdl_wait();  // the kernel that left the parts has finished
   if (m < M)
     for (long long p = w; p < parts; p += 4 * COLSUM_WARPS) {
       float v[4];
@@ -261,9 +262,18 @@ column_sum_kernel(const float *__restrict__ part, long long parts, int M, Column
   }
 }
 
-inline void launch_column_sum(const float *part, long long parts, int M, const ColumnSumOut &out,
-                              cudaStream_t st) {
-  column_sum_kernel<<<ceil_div(M, COLSUM_LANES), COLSUM_LANES * COLSUM_WARPS, 0, st>>>(part, parts, M, out);
+// Launched so that its start-up runs under the end of the kernel that leaves the parts.
+inline void launch_column_sum(const float *part, long long parts, int M, const ColumnSumOut &out, cudaStream_t st) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)ceil_div(M, COLSUM_LANES));
+  cfg.blockDim = dim3(COLSUM_LANES * COLSUM_WARPS);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  (void)cudaLaunchKernelEx(&cfg, column_sum_kernel, part, parts, M, out);
 }
 
 // ---- host checks -------------------------------------------------------------------------------

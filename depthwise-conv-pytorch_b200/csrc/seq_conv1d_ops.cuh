@@ -26,18 +26,19 @@ struct ConvArgs {
   int taps, act;
 };
 
-// Rows of a run: the choice whose rounds of resident warps (24 per SM forward, 16 backward), each a run and
+// Rows of a run: the choice whose rounds of resident CTAs (three per SM forward, two backward), each a run and
 // what it costs beside its rows, take least.  That cost is worth 5 rows forward (the filter, the K-1 rows
 // in front) and 12 backward (those on both sides, the sums at the end).  Measured on 4 x 4096 rows of 2560
-// channels in bf16, four taps, with runs of 16 / 32 / 48 / 64 / 128 rows: forward 46 / 44 / 44 / 47 / 49 us,
-// backward 134 / 107 / 99 / 105 / 118 us; the rule takes 48 for both.
+// channels in bf16, four taps, before rows were copied ahead, with runs of 16 / 32 / 48 / 64 / 128 rows:
+// forward 46 / 44 / 44 / 47 / 49 us, backward 134 / 107 / 99 / 105 / 118 us; the rule takes 48 for both.
 inline int conv_run(const dwconv_b200_sequence &s, int group, bool backward) {
   static const int runs[] = {8, 16, 24, 32, 48, 64, 96, 128};
-  const long long slots = 148 * (backward ? 16 : 24), per_row = (long long)s.B * ceil_div(s.C, group);
+  const long long slots = 148 * (backward ? 2 : 3), per_block = (long long)s.B * ceil_div(s.C, group);
   int best = runs[0];
   long long cost = 0;
   for (int R : runs) {
-    const long long c = ceil_div_ll(per_row * ceil_div(s.T, R), slots) * (R + (backward ? 12 : 5));
+    const long long ctas = per_block * ceil_div(ceil_div(s.T, R), CONV_WARPS);
+    const long long c = ceil_div_ll(ctas, slots) * (R + (backward ? 12 : 5));
     if (R == runs[0] || c < cost) {
       best = R;
       cost = c;

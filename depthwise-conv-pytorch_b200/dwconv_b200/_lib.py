@@ -184,7 +184,8 @@ def status_string(code):
 def device_status():
     """Synchronises the current device and returns (and clears) the flags its kernels raised
     when one of their bounded waits ran out: 0 = none, bit 0 forward / backward-input, bit 1
-    backward-filter, bit 2 the exchange between GPUs, -1 = the device reported an error."""
+    backward-filter, bit 2 the exchange between GPUs, bit 3 the sequence operators, -1 = the device
+    reported an error."""
     return int(lib.dwconv_b200_device_status())
 
 
@@ -193,7 +194,7 @@ def check_device_status(what):
     v = device_status()
     if v != 0:
         names = [n for bit, n in ((1, "forward/backward-input"), (2, "backward-filter"),
-                                  (4, "exchange between GPUs")) if v > 0 and v & bit]
+                                  (4, "exchange between GPUs"), (8, "sequence operators")) if v > 0 and v & bit]
         raise RuntimeError(f"dwconv_b200.{what}: a kernel's bounded wait expired "
                            f"(device status {v}: {', '.join(names) or 'CUDA error'}); "
                            "the results of the calls since the last check are incomplete")

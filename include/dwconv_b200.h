@@ -94,7 +94,7 @@ DWCONV_B200_API int dwconv_b200_last_cuda_error(void);
  * whose wait expires raises a flag, finishes without hanging and leaves wrong output.
  * This call synchronises the device, returns the flags raised since the last call (0 = none;
  * bit 0 forward/backward-input kernels, bit 1 backward-filter kernels, bit 2 the exchange between
- * GPUs) and clears them.
+ * GPUs, bit 3 the sequence operators) and clears them.
  * Diagnostic: not needed on the hot path.  No counterpart in the reference. */
 DWCONV_B200_API int dwconv_b200_device_status(void);
 
