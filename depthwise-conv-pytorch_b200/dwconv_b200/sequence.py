@@ -592,9 +592,8 @@ class CausalDepthwiseConv1d(nn.Module):
 
 class GatedLinearRecurrence(nn.Module):
     """Module form of ``gated_linear_recurrence``: holds ``decay``, drawn so that a fully open gate
-    decays by a factor between ``low`` and ``high`` per row.  The parameter stays fp32 under
-    ``.half()`` / ``.bfloat16()`` of an enclosing model only if converted back; the operator refuses
-    another dtype."""
+    decays by a factor between ``low`` and ``high`` per row.  The parameter stays fp32, unrounded, when
+    the module or a model around it is converted (``.half()``, ``.bfloat16()``, ``.to(dtype)``)."""
 
     def __init__(self, channels, scale=8.0, low=0.9, high=0.999):
         super().__init__()
@@ -603,6 +602,13 @@ class GatedLinearRecurrence(nn.Module):
         self.channels, self.scale = channels, float(scale)
         a = low + (high - low) * torch.rand(channels, dtype=torch.float64)
         self.decay = nn.Parameter(torch.log(torch.expm1(-torch.log(a) / scale)).float())
+
+    def _apply(self, fn, recurse=True):
+        kept = self.decay.data
+        out = super()._apply(fn, recurse)
+        if self.decay.dtype != torch.float32:
+            self.decay.data = kept.to(self.decay.device)
+        return out
 
     def forward(self, input, recurrence_gate, input_gate, initial_state=None, offsets=None, return_state=False):
         return gated_linear_recurrence(input, recurrence_gate, input_gate, self.decay, initial_state, offsets,
@@ -646,13 +652,6 @@ class RecurrentMixer(nn.Module):
         self.recurrence = GatedLinearRecurrence(width, scale)
         self.project_out = nn.Linear(width, channels)
 
-    def _apply(self, fn, recurse=True):
-        out = super()._apply(fn, recurse)
-        p = self.recurrence.decay  # the operator takes it in fp32 whatever the model's dtype
-        if p.dtype != torch.float32:
-            p.data = p.data.float()
-        return out
-
     def initial_state(self, count, dtype=None, device=None):
         w = self.conv.weight
         dtype, device = dtype or w.dtype, device or w.device
@@ -667,6 +666,7 @@ class RecurrentMixer(nn.Module):
         h, rec_state = self.recurrence(z, u, v, rec_state, offsets, return_state=True)
         return x + self.project_out(h * nn.functional.gelu(gate)), (conv_state, rec_state)
 
+    @torch.no_grad()
     def step(self, x, state):
         """x [B, C]; ``state`` as from ``forward`` or ``initial_state``, updated in place."""
         gate, z = self.project_in(self.norm(x)).chunk(2, dim=-1)

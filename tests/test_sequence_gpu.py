@@ -700,6 +700,94 @@ def test_mixer_in_bf16_keeps_its_decay_in_fp32():
     assert state[0].dtype == torch.bfloat16 and state[1].dtype == torch.float32
 
 
+# ---- lists and sizes drawn at random ------------------------------------------------------------
+
+@pytest.mark.parametrize("seed", range(24))
+def test_random_problems(seed):
+    """Sizes, types, states and packed lists drawn anew; lists may begin behind row 0 and hold more sequences
+    than the kernels keep on chip."""
+    import random
+    r = random.Random(1000 + seed)
+    dtype = r.choice(DTYPES)
+    C = r.choice([1, 2, 7, 8, 24, 63, 64, 72, 130, 200])
+    state = r.random() < 0.5
+    offsets = on_gpu = None
+    if r.random() < 0.6:
+        B, count = 1, r.choice([1, 3, 20, 1500 if C <= 24 else 40])
+        o = [r.choice([0, 0, 5])]
+        for _ in range(count):
+            o.append(o[-1] + (r.choice([0, 1, 2]) if count > 100 else r.choice([0, 1, 3, 31, 32, 65, r.randint(0, 300)])))
+        offsets, T = o, max(1, o[-1] + r.choice([0, 4]))
+        on_gpu = torch.tensor(o, dtype=torch.int32, device="cuda")
+        n = count
+    else:
+        B, T = r.choice([1, 2, 5]), r.choice([1, 31, 32, 33, 64, 200, 517, 1100])
+        n = B
+    run_recurrence(*recurrence_inputs(B, T, C, n, dtype, seed, state), on_gpu, offsets, scale=r.choice([1.0, 8.0]))
+    K = r.randint(1, 8)
+    run_conv(*conv_inputs(B, T, C, K, n, dtype, seed, state, r.random() < 0.5), r.choice(["silu", None]), on_gpu, offsets)
+    g = torch.Generator().manual_seed(seed)
+    w, b = randn(g, C, dtype=dtype), randn(g, C, dtype=dtype)
+    run_norm(randn(g, B, T, C, dtype=dtype), w, b, randn(g, B, T, C, dtype=dtype, grad=False))
+
+
+def test_rows_that_the_copy_engine_cannot_address():
+    """Odd strides in one operand, an expanded batch in another, an expanded gradient: the same values as
+    for contiguous tensors, forward and backward."""
+    import dwconv_b200 as d
+    g = torch.Generator().manual_seed(51)
+    B, T, C = 2, 150, 72
+    u, v = randn(g, B, T, C, grad=False), randn(g, B, T, C, grad=False)
+    odd = randn(g, B, T, C + 1, grad=False)[..., :C]
+    one = randn(g, 1, T, C, grad=False).expand(B, T, C)
+    decay = (torch.rand(C, generator=g) * 6 - 8).cuda()
+    w = randn(g, C, 1, 4, grad=False)
+    dys = [randn(g, B, T, C, grad=False), torch.ones((), device="cuda").expand(B, T, C), odd]
+    for x in (odd, one):
+        for dy in dys:
+            for f in (lambda t: d.gated_linear_recurrence(t, u, v, decay), lambda t: d.depthwise_conv1d_causal(t, w),
+                      lambda t: d.gated_linear_recurrence(u, t, v, decay)):
+                a, b = x.detach().requires_grad_(), x.contiguous().requires_grad_()
+                ya, yb = f(a), f(b)
+                assert torch.equal(ya, yb)
+                ga, = torch.autograd.grad(ya, a, dy)
+                gb, = torch.autograd.grad(yb, b, dy.contiguous())
+                assert torch.equal(ga, gb)
+
+
+def test_interpreted_nodes_give_the_same_gradients():
+    """The autograd functions that run without the compiled module."""
+    import dwconv_b200 as d
+    from dwconv_b200 import sequence as S
+    x, u, v, decay, w = three_inputs(52, T=70)
+    b, c0 = torch.randn(66, device="cuda", requires_grad=True), torch.randn(2, 3, 66, device="cuda", requires_grad=True)
+    h0 = torch.randn(2, 66, device="cuda", requires_grad=True)
+    pairs = [
+        (d.depthwise_conv1d_causal(x, w, b, "silu", c0, return_state=True),
+         S.CausalConv1dFunction.apply(x, w, b, c0, None, 3, True), [x, w, b, c0]),
+        (d.gated_linear_recurrence(x, u, v, decay, h0, return_state=True),
+         S.GatedLinearRecurrenceFunction.apply(x, u, v, decay, h0, None, 8.0, True), [x, u, v, decay, h0]),
+        ((d.layer_norm(x, b, b),), (S.LayerNormFunction.apply(x, b, b, 1e-5),), [x, b]),
+    ]
+    for native, plain, leaves in pairs:
+        given = [torch.randn_like(t) for t in native]
+        for p, q in zip(native, plain):
+            assert torch.equal(p, q)
+        for p, q in zip(torch.autograd.grad(native, leaves, given, retain_graph=True),
+                        torch.autograd.grad(plain, leaves, given)):
+            assert torch.equal(p, q)
+        # a graph is released behind its first use; asking for the input alone is enough
+        torch.autograd.grad(native, leaves[:1], given)
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(native, leaves[:1], given)
+
+
+def test_no_wait_ran_out():
+    """After all of the above: no kernel gave up waiting for its copies or its cluster."""
+    from dwconv_b200 import _lib
+    assert _lib.device_status() == 0
+
+
 # ---- refusals on the device --------------------------------------------------------------------
 
 def test_refusals():

@@ -112,7 +112,10 @@ def test_module_surfaces():
     r = d.GatedLinearRecurrence(1000)
     a = torch.exp(-8.0 * torch.nn.functional.softplus(r.decay.double()))
     assert r.decay.dtype == torch.float32 and 0.8999 < float(a.min()) and float(a.max()) < 0.99901
-    m = d.RecurrentMixer(6, width=8).to(torch.bfloat16)
+    m = d.RecurrentMixer(6, width=8)
+    before = m.recurrence.decay.detach().clone()
+    m = m.to(torch.bfloat16)
+    assert torch.equal(m.recurrence.decay, before)  # neither converted nor rounded
     assert m.recurrence.decay.dtype == torch.float32 and m.norm.weight.dtype == torch.bfloat16
     assert [tuple(t.shape) for t in m.initial_state(3)] == [(3, 3, 8), (3, 8)]
     assert [t.dtype for t in m.initial_state(3)] == [torch.bfloat16, torch.float32]
