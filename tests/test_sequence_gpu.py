@@ -421,6 +421,27 @@ def test_norm_matches_its_definition(size, dtype):
     run_norm(x, None, None, dy)
 
 
+@by_dtype
+@pytest.mark.parametrize("C", [520, 776, 1000, 2048, 3080, 4096])
+def test_norm_of_many_rows(C, dtype):
+    """CTAs that stay for many rows; widths with and without a tail."""
+    g = torch.Generator().manual_seed(53)
+    x = (torch.randn(4800, C, generator=g) * 2 + 0.5).to(dtype).cuda()
+    w, b = (1 + 0.3 * torch.randn(C, generator=g)).to(dtype).cuda(), randn(g, C, dtype=dtype, grad=False)
+    import dwconv_b200 as d
+    for wt, bt in ((w, b), (None, b), (w, None)):
+        y = d.layer_norm(x, wt, bt)
+        want, tol = ref.norm(x, wt, bt, 1e-5)
+        ref.check(y, want["y"], tol["y"], dtype, "y")
+    # with a graph: the statistics that the backward reads
+    rows = slice(0, 4800, 37)
+    leaf = x.clone().requires_grad_()
+    dy = randn(g, 4800, C, dtype=dtype, grad=False)
+    dx, = torch.autograd.grad(d.layer_norm(leaf, w, b), leaf, dy)
+    want, tol = ref.norm(x[rows], w, b, 1e-5, dy[rows])
+    ref.check(dx[rows], want["dx"], tol["dx"], dtype, "dx")
+
+
 def test_norm_far_from_zero_and_constant_rows():
     g = torch.Generator().manual_seed(19)
     for C in (40, 1000, 20000):
