@@ -15,6 +15,7 @@
 #include <torch/extension.h>
 
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -679,8 +680,37 @@ template <typename... T> bool wants_grad(const T &...t) {
   return at::GradMode::is_enabled() && ((t.defined() && t.requires_grad()) || ...);
 }
 
+// There are no forward-mode derivatives: a tangent that an operand carries would be lost.
+template <typename... T> void refuse_tangents(const char *fn, const T &...t) {
+  TORCH_CHECK(!(torch::autograd::isFwGradDefined(t) || ...), "dwconv_b200.", fn,
+              ": forward-mode differentiation is not supported");
+}
+
 struct OnceNode : torch::autograd::Node {
+  // A leaf's gradient is accumulated on the stream that was current when a live graph first reached the
+  // leaf.  Where that is the legacy default stream, which cannot take part in a capture, the engine would
+  // break the capture in the middle; refused here, before anything is recorded.
+  void check_capture() {
+    const at::DeviceIndex device = this->device().index();
+    const c10::cuda::CUDAStream current = c10::cuda::getCurrentCUDAStream(device);
+    if (current.id() == 0) return;
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(current.stream(), &status) != cudaSuccess || status == cudaStreamCaptureStatusNone)
+      return;
+    for (size_t i = 0; i < num_outputs(); ++i) {
+      const auto &fn = next_edge(i).function;
+      if (fn == nullptr || !task_should_compute_output(i) ||
+          dynamic_cast<torch::autograd::AccumulateGrad *>(fn.get()) == nullptr)
+        continue;
+      const auto stream = fn->stream();
+      TORCH_CHECK(!stream.has_value() || stream->id() != 0, "dwconv_b200: ", name(),
+                  " is being captured into a CUDA graph, but an eager autograd graph of the same leaf is still alive "
+                  "on the default stream; release it before the capture");
+    }
+  }
   variable_list apply(variable_list &&grads) override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    check_capture();
     bool twice = false, any = false;
     for (const at::Tensor &g : grads) {
       any = any || g.defined();
@@ -735,6 +765,7 @@ py::object conv1d_causal_autograd(const at::Tensor &input, const at::Tensor &wei
   const at::Tensor b = or_undefined(bias), h = or_undefined(initial);
   at::Tensor y;
   OptTensor state;
+  refuse_tangents("depthwise_conv1d_causal", input, weight, b, h);
   const bool grad = wants_grad(input, weight, b, h);
   {
     at::AutoGradMode no_grad(false);
@@ -782,6 +813,7 @@ py::object recurrence_autograd(const at::Tensor &input, const at::Tensor &u, con
   const at::Tensor h = or_undefined(initial);
   at::Tensor y;
   OptTensor state, ckpt;
+  refuse_tangents("gated_linear_recurrence", input, u, v, decay, h);
   const bool grad = wants_grad(input, u, v, decay, h);
   {
     at::AutoGradMode no_grad(false);
@@ -826,6 +858,7 @@ at::Tensor layer_norm_autograd(const at::Tensor &input, const OptTensor &weight,
   const at::Tensor w = or_undefined(weight), b = or_undefined(bias);
   at::Tensor y;
   OptTensor stats;
+  refuse_tangents("layer_norm", input, w, b);
   const bool grad = wants_grad(input, w, b);
   {
     at::AutoGradMode no_grad(false);
@@ -847,6 +880,7 @@ at::Tensor conv1d_causal_step_checked(const at::Tensor &input, const at::Tensor 
   TORCH_CHECK(!wants_grad(input, weight, state, or_undefined(bias)),
               "dwconv_b200.depthwise_conv1d_causal_step: the state is updated in place and has no gradient; use "
               "depthwise_conv1d_causal or torch.no_grad()");
+  refuse_tangents("depthwise_conv1d_causal_step", input, weight, state, or_undefined(bias));
   return conv1d_causal_step(input, weight, state, bias, act);
 }
 
@@ -855,6 +889,7 @@ at::Tensor recurrence_step_checked(const at::Tensor &input, const at::Tensor &u,
   TORCH_CHECK(!wants_grad(input, u, v, decay, state),
               "dwconv_b200.gated_linear_recurrence_step: the state is updated in place and has no gradient; use "
               "gated_linear_recurrence or torch.no_grad()");
+  refuse_tangents("gated_linear_recurrence_step", input, u, v, decay, state);
   return recurrence_step(input, u, v, decay, state, scale);
 }
 

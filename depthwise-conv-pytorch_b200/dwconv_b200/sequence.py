@@ -12,7 +12,8 @@ sequence: zeros in every output, and what they hold is not looked at.  The list 
 a list that is not ascending gives unspecified values (never an access out of bounds).
 
 Every function runs on the current stream of the input's device, never synchronises, and may be
-captured into a CUDA graph.  Gradients are first-order only.
+captured into a CUDA graph.  Gradients are first-order and reverse-mode only.  A backward pass is not
+captured while an eager graph of the same leaves is alive on the default stream (refused).
 """
 import torch
 from torch import nn
@@ -408,6 +409,12 @@ def _wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _refuse_tangents(fn, *tensors):
+    # there are no forward-mode derivatives: a tangent that an operand carries would be lost
+    if any(t is not None and torch.autograd.forward_ad.unpack_dual(t, level=0).tangent is not None for t in tensors):
+        raise RuntimeError(f"dwconv_b200.{fn}: forward-mode differentiation is not supported")
+
+
 def _activation(activation):
     if activation not in _ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}; expected one of "
@@ -495,6 +502,7 @@ def depthwise_conv1d_causal(input, weight, bias=None, activation=None, initial_s
     act = _activation(activation)
     if _nodes is not None:
         return _nodes.conv1d_causal_autograd(input, weight, bias, act, initial_state, offsets, bool(return_state))
+    _refuse_tangents("depthwise_conv1d_causal", input, weight, bias, initial_state)
     if _wants_grad(input, weight, bias, initial_state):
         return CausalConv1dFunction.apply(input, weight, bias, initial_state, offsets, act, bool(return_state))
     y, state = _forms.conv1d_causal(input, weight, bias, act, initial_state, offsets, bool(return_state))
@@ -508,6 +516,7 @@ def depthwise_conv1d_causal_step(input, weight, state, bias=None, activation=Non
     act = _activation(activation)
     if _nodes is not None:
         return _nodes.conv1d_causal_step_checked(input, weight, state, bias, act)
+    _refuse_tangents("depthwise_conv1d_causal_step", input, weight, state, bias)
     if _wants_grad(input, weight, state, bias):
         raise RuntimeError("dwconv_b200.depthwise_conv1d_causal_step: the state is updated in place and "
                            "has no gradient; use depthwise_conv1d_causal or torch.no_grad()")
@@ -533,6 +542,7 @@ def gated_linear_recurrence(input, recurrence_gate, input_gate, decay, initial_s
     if _nodes is not None:
         return _nodes.recurrence_autograd(input, recurrence_gate, input_gate, decay, initial_state, offsets, scale,
                                           bool(return_state))
+    _refuse_tangents("gated_linear_recurrence", input, recurrence_gate, input_gate, decay, initial_state)
     if _wants_grad(input, recurrence_gate, input_gate, decay, initial_state):
         return GatedLinearRecurrenceFunction.apply(input, recurrence_gate, input_gate, decay, initial_state,
                                                    offsets, scale, bool(return_state))
@@ -546,6 +556,7 @@ def gated_linear_recurrence_step(input, recurrence_gate, input_gate, decay, stat
     updated in place.  Inference only."""
     if _nodes is not None:
         return _nodes.recurrence_step_checked(input, recurrence_gate, input_gate, decay, state, float(scale))
+    _refuse_tangents("gated_linear_recurrence_step", input, recurrence_gate, input_gate, decay, state)
     if _wants_grad(input, recurrence_gate, input_gate, decay, state):
         raise RuntimeError("dwconv_b200.gated_linear_recurrence_step: the state is updated in place and "
                            "has no gradient; use gated_linear_recurrence or torch.no_grad()")
@@ -562,6 +573,7 @@ def layer_norm(input, weight=None, bias=None, eps=1e-5):
     eps = float(eps)
     if _nodes is not None:
         return _nodes.layer_norm_autograd(input, weight, bias, eps)
+    _refuse_tangents("layer_norm", input, weight, bias)
     if _wants_grad(input, weight, bias):
         return LayerNormFunction.apply(input, weight, bias, eps)
     return _forms.layer_norm(input, weight, bias, eps, False)[0]

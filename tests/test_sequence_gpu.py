@@ -582,6 +582,46 @@ def test_captured_training_step_and_decoding_step():
     assert torch.allclose(torch.stack(rows, 1), whole, rtol=1e-5, atol=1e-5)
 
 
+@pytest.mark.parametrize("op", ["conv", "recurrence", "norm"])
+def test_capture_beside_a_live_eager_graph(op):
+    """An eager graph on the default stream holds the leaves: a captured backward is refused before the
+    engine can break the capture; once it is gone the same capture runs."""
+    import gc
+    import dwconv_b200 as d
+    if not d.sequence._nodes:
+        pytest.skip("the compiled nodes are not in use")
+    x, u, v, decay, w = three_inputs(44)
+
+    def work():
+        if op == "conv":
+            return d.depthwise_conv1d_causal(x, w, None, "silu"), [x, w]
+        if op == "recurrence":
+            return d.gated_linear_recurrence(x, u, v, decay), [x, u, v, decay]
+        return d.layer_norm(x), [x]
+
+    seeds = torch.ones_like(x)
+    want = torch.autograd.grad(*work(), seeds)
+
+    def captured():
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            y, leaves = work()
+            grads = torch.autograd.grad(y, leaves, seeds)
+        gr.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(grads, want):
+            assert torch.equal(a, b)
+
+    alive = work()
+    with pytest.raises(RuntimeError, match="still alive on the default stream"):
+        captured()
+    for a, b in zip(torch.autograd.grad(*alive, seeds), want):   # the eager graph itself goes on
+        assert torch.equal(a, b)
+    del alive
+    gc.collect()   # frames of the refused call hold a graph of the leaves as well
+    captured()
+
+
 def test_offsets_into_tensors_pass_32_bits():
     """Tensors of more than 2^31 elements; the inputs are one row seen many times."""
     import dwconv_b200 as d

@@ -103,6 +103,28 @@ def test_cpu_tensors_and_unknown_activations_are_refused():
         d.GatedLinearRecurrence(8, low=0.0)
 
 
+def test_forward_mode_derivatives_are_refused():
+    """A tangent would be lost without a word: every function refuses it, compiled or not."""
+    import dwconv_b200 as d
+    import dwconv_b200.sequence as seq
+    x, w, vec = torch.ones(1, 4, 2), torch.ones(2, 1, 3), torch.ones(2)
+    native = seq._nodes
+    try:
+        for seq._nodes in {native, None}:
+            with torch.autograd.forward_ad.dual_level():
+                t = torch.autograd.forward_ad.make_dual(x, x)
+                row = torch.autograd.forward_ad.make_dual(x[:, 0], x[:, 0])
+                for call in (lambda: d.depthwise_conv1d_causal(t, w), lambda: d.layer_norm(t),
+                             lambda: d.gated_linear_recurrence(x, t, x, vec),
+                             lambda: d.layer_norm(x[0], torch.autograd.forward_ad.make_dual(vec, vec)),
+                             lambda: d.depthwise_conv1d_causal_step(row, w, torch.zeros(1, 2, 2)),
+                             lambda: d.gated_linear_recurrence_step(row, row, row, vec, torch.zeros(1, 2))):
+                    with pytest.raises(RuntimeError, match="forward-mode differentiation is not supported"):
+                        call()
+    finally:
+        seq._nodes = native
+
+
 def test_module_surfaces():
     import dwconv_b200 as d
     c = d.CausalDepthwiseConv1d(6, 4)
