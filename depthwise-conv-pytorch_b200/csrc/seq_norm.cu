@@ -86,7 +86,7 @@ template <typename T, int V, int NV> struct RowPart {
 
 // BLOCK: rows of tpr > 32 threads, blockDim / tpr of them at a time; otherwise 32 / tpr rows per warp.
 template <typename T, int V, int NV, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? NORM_CTA : NORM_ROW_THREADS, BLOCK ? 2 : 6)
+__global__ void __launch_bounds__(BLOCK ? NORM_CTA : NORM_ROW_THREADS, BLOCK ? 2 : (V * NV > 24 ? 4 : 6))
 norm_forward_kernel(const T *__restrict__ x, const T *__restrict__ w, const T *__restrict__ b, T *__restrict__ y,
                     float2 *stats, NormParams p) {
   using R = RowPart<T, V, NV>;
@@ -345,6 +345,10 @@ norm_backward_wide_kernel(const T *x, const T *w, const float2 *stats, const T *
 
 // ---- variant selection -------------------------------------------------------------------------
 
+// Values of a row that a thread holds at most: rows within a warp, rows that span warps (whose CTAs have
+// fewer registers per thread), and the backward pass, which keeps the sums of dw and db beside the row.
+constexpr int NORM_MOST_WARP = 48, NORM_MOST = 16;
+
 struct NormShape {
   int V, NV, tpr;  // tpr 0: the wide kernels
 };
@@ -356,16 +360,24 @@ inline int pow2_at_least(int v) {
 }
 
 // The split of a row among threads that hold at most 16 values (8 in vectors of one element) with the
-// fewest idle places; among equals the one with most values per thread (fewer steps in the row's sums).
-// `es`: bytes of an element, 0: vectors of one element only.
-inline NormShape norm_shape(int C, int es) {
-  static const NormShape choices[] = {{8, 1, 0}, {8, 2, 0}, {4, 1, 0}, {4, 2, 0}, {4, 3, 0}, {4, 4, 0}, {1, 1, 0}, {1, 2, 0}, {1, 4, 0}, {1, 8, 0}};
+// fewest idle places; among equals the one with most values per thread (fewer steps in the row's sums, more
+// bytes on their way).  `es`: bytes of an element, 0: vectors of one element only.
+//
+// With `most` = NORM_MOST_WARP also 3 and 6 vectors of 8, where they keep within a warp rows that would
+// not fit one otherwise: no barriers.  Forward, 16 bits, against 3 vectors of 4: 200704 rows of 768, 113 us and
+// 143; 131072 of 1536, 143 and 190; 200704 of 96, 22 and 25.  6 vectors are for rows that 3 do not hold (of 96:
+// 24) and for more than a few per warp (8192 rows of 1536: 20 and 18).  4 vectors against 2 made no
+// difference on rows of 64 to 1024 and are not in the choice.
+inline NormShape norm_shape(int C, int es, int most, long long rows) {
+  static const NormShape choices[] = {{8, 1, 0}, {8, 2, 0}, {8, 3, 0}, {8, 6, 0}, {4, 1, 0}, {4, 2, 0},
+                                      {4, 3, 0}, {4, 4, 0}, {1, 1, 0}, {1, 2, 0}, {1, 4, 0}, {1, 8, 0}};
   NormShape best{1, 0, 0};
   long long cost = 0;
   for (const NormShape &n : choices) {
+    if (n.V * n.NV > most || (n.NV == 6 && rows < 16384)) continue;
     if (n.V != 1 ? (es == 0 || n.V * es > 16 || C % n.V != 0) : es != 0) continue;
     const int tpr = pow2_at_least(ceil_div(C / n.V, n.NV));
-    if (tpr > NORM_CTA) continue;
+    if (tpr > (n.V * n.NV > NORM_MOST ? 32 : NORM_CTA) || (n.NV == 6 && tpr < 32)) continue;
     const long long places = (long long)tpr * n.NV * n.V;
     if (best.tpr == 0 || places < cost || (places == cost && n.V * n.NV > best.V * best.NV)) {
       best = NormShape{n.V, n.NV, tpr};
@@ -434,13 +446,16 @@ void forward_t(const void *xv, const void *wv, const void *bv, void *yv, float *
   constexpr int V = 16 / sizeof(T);
   const bool vec = p.C % V == 0 && p.xs % V == 0 && aligned_to(x, 16) && aligned_to(y, 16) &&
                    (!w || aligned_to(w, 16)) && (!b || aligned_to(b, 16));
-  const NormShape sh = norm_shape(p.C, vec ? (int)sizeof(T) : 0);
+  const NormShape sh = norm_shape(p.C, vec ? (int)sizeof(T) : 0, NORM_MOST_WARP, p.rows);
   p.tpr = sh.tpr;
   if (sh.tpr == 0) {
     const int grid = (int)(p.rows < 148 * 2 ? p.rows : 148 * 2);
     norm_forward_wide_kernel<T><<<grid, WIDE_THREADS, 0, st>>>(x, w, b, y, s2, p);
     return;
   }
+  if constexpr (sizeof(T) == 2)
+    if (sh.V == 8 && sh.NV >= 3)
+      return sh.NV == 3 ? launch_forward<T, 8, 3>(x, w, b, y, s2, p, st) : launch_forward<T, 8, 6>(x, w, b, y, s2, p, st);
   DWB_NORM_SWITCH(launch_forward, x, w, b, y, s2, p, st)
 }
 
@@ -454,7 +469,7 @@ int backward_t(const void *xv, const void *wv, const float *stats, const void *d
   constexpr int V = 16 / sizeof(T);
   const bool vec = p.C % V == 0 && p.xs % V == 0 && p.dys % V == 0 && aligned_to(x, 16) && aligned_to(dy, 16) &&
                    aligned_to(dx, 16) && (!w || aligned_to(w, 16));
-  const NormShape sh = norm_shape(p.C, vec ? (int)sizeof(T) : 0);
+  const NormShape sh = norm_shape(p.C, vec ? (int)sizeof(T) : 0, NORM_MOST, p.rows);
   p.tpr = sh.tpr;
   int parts = (int)(p.rows < 148 * 2 ? p.rows : 148 * 2);
   if (sh.tpr == 0) {

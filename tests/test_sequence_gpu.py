@@ -442,6 +442,44 @@ def test_norm_of_many_rows(C, dtype):
     ref.check(dx[rows], want["dx"], tol["dx"], dtype, "dx")
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("rows", [1, 37, 9001])
+@pytest.mark.parametrize("C", [24, 48, 88, 192, 376, 744, 768])
+def test_norm_of_three_wide_vectors_per_thread(C, rows, dtype):
+    """Rows within a warp whose threads hold three vectors, full ones and with places beyond the row; and
+    the same rows off 16-byte boundaries, which go another way."""
+    import dwconv_b200 as d
+    g = torch.Generator().manual_seed(54)
+    x = (torch.randn(rows, C + 1, generator=g) * 2 - 0.5).to(dtype).cuda()
+    w, b = (1 + 0.3 * torch.randn(C, generator=g)).to(dtype).cuda(), randn(g, C, dtype=dtype, grad=False)
+    for rows_of_x in (x[:, :C].contiguous(), x[:, :C]):
+        want, tol = ref.norm(rows_of_x, w, b, 1e-5)
+        ref.check(d.layer_norm(rows_of_x, w, b), want["y"], tol["y"], dtype, "y")
+        leaf = rows_of_x.clone().requires_grad_()
+        dy = randn(g, rows, C, dtype=dtype, grad=False)
+        y = d.layer_norm(leaf, w, b)
+        want, tol = ref.norm(rows_of_x, w, b, 1e-5, dy)
+        ref.check(y, want["y"], tol["y"], dtype, "y")
+        ref.check(torch.autograd.grad(y, leaf, dy)[0], want["dx"], tol["dx"], dtype, "dx")
+
+
+@pytest.mark.parametrize("C", [784, 1200, 1528, 1536])
+def test_norm_of_six_wide_vectors_per_thread(C):
+    """Many rows that one warp holds in six vectors per thread; a slice of them against the definition, and
+    all of them against calls with few rows, which hold them otherwise."""
+    import dwconv_b200 as d
+    g = torch.Generator().manual_seed(55)
+    rows = 16384 + 5
+    x = (torch.randn(rows, C, generator=g) * 2 - 0.5).to(torch.bfloat16).cuda()
+    w, b = (1 + 0.3 * torch.randn(C, generator=g)).to(x.dtype).cuda(), randn(g, C, dtype=x.dtype, grad=False)
+    y = d.layer_norm(x, w, b)
+    want, tol = ref.norm(x[-700:], w, b, 1e-5)
+    ref.check(y[-700:], want["y"], tol["y"], x.dtype, "y")
+    few = torch.cat([d.layer_norm(part, w, b) for part in x.split(4096)])
+    # each side is off by half a step of its value and the fp32 difference before it
+    assert ((y.float() - few.float()).abs() <= 2 ** -7 * few.float().abs() + 1e-4).all()
+
+
 def test_norm_far_from_zero_and_constant_rows():
     g = torch.Generator().manual_seed(19)
     for C in (40, 1000, 20000):
