@@ -616,10 +616,12 @@ class GatedLinearRecurrence(nn.Module):
         self.decay = nn.Parameter(torch.log(torch.expm1(-torch.log(a) / scale)).float())
 
     def _apply(self, fn, recurse=True):
-        kept = self.decay.data
+        kept, grad = self.decay.data, self.decay.grad
+        grad = None if grad is None else grad.data
         out = super()._apply(fn, recurse)
         if self.decay.dtype != torch.float32:
             self.decay.data = kept.to(self.decay.device)
+            self.decay.grad = None if grad is None else grad.to(self.decay.device)
         return out
 
     def forward(self, input, recurrence_gate, input_gate, initial_state=None, offsets=None, return_state=False):

@@ -153,6 +153,19 @@ def differences(f, args, grads, gen, h=1e-5):
         assert abs((ends[0] - ends[1]) / (2 * h) - want) <= 1e-7 * (1 + abs(want)), name
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float64])
+def test_a_converted_recurrence_keeps_its_gradient_too(dtype):
+    import dwconv_b200 as d
+    r = d.GatedLinearRecurrence(5)
+    value, grad = r.decay.detach().clone(), torch.randn(5)
+    r.decay.grad = grad.clone()
+    r.to(dtype)
+    assert r.decay.dtype == r.decay.grad.dtype == torch.float32
+    assert torch.equal(r.decay, value) and torch.equal(r.decay.grad, grad)
+    torch.optim.SGD(r.parameters(), lr=1.).step()
+    assert torch.equal(r.decay, value - grad)
+
+
 def test_the_definitions_gradients_are_derivatives():
     gen = torch.Generator().manual_seed(21)
 
