@@ -198,12 +198,44 @@ __device__ __forceinline__ void rows_load(void *to, const CUtensorMap *map, int 
       "l"(map), "r"(c), "r"(t), "r"(b), "r"(smem_u32(bar))
       : "memory");
 }
-// Bounded wait for what this CTA's copies and its peers' stores signal.  A wait that runs out raises the
-// flag that dwconv_b200_device_status reports; the kernel goes on to its end.  (The wait acquires at CTA
-// scope: what it waits for lies in this CTA's shared memory, counted by the barrier as it arrives.  At
-// cluster scope every poll would throw the L1 cache away as well.)
-__device__ __forceinline__ void wait_or_flag(uint64_t *bar, uint32_t parity) {
-  if (!mbar_wait_bounded(bar, parity) && (threadIdx.x & 31) == 0) atomicExch(&g_seq_error_flag, 8);
+// What became of a CTA's waits (beside the barriers, in shared memory).
+struct RecWaits {
+  int give_up;    // from this iteration on the CTA has no part in the cluster's exchange
+  int stuck[8];   // by warp: 0, or 1 + the parity of the copies that it waited for in vain
+  int sent[16];   // by rank, at the end: the iterations whose pairs that CTA has sent
+};
+__device__ __forceinline__ int look_at(const int &word) { return *(const volatile int *)&word; }
+__device__ __forceinline__ bool mbar_test_wait(uint64_t *bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Bounded waits.  One that runs out raises the flag that dwconv_b200_device_status reports; the kernel goes on to its
+// end, but a barrier whose phase is not complete is not armed again: a warp copies no more rows ahead, or the CTA has
+// no more part in its cluster's exchange (nor waits for it again).  (The waits acquire at CTA scope: what they wait
+// for lies in this CTA's shared memory, counted by the barrier as it arrives.  At cluster scope every poll would throw
+// the L1 cache away as well.)  Lanes poll for themselves: any that fails says so, in front of the warp's or the CTA's
+// next barrier.
+__device__ __forceinline__ bool wait_polls(uint64_t *bar, uint32_t parity, unsigned polls) {
+  for (unsigned i = 0; i < polls; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return false;
+}
+__device__ __forceinline__ void wait_copies(uint64_t *bar, uint32_t parity, unsigned polls, int &stuck) {
+  if (mbar_test_wait(bar, parity) || look_at(stuck) != 0 || wait_polls(bar, parity, polls)) return;
+  atomicExch(&g_seq_error_flag, 8);
+  stuck = 1 + (int)parity;
+}
+__device__ __forceinline__ void wait_peers(uint64_t *bar, int iteration, unsigned polls, int &give_up) {
+  if (wait_polls(bar, iteration >> 1 & 1, polls)) return;
+  atomicExch(&g_seq_error_flag, 8);
+  atomicMin(&give_up, iteration + 1);
 }
 
 // Rows at T and behind: a gate of -infinity is closed, the state passes through it.  Every lane
@@ -305,6 +337,47 @@ __device__ __forceinline__ void store_peer(const void *mine, const uint64_t *bar
       : "memory");
 }
 
+// The bytes of which no store will tell this CTA's barrier.
+__device__ __forceinline__ void complete_tx(uint64_t *bar, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void store_peer_word(const int *mine, int rank, int v) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(mine)), "r"(rank));
+  asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
+
+// The end of a cluster's walk, for every thread of it: no CTA leaves before its peers have sent it all they
+// will, nor, where a wait ran out, before that has landed.
+// A CTA sends the pairs of iteration n only where it has all pairs of n - 1.  One that gives up before iteration n has
+// sent those of n - 1, for which its barrier still waits, and its peers may have sent theirs of n, for which it has
+// not armed its barrier; nobody can have sent more.
+__device__ __forceinline__ void leave_cluster(RecWaits *waits, uint64_t *met, int cs, int rank, int steps) {
+  __syncthreads();
+  const int n = waits->give_up;
+  if (threadIdx.x < cs) store_peer_word(&waits->sent[rank], threadIdx.x, min(n, steps));
+  __syncwarp();
+  cluster_arrive();
+  cluster_wait();
+  if (n > steps || threadIdx.x != 0) return;
+  uint32_t missing = 0, ahead = 0;
+  for (int r = 0; r < cs; ++r) {
+    missing += waits->sent[r] < n ? 512 : 0;
+    ahead += waits->sent[r] > n ? 512 : 0;
+  }
+  uint64_t *bar = met + ((n - 1) & 1), *next = met + (n & 1);
+  if (missing > 0) complete_tx(bar, missing);
+  (void)mbar_wait_bounded(bar, (n - 1) >> 1 & 1);
+  if (ahead == 0) return;
+  mbar_arrive_expect_tx(next, ahead);
+  (void)mbar_wait_bounded(next, n >> 1 & 1);
+}
+// The end of a warp's walk: copies that it waited for in vain land before the CTA's shared memory is another's.
+__device__ __forceinline__ void land_copies(uint64_t *bar, const int &stuck) {
+  const int s = look_at(stuck);
+  if (s != 0) (void)mbar_wait_bounded(bar, s - 1);
+}
+
 // The warp's number, known to the compiler to be the same in all its lanes.
 __device__ __forceinline__ int uniform_warp() { return __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0); }
 
@@ -312,6 +385,8 @@ struct RecParams {
   SeqList q;
   int B, groups, cs;  // cs: CTAs of a cluster
   float scale;
+  unsigned polls;  // of a wait, before it has run out
+  int leaver;      // -1, or the rank of a CTA that gives up before iteration 1 (dwconv_b200_debug_expire)
 };
 
 // Sequences without a row: what enters leaves.
@@ -325,7 +400,7 @@ __device__ __forceinline__ void empty_states(const RecParams &p, int warp, const
 // Shared memory of a CTA of W warps: the rows of NT tensors (FAST), barriers, the pairs of the warps for two
 // tiles, what enters the CTA's tile (two), backward the rows' decays, the pairs of the cluster for two tiles, PACKED the first offsets.
 template <typename T> constexpr int rec_stage(int W, int NT) { return W * REC_L * REC_GROUP * NT * (int)sizeof(T); }
-constexpr int REC_BARRIERS = 256;  // one per warp for its copies, two for the cluster's pairs
+constexpr int REC_BARRIERS = 256;  // one per warp for its copies, two for the cluster's pairs; from 128 on RecWaits
 constexpr int REC_OFFSETS = 1024;  // as many offsets of packed sequences are kept in shared memory
 constexpr int rec_smem(int W, int stage, bool backward, bool packed, int cs) {
   return stage + (packed ? REC_OFFSETS * 4 : 0) + (backward ? 0 : 2 * 32 * 8) + REC_BARRIERS + 2 * W * 32 * (backward ? 24 : 16) + (backward ? W * REC_L * REC_GROUP * 4 : 0) +
@@ -341,14 +416,17 @@ __device__ __forceinline__ void keep_offsets(SeqList &q, int *kept) {
 }
 
 // Barriers of a CTA; with clusters, a peer's shared memory may be written once the peer has passed here.
-template <int W, bool FAST> __device__ __forceinline__ void start_cta(uint64_t *bars, int cs) {
-  if (!FAST && cs == 1) return;
+template <int W, bool FAST>
+__device__ __forceinline__ void start_cta(uint64_t *bars, RecWaits *waits, const RecParams &p, int rank) {
+  if (!FAST && p.cs == 1) return;
   if (threadIdx.x == 0) {
+    waits->give_up = rank == p.leaver ? 1 : 0x7fffffff;
+    for (int n = 0; n < W; ++n) waits->stuck[n] = 0;
     for (int n = 0; n < W + 2; ++n) mbar_init(bars + n, 1);
     fence_barrier_init();
   }
   __syncthreads();
-  if (cs > 1) {
+  if (p.cs > 1) {
     cluster_arrive();
     cluster_wait();
   }
@@ -369,6 +447,7 @@ __device__ __forceinline__ void forward_body(const RecMaps &maps, SeqIn<T> x, Se
   extern __shared__ __align__(128) unsigned char smem[];
   T *stage = reinterpret_cast<T *>(smem);
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (FAST ? rec_stage<T>(W, NT) : 0)), *met = bars + W;
+  RecWaits *waits = reinterpret_cast<RecWaits *>(bars + 16);
   float4(*agg)[W][32] = reinterpret_cast<float4(*)[W][32]>(reinterpret_cast<unsigned char *>(bars) + REC_BARRIERS);
   float2(*entry)[32] = reinterpret_cast<float2(*)[32]>(agg + 2);  // [2]: the state that enters the CTA's tile
   float4 *far = reinterpret_cast<float4 *>(entry + 2);            // [2][cs][32]
@@ -382,7 +461,7 @@ __device__ __forceinline__ void forward_body(const RecMaps &maps, SeqIn<T> x, Se
   T *mine = stage + warp * (NT * L * REC_GROUP);
   const int col = c.c0 - grp * REC_GROUP;  // of this lane in the staged rows
   auto start_copies = [&](int tile) {
-    if (lane == 0) {
+    if (lane == 0 && look_at(waits->stuck[warp]) == 0) {
       const int t = tile * TILE + warp * L;
       mbar_arrive_expect_tx(bars + warp, NT * L * REC_GROUP * (uint32_t)sizeof(T));
 #pragma unroll
@@ -394,7 +473,7 @@ __device__ __forceinline__ void forward_body(const RecMaps &maps, SeqIn<T> x, Se
     int *kept = reinterpret_cast<int *>(far + (p.cs > 1 ? 2 * p.cs * 32 : 0));
     keep_offsets(q, kept);
   }
-  start_cta<W, FAST>(bars, p.cs);
+  start_cta<W, FAST>(bars, waits, p, rank);
   if (FAST && steps > 0) start_copies(rank);
   if (PACKED && fin != nullptr && rank == 0) empty_states<W>(p, warp, initial, fin, c);
   RowWalk walk;
@@ -410,14 +489,13 @@ __device__ __forceinline__ void forward_body(const RecMaps &maps, SeqIn<T> x, Se
   if (PACKED && steps > 0) look(rank * TILE + warp * L);
   for (int it = 0; it < steps; ++it) {
     const int tile = it * p.cs + rank, t0 = tile * TILE + warp * L, rows = p.q.T - t0, half = it & 1;
-    if (p.cs > 1 && threadIdx.x == 0) mbar_arrive_expect_tx(met + half, p.cs * 512);
     float2 a[L], bb[L];
     const RowMasks m = next_m;
     const float2 first = next_entry;
     {
       typename Q::Raw rx[L], ru[L], rv[L];
       if constexpr (FAST) {
-        wait_or_flag(bars + warp, it & 1);
+        wait_copies(bars + warp, it & 1, p.polls, waits->stuck[warp]);
         if (!PACKED && rows < L) close_rows<T>(mine + L * REC_GROUP, rows, col);
 #pragma unroll
         for (int j = 0; j < L; ++j) {
@@ -475,13 +553,18 @@ __device__ __forceinline__ void forward_body(const RecMaps &maps, SeqIn<T> x, Se
     bool cuts = false;  // whether a sequence begins in this CTA's tile
     if (PACKED) cuts = __syncthreads_or((int)(m.start | m.none));
     else __syncthreads();
+    const bool part = p.cs > 1 && look_at(waits->give_up) > it;
     if (p.cs > 1 && warp < p.cs) {
       // the CTA's pair, folded by each of the warps that pass it on
       float2 TP = f2(1.f), TH = f2(0.f);
       if (cuts) fold<PACKED, W>(agg[half], lane, 0, W, TP, TH);
       else fold<false, W>(agg[half], lane, 0, W, TP, TH);
       float4 *there = far + (half * p.cs + rank) * 32 + lane;
-      for (int peer = warp; peer < p.cs; peer += W) store_peer(there, met + half, peer, make_float4(TP.x, TP.y, TH.x, TH.y));
+      if (part) {
+        for (int peer = warp; peer < p.cs; peer += W)
+          store_peer(there, met + half, peer, make_float4(TP.x, TP.y, TH.x, TH.y));
+        if (threadIdx.x == 0) mbar_arrive_expect_tx(met + half, p.cs * 512);
+      }
     }
     float2 h = carry;
     if (p.cs > 1) {
@@ -491,7 +574,7 @@ __device__ __forceinline__ void forward_body(const RecMaps &maps, SeqIn<T> x, Se
       else fold<false, W>(agg[half], lane, 0, warp, FP, FH);
       if (PACKED && it + 1 < steps) look(t0 + p.cs * TILE);
       if (warp == 0) {  // one warp waits for the peers' pairs and folds them for all
-        wait_or_flag(met + half, it >> 1 & 1);
+        if (part) wait_peers(met + half, it, p.polls, waits->give_up);
         for (int w = 0; w < p.cs; ++w) {
           if (w == rank) entry[half][lane] = carry;
           const float4 e = far[(half * p.cs + w) * 32 + lane];
@@ -532,6 +615,8 @@ __device__ __forceinline__ void forward_body(const RecMaps &maps, SeqIn<T> x, Se
     }
   }
   if (!PACKED && fin != nullptr && rank == 0 && warp == 0) store_state(fin, b, C, c, carry);
+  if (FAST) land_copies(bars + warp, waits->stuck[warp]);
+  if (p.cs > 1) leave_cluster(waits, met, p.cs, rank, steps);
 }
 
 constexpr int REC_BW = REC_CKPT / REC_L;  // warps of a backward CTA: its tile starts from a kept state
@@ -546,6 +631,7 @@ __device__ __forceinline__ void backward_body(const RecMaps &maps, SeqIn<T> x, S
   extern __shared__ __align__(128) unsigned char smem[];
   T *stage = reinterpret_cast<T *>(smem);
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (FAST ? rec_stage<T>(W, NT) : 0)), *met = bars + W;
+  RecWaits *waits = reinterpret_cast<RecWaits *>(bars + 16);
   // P, H of each warp's rows, and what leaves them towards earlier rows
   float4(*agg)[W][32] = reinterpret_cast<float4(*)[W][32]>(reinterpret_cast<unsigned char *>(bars) + REC_BARRIERS);
   float2(*aggq)[W][32] = reinterpret_cast<float2(*)[W][32]>(agg + 2);
@@ -561,7 +647,7 @@ __device__ __forceinline__ void backward_body(const RecMaps &maps, SeqIn<T> x, S
   T *mine = stage + warp * (NT * L * REC_GROUP);
   const int col = c.c0 - grp * REC_GROUP;  // of this lane in the staged rows
   auto start_copies = [&](int tile) {
-    if (lane == 0) {
+    if (lane == 0 && look_at(waits->stuck[warp]) == 0) {
       const int t = tile * TILE + warp * L;
       mbar_arrive_expect_tx(bars + warp, NT * L * REC_GROUP * (uint32_t)sizeof(T));
 #pragma unroll
@@ -573,7 +659,7 @@ __device__ __forceinline__ void backward_body(const RecMaps &maps, SeqIn<T> x, S
     int *kept = reinterpret_cast<int *>(far + (p.cs > 1 ? 2 * p.cs * 32 : 0));
     keep_offsets(list, kept);
   }
-  start_cta<W, FAST>(bars, p.cs);
+  start_cta<W, FAST>(bars, waits, p, rank);
   if (FAST && steps > 0) start_copies((steps - 1) * p.cs + rank);
   if (PACKED && dinit != nullptr && rank == 0) empty_states<W>(p, warp, dfin, dinit, c);
   RowWalk walk;
@@ -582,10 +668,9 @@ __device__ __forceinline__ void backward_body(const RecMaps &maps, SeqIn<T> x, S
   RowMasks next_m{0u, 0u, 0u, -1, -1};
   if (PACKED && steps > 0) next_m = walk.masks<L>(list, ((steps - 1) * p.cs + rank) * TILE + warp * L);
   for (int it = steps - 1; it >= 0; --it) {
-    const int n = steps - 1 - it, half = n & 1, phase = n >> 1 & 1;
+    const int n = steps - 1 - it, half = n & 1;
     const int tile = it * p.cs + rank, t0 = tile * TILE + warp * L;
     const int rows = p.q.T - t0;
-    if (p.cs > 1 && threadIdx.x == 0) mbar_arrive_expect_tx(met + half, p.cs * 512);
     const RowMasks mk = next_m;
     const unsigned special = mk.start | mk.none;
     float2 h = f2(0.f);
@@ -595,7 +680,7 @@ __device__ __forceinline__ void backward_body(const RecMaps &maps, SeqIn<T> x, S
     {
       typename Q::Raw ru[L], rv[L], rg[L];
       if constexpr (FAST) {
-        wait_or_flag(bars + warp, n & 1);
+        wait_copies(bars + warp, n & 1, p.polls, waits->stuck[warp]);
         if (!PACKED && rows < L) close_rows<T>(mine + L * REC_GROUP, rows, col);
 #pragma unroll
         for (int j = 0; j < L; ++j) {
@@ -666,6 +751,7 @@ __device__ __forceinline__ void backward_body(const RecMaps &maps, SeqIn<T> x, S
     float2 q = carry;
     if (p.cs > 1) {
       float4 *there = far + (half * p.cs + rank) * 32 + lane;
+      const bool part = look_at(waits->give_up) > n;
       if (warp < p.cs) {
         float2 TP = f2(1.f), TG = f2(0.f);
 #pragma unroll
@@ -675,9 +761,13 @@ __device__ __forceinline__ void backward_body(const RecMaps &maps, SeqIn<T> x, S
           TG = apply<PACKED>(P2, aggq[half][w][lane], TG);
           TP = join<PACKED>(TP, P2);
         }
-        for (int peer = warp; peer < p.cs; peer += W) store_peer(there, met + half, peer, make_float4(TP.x, TP.y, TG.x, TG.y));
+        if (part) {
+          for (int peer = warp; peer < p.cs; peer += W)
+            store_peer(there, met + half, peer, make_float4(TP.x, TP.y, TG.x, TG.y));
+          if (threadIdx.x == 0) mbar_arrive_expect_tx(met + half, p.cs * 512);
+        }
       }
-      wait_or_flag(met + half, phase);
+      if (part) wait_peers(met + half, n, p.polls, waits->give_up);
       for (int w = p.cs - 1; w >= 0; --w) {
         if (w == rank) q = carry;
         const float4 e = far[(half * p.cs + w) * 32 + lane];
@@ -739,6 +829,7 @@ __device__ __forceinline__ void backward_body(const RecMaps &maps, SeqIn<T> x, S
     ddecay = add2(ddecay, sum);
   }
   if (!PACKED && dinit != nullptr && rank == 0 && warp == 0) store_state(dinit, b, C, c, carry);
+  if (FAST) land_copies(bars + warp, waits->stuck[warp]);
   // this CTA's part of ddecay: the warps' sums in order
   __syncthreads();
   aggq[0][warp][lane] = ddecay;
@@ -749,6 +840,7 @@ __device__ __forceinline__ void backward_body(const RecMaps &maps, SeqIn<T> x, S
     for (int w = 1; w < W; ++w) s = add2(s, aggq[0][w][lane]);
     store_state(part, (long long)b * p.cs + rank, C, c, s);
   }
+  if (p.cs > 1) leave_cluster(waits, met, p.cs, rank, steps);
 }
 
 __device__ __forceinline__ Rate rate_of(const float *decay, float scale, const Chan &c) {
@@ -855,8 +947,14 @@ inline RecChoice rec_cluster(const dwconv_b200_sequence &s, const RecShape &r) {
   return best;
 }
 
+std::atomic<int> g_expire{0};  // dwconv_b200_debug_expire
+constexpr unsigned REC_SHORT_POLLS = 64;  // some milliseconds
+
 inline RecParams rec_params(const dwconv_b200_sequence &s, float scale, int cs) {
   RecParams p;
+  const int expire = g_expire.load(std::memory_order_relaxed);
+  p.polls = expire == 0 ? ROWS_WAIT_LIMIT : (expire == 1 ? 0 : REC_SHORT_POLLS);
+  p.leaver = expire == 2 ? cs - 1 : -1;
   p.q = seq_list(s);
   p.B = s.B;
   p.groups = ceil_div(s.C, REC_GROUP);
@@ -1012,6 +1110,8 @@ int seq_take_error() {
 using namespace dwb;
 
 extern "C" {
+
+int dwconv_b200_debug_expire(int how) { return g_expire.exchange(how == 1 || how == 2 ? how : 0); }
 
 size_t dwconv_b200_recurrence_checkpoint_bytes(const dwconv_b200_sequence *seq) {
   if (check_recurrence(DWCONV_B200_F32, seq) != DWCONV_B200_OK) return 0;

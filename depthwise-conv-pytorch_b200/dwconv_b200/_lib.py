@@ -61,6 +61,7 @@ def _load():
         "dwconv_b200_set_path": (ci, [ci]),
         "dwconv_b200_last_path": (ci, []),
         "dwconv_b200_device_status": (ci, []),
+        "dwconv_b200_debug_expire": (ci, [ci]),
         "dwconv_b200_debug_plan": (ci, [ci, ci, sp, ci, ctypes.POINTER(ci)]),
         "dwconv_b200_out_size": (ci, [ci] * 6),
         "dwconv_b200_forward": (ci, [vp, vp, vp, ci, sp, vp]),
@@ -155,7 +156,7 @@ native = _load_native()
 EXPORTS = (
     "dwconv_b200_version", "dwconv_b200_status_string", "dwconv_b200_last_cuda_error",
     "dwconv_b200_set_path", "dwconv_b200_last_path", "dwconv_b200_device_status",
-    "dwconv_b200_debug_plan", "dwconv_b200_out_size",
+    "dwconv_b200_debug_expire", "dwconv_b200_debug_plan", "dwconv_b200_out_size",
     "dwconv_b200_forward", "dwconv_b200_forward_epilogue", "dwconv_b200_backward_input",
     "dwconv_b200_backward_filter_workspace_bytes", "dwconv_b200_backward_filter",
     "dwconv_b200_forward_nhwc", "dwconv_b200_backward_input_nhwc", "dwconv_b200_backward_filter_nhwc",

@@ -98,6 +98,11 @@ DWCONV_B200_API int dwconv_b200_last_cuda_error(void);
  * Diagnostic: not needed on the hot path.  No counterpart in the reference. */
 DWCONV_B200_API int dwconv_b200_device_status(void);
 
+/* Testing: makes waits of the recurrence run out, with wrong output and bit 3 of the status above raised.
+ * 1: every wait whose condition does not hold yet; 2: in each cluster the last CTA leaves the exchange early, and the
+ * others' waits for it run out after some milliseconds; 0: none.  Process-wide; returns the previous value. */
+DWCONV_B200_API int dwconv_b200_debug_expire(int how);
+
 /* Host-only: the kernel variant and tiling the rows family would use for an operator
  * (op 0 forward, 1 backward-input, 2 backward-filter, 3 fused backward), as 24 ints; returns 0 if that family
  * declines the problem.  For tests that model the kernels' index arithmetic on the CPU.

@@ -1,0 +1,64 @@
+"""The sequence operators on the GPU where something goes wrong or is out of the ordinary: waits that run out,
+non-finite parameters, gradients of gradients, saved tensors, mixed precision, long runs and many rows."""
+import pytest
+import torch
+
+import sequence_util as ref
+from test_sequence_gpu import DTYPES, by_dtype, conv_inputs, packed, randn, recurrence_inputs
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- waits that run out ------------------------------------------------------------------------
+
+@pytest.fixture
+def expire():
+    """Makes waits run out, or (0) leaves them as they are."""
+    from dwconv_b200 import _lib
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 0
+    yield _lib.lib.dwconv_b200_debug_expire
+    _lib.lib.dwconv_b200_debug_expire(0)
+    _lib.device_status()
+
+
+@by_dtype
+@pytest.mark.parametrize("lengths", [None, [700, 0, 1, 1299]], ids=["dense", "packed"])
+@pytest.mark.parametrize("size", [(1, 2000, 64), (1, 2000, 63), (2, 1000, 200), (1, 8, 64), (1, 40, 63), (1, 8, 63)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_a_wait_that_runs_out_is_reported_and_ends(size, lengths, dtype, expire):
+    """Rows copied ahead (even widths) and read in place (odd ones), alone and in clusters of CTAs, some of which
+    leave early while their peers wait in vain: the kernels end, say so, and leave the device as they found it."""
+    import dwconv_b200 as d
+    from dwconv_b200 import _lib
+    B, T, C = size
+    offsets = on_gpu = None
+    n = B
+    if lengths is not None:
+        if (B, T) != (1, 2000):
+            pytest.skip("the list has 2000 rows")
+        offsets, _, on_gpu = packed(lengths)
+        n = len(lengths)
+    x, u, v, dy, decay, init, dstate = recurrence_inputs(B, T, C, n, dtype, 60, True)
+    leaves = [x, u, v, decay, init]
+
+    def both():
+        out = d.gated_linear_recurrence(x, u, v, decay, init, on_gpu, return_state=True)
+        return [t.detach() for t in out] + list(torch.autograd.grad(out, leaves, [dy, dstate]))
+
+    want = both()
+    assert _lib.device_status() == 0
+    for how in (1, 2, 2, 1):
+        expire(how)
+        both()
+        status = _lib.device_status()
+        if T >= 1000:       # clusters, and more tiles than a cluster has CTAs
+            assert status == 8
+        elif C % 2:         # no copies; no peers, or none that leave before the walk's end
+            assert status == (8 if how == 1 and T > 32 else 0)
+        else:               # the copies of the only tile, which may have landed before the first look at them
+            assert status == 0 or (status == 8 and how == 1)
+        expire(0)
+        for a, b in zip(both(), want):
+            assert torch.equal(a, b)
+        assert _lib.device_status() == 0
