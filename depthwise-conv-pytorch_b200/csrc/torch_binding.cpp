@@ -711,18 +711,16 @@ struct OnceNode : torch::autograd::Node {
   variable_list apply(variable_list &&grads) override {
     const std::lock_guard<std::mutex> lock(mutex_);
     check_capture();
-    bool twice = false, any = false;
-    for (const at::Tensor &g : grads) {
-      any = any || g.defined();
-      twice = twice || (g.defined() && g.requires_grad());
-    }
+    bool any = false;
+    for (const at::Tensor &g : grads) any = any || g.defined();
     variable_list out(num_outputs());
     if (!any) return out;
     {
       at::AutoGradMode no_grad(false);
       backward(grads, out);
     }
-    if (at::GradMode::is_enabled() && twice) {
+    // with create_graph: the gradients depend on the inputs even where those that came in are constants
+    if (at::GradMode::is_enabled()) {
       auto error = std::make_shared<torch::autograd::DelayedError>(
           "trying to differentiate twice a function that was marked with @once_differentiable", (int64_t)out.size());
       for (at::Tensor &t : out)

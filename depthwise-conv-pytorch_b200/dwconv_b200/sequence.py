@@ -15,10 +15,11 @@ Every function runs on the current stream of the input's device, never synchroni
 captured into a CUDA graph.  Gradients are first-order and reverse-mode only.  A backward pass is not
 captured while an eager graph of the same leaves is alive on the default stream (refused).
 """
+import functools
+
 import torch
 from torch import nn
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _C, _lib
 from .dwconv import _ACTIVATIONS, _native
@@ -422,6 +423,22 @@ def _activation(activation):
     return _ACTIVATIONS[activation]
 
 
+def _first_order(backward):
+    """A backward pass whose results cannot be differentiated: with ``create_graph`` they carry an error.
+    (``once_differentiable`` lets them pass as constants where the incoming gradients are constants, although
+    they depend on the inputs.)"""
+    @functools.wraps(backward)
+    def wrapped(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not torch.is_grad_enabled() or all(t is None for t in out):
+            return out
+        error = torch._C._functions.DelayedError(
+            "trying to differentiate twice a function that was marked with @once_differentiable", len(out))
+        return error(*[t if t is None else t.detach().requires_grad_() for t in out])
+    return wrapped
+
+
 class CausalConv1dFunction(Function):
     @staticmethod
     def forward(ctx, input, weight, bias, initial, offsets, act, want_state):
@@ -432,7 +449,7 @@ class CausalConv1dFunction(Function):
         return (y, state) if want_state else y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, grad, grad_state=None):
         input, weight, bias, initial, offsets = ctx.saved_tensors
         if grad is None and grad_state is None:
@@ -454,7 +471,7 @@ class GatedLinearRecurrenceFunction(Function):
         return (y, state) if want_state else y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, grad, grad_state=None):
         input, u, v, decay, initial, offsets, ckpt = ctx.saved_tensors
         if grad is None and grad_state is None:
@@ -474,7 +491,7 @@ class LayerNormFunction(Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, grad):
         input, weight, stats = ctx.saved_tensors
         dx, dw, db = _forms.layer_norm_backward(input, weight, stats, grad, ctx.needs_input_grad[1],

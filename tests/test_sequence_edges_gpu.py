@@ -62,3 +62,43 @@ def test_a_wait_that_runs_out_is_reported_and_ends(size, lengths, dtype, expire)
         for a, b in zip(both(), want):
             assert torch.equal(a, b)
         assert _lib.device_status() == 0
+
+
+# ---- autograd ----------------------------------------------------------------------------------
+
+def calls(dtype=torch.float32, B=2, T=20, C=10):
+    """Every operator over the compiled nodes and over the interpreted ones: (name, call, leaves)."""
+    import dwconv_b200 as d
+    from dwconv_b200 import sequence as S
+    g = torch.Generator().manual_seed(61)
+    x, u, v = (randn(g, B, T, C, dtype=dtype) for _ in range(3))
+    w, b = randn(g, C, 1, 4, dtype=dtype), randn(g, C, dtype=dtype)
+    decay = (torch.rand(C, generator=g) * 6 - 8).cuda().requires_grad_()
+    return [
+        ("conv", lambda: d.depthwise_conv1d_causal(x, w, b, "silu"), [x, w, b]),
+        ("conv interpreted", lambda: S.CausalConv1dFunction.apply(x, w, b, None, None, 3, False), [x, w, b]),
+        ("recurrence", lambda: d.gated_linear_recurrence(x, u, v, decay), [x, u, v, decay]),
+        ("recurrence interpreted",
+         lambda: S.GatedLinearRecurrenceFunction.apply(x, u, v, decay, None, None, 8.0, False), [x, u, v, decay]),
+        ("norm", lambda: d.layer_norm(x, b, b), [x, b]),
+        ("norm interpreted", lambda: S.LayerNormFunction.apply(x, b, b, 1e-5), [x, b]),
+    ]
+
+
+def test_a_penalty_on_gradients_is_refused_whatever_came_in():
+    """The gradients depend on the inputs; taken for constants, a penalty on them would lose its part without a word.
+    What does not differentiate them goes on."""
+    for name, call, leaves in calls():
+        first = torch.autograd.grad(call().sum(), leaves)
+        grads = torch.autograd.grad(call().sum(), leaves, create_graph=True)
+        for a, b in zip(first, grads):
+            assert torch.equal(a, b), name
+            with pytest.raises(RuntimeError, match="once_differentiable"):
+                ((b * b).sum() + (leaves[0] ** 2).sum()).backward()
+        for t in leaves:
+            t.grad = None
+        y = call()
+        y.sum().backward(create_graph=True)
+        for t, a in zip(leaves, first):
+            assert torch.equal(t.grad, a), name
+            t.grad = None
