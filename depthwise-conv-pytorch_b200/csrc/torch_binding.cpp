@@ -316,6 +316,12 @@ void check_operand(const char *fn, const char *name, const at::Tensor &t, at::In
   }
 }
 
+// What the forward call left for this one, and hooks on saved tensors may have had in hand since.
+void check_kept(const char *fn, const char *name, const at::Tensor &t, at::IntArrayRef shape, const at::Tensor &input) {
+  check_operand(fn, name, t, shape, at::kFloat, input);
+  TORCH_CHECK(t.is_contiguous(), "dwconv_b200.", fn, ": ", name, " must be contiguous");
+}
+
 dwconv_b200_sequence check_sequences(const char *fn, const at::Tensor &input, const OptTensor &offsets) {
   check_cuda(input, "input");
   sequence_dtype(input);
@@ -539,6 +545,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, OptTensor> recurrence
     if (want_initial) dinit = state_or_zeros(grad_state, r.state, wide);
     return {dx, du, dv, at::zeros(decay.sizes(), wide), dinit};
   }
+  check_kept(fn, "checkpoints", ckpt, {(int64_t)(dwconv_b200_recurrence_checkpoint_bytes(&r.s) / 4)}, input);
   at::Tensor dd = at::empty(decay.sizes(), wide);
   if (want_initial) dinit = at::empty(r.state, wide);
   const at::Tensor x = rows_of(input), u = rows_of(gate_u), v = rows_of(gate_v), d = decay.contiguous();
@@ -646,6 +653,7 @@ std::tuple<at::Tensor, OptTensor, OptTensor> layer_norm_backward(const at::Tenso
     if (want_bias) db = at::zeros({C}, input.options());
     return {dx, dw, db};
   }
+  check_kept(fn, "stats", stats, {rows, 2}, input);
   if (want_weight) dw = at::empty({C}, input.options());
   if (want_bias) db = at::empty({C}, input.options());
   const at::Tensor x = norm_rows(input), g = norm_rows(grad);
@@ -785,18 +793,16 @@ py::object conv1d_causal_autograd(const at::Tensor &input, const at::Tensor &wei
 }
 
 struct RecurrenceNode : OnceNode {
-  SavedVariable input, u, v, decay, initial, offsets;
-  at::Tensor ckpt;
+  SavedVariable input, u, v, decay, initial, offsets, ckpt;
   double scale;
   std::string name() const override { return "GatedLinearRecurrenceBackward"; }
   void release_variables() override {
-    for (SavedVariable *s : {&input, &u, &v, &decay, &initial, &offsets}) s->reset_data();
-    ckpt.reset();
+    for (SavedVariable *s : {&input, &u, &v, &decay, &initial, &offsets, &ckpt}) s->reset_data();
   }
   void backward(const variable_list &grads, variable_list &out) override {
     auto [dx, du, dv, dd, dinit] = recurrence_backward(
-        saved(input), saved(u), saved(v), saved(decay), saved_or_none(initial), saved_or_none(offsets), scale, ckpt,
-        or_none(grads[0]), grads.size() > 1 ? or_none(grads[1]) : OptTensor(), task_should_compute_output(4));
+        saved(input), saved(u), saved(v), saved(decay), saved_or_none(initial), saved_or_none(offsets), scale,
+        saved(ckpt), or_none(grads[0]), grads.size() > 1 ? or_none(grads[1]) : OptTensor(), task_should_compute_output(4));
     out[0] = dx;
     out[1] = du;
     out[2] = dv;
@@ -825,7 +831,7 @@ py::object recurrence_autograd(const at::Tensor &input, const at::Tensor &u, con
     n->decay = SavedVariable(decay, false);
     n->initial = SavedVariable(h, false);
     n->offsets = SavedVariable(or_undefined(offsets), false);
-    n->ckpt = *ckpt;
+    n->ckpt = SavedVariable(*ckpt, false);
     n->scale = scale;
     torch::autograd::set_history(y, n);
     if (want_state) torch::autograd::set_history(*state, n);
@@ -835,16 +841,13 @@ py::object recurrence_autograd(const at::Tensor &input, const at::Tensor &u, con
 }
 
 struct LayerNormNode : OnceNode {
-  SavedVariable input, weight;
-  at::Tensor stats;
+  SavedVariable input, weight, stats;
   std::string name() const override { return "ChannelLayerNormBackward"; }
   void release_variables() override {
-    input.reset_data();
-    weight.reset_data();
-    stats.reset();
+    for (SavedVariable *s : {&input, &weight, &stats}) s->reset_data();
   }
   void backward(const variable_list &grads, variable_list &out) override {
-    auto [dx, dw, db] = layer_norm_backward(saved(input), saved_or_none(weight), stats, grads[0],
+    auto [dx, dw, db] = layer_norm_backward(saved(input), saved_or_none(weight), saved(stats), grads[0],
                                             task_should_compute_output(1), task_should_compute_output(2));
     out[0] = dx;
     out[1] = or_undefined(dw);
@@ -866,7 +869,7 @@ at::Tensor layer_norm_autograd(const at::Tensor &input, const OptTensor &weight,
     auto n = new_node<LayerNormNode>(input, w, b);
     n->input = SavedVariable(input, false);
     n->weight = SavedVariable(w, false);
-    n->stats = *stats;
+    n->stats = SavedVariable(*stats, false);
     torch::autograd::set_history(y, n);
   }
   return y;

@@ -67,6 +67,13 @@ def _check_operand(fn, name, t, shape, dtype, input):
         raise RuntimeError(f"dwconv_b200.{fn}: {name} must be {tuple(shape)}, got {tuple(t.shape)}")
 
 
+def _check_kept(fn, name, t, shape, input):
+    # what the forward call left, and hooks on saved tensors may have had in hand since
+    _check_operand(fn, name, t, shape, torch.float32, input)
+    if not t.is_contiguous():
+        raise RuntimeError(f"dwconv_b200.{fn}: {name} must be contiguous")
+
+
 def _check_sequences(fn, input, offsets):
     _C._check_cuda(input, "input")
     _sequence_dtype(input)
@@ -263,6 +270,7 @@ def _recurrence_backward(input, u, v, decay, initial, offsets, scale, ckpt, grad
         if want_initial:
             dinit = _state_or_zeros(grad_state, state_shape, torch.float32, input.device)
         return dx, du, dv, torch.zeros(decay.shape, **wide), dinit
+    _check_kept(fn, "checkpoints", ckpt, (int(_lib.lib.dwconv_b200_recurrence_checkpoint_bytes(s)) // 4,), input)
     dd = torch.empty(decay.shape, **wide)
     if want_initial:
         dinit = torch.empty(state_shape, **wide)
@@ -360,6 +368,7 @@ def _layer_norm_backward(input, weight, stats, grad, want_weight, want_bias):
     if rows == 0:
         return (dx, torch.zeros(C, **like) if want_weight else None,
                 torch.zeros(C, **like) if want_bias else None)
+    _check_kept(fn, "stats", stats, (rows, 2), input)
     dw = torch.empty(C, **like) if want_weight else None
     db = torch.empty(C, **like) if want_bias else None
     x, g, w = _norm_rows(input), _norm_rows(grad), _contiguous(weight)

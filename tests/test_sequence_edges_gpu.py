@@ -102,3 +102,54 @@ def test_a_penalty_on_gradients_is_refused_whatever_came_in():
         for t, a in zip(leaves, first):
             assert torch.equal(t.grad, a), name
             t.grad = None
+
+
+def test_saved_tensor_hooks_see_all_that_is_kept():
+    """Offloading moves all that a graph keeps to the host, what the kernels leave for their backward passes
+    included, and brings the same gradients back."""
+    kept = {}
+    for name, call, leaves in calls():
+        want = torch.autograd.grad(call().sum(), leaves)
+        sizes = []
+
+        def pack(t):
+            sizes.append((tuple(t.shape), t.dtype))
+            return t.cpu()
+
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t.cuda()):
+            y = call()
+        for a, b in zip(torch.autograd.grad(y.sum(), leaves), want):
+            assert torch.equal(a, b), name
+        kept[name] = sorted(map(str, sizes))
+    for name in ("conv", "recurrence", "norm"):
+        assert kept[name] == kept[name + " interpreted"], name
+    assert len(kept["recurrence"]) == 5 and len(kept["norm"]) == 3
+
+
+def test_checkpointed_operators_give_the_same_gradients():
+    from torch.utils.checkpoint import checkpoint
+    for name, call, leaves in calls():
+        want = torch.autograd.grad(call().sum(), leaves)
+        got = torch.autograd.grad(checkpoint(call, use_reentrant=False).sum(), leaves)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), name
+
+
+def test_what_a_hook_hands_back_is_checked():
+    for name, call, leaves in calls():
+        if name.startswith("conv"):
+            continue
+        # the last of the saved tensors is the kernel's own
+        for spoil, text in ((lambda t: t.cpu(), "must be float on"), (lambda t: t.half(), "must be float on"),
+                            (lambda t: t[:-1], r"must be \(.*got"),
+                            (lambda t: t.repeat_interleave(2, -1)[..., ::2], "must be contiguous")):
+            own = {"recurrence": 1, "norm": 2}[name.split()[0]]   # its rank, which no other fp32 one of its size has
+
+            def unpack(t):
+                mine = t.dtype == torch.float32 and t.dim() == own and t.shape != leaves[-1].shape
+                return spoil(t) if mine else t
+
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+                y = call()
+            with pytest.raises(RuntimeError, match=text):
+                torch.autograd.grad(y.sum(), leaves)
