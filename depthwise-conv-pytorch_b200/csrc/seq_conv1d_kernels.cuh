@@ -334,6 +334,18 @@ conv1d_backward_kernel(SeqIn<T> x, const T *__restrict__ w, const T *__restrict_
         for (int k = 1; k < K; ++k) o[h] = fma2(taps.w[k][h], dpw[ring<K>(at, K - 1 - k)][h], o[h]);
       }
     };
+    // the same outside the chunks, where rows of the window may lie outside the sequence: taps lo .. hi
+    // alone (a tap times a zero is no zero where the tap is not finite)
+    auto border_gradient = [&](int lo, int hi, float2 (&o)[H]) {
+#pragma unroll
+      for (int h = 0; h < H; ++h) o[h] = f2(0.f);
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (k >= lo && k <= hi) {
+#pragma unroll
+          for (int h = 0; h < H; ++h) o[h] = fma2(taps.w[k][h], dpw[K - 1 - k][h], o[h]);
+        }
+    };
     // a row's gradient to where it belongs: dx, or the initial rows of a sequence that starts here
     auto emit = [&](int row, const float2 (&o)[H]) {
       if (row >= sp.begin) {
@@ -370,9 +382,7 @@ conv1d_backward_kernel(SeqIn<T> x, const T *__restrict__ w, const T *__restrict_
 #pragma unroll
         for (int f = 0; f < K - 1; ++f) {
           float2 o[H];
-#pragma unroll
-          for (int h = 0; h < H; ++h) dpw[K - 1][h] = f2(0.f);
-          gradient(0, o);
+          border_gradient(f + 1, sp.seq >= 0 ? t + f - sp.begin : -1, o);
           if (dfin != nullptr && sp.seq >= 0) {
             float2 d[H];
             ln.get(ln.load(dfin + ((long long)sp.seq * (K - 1) + f) * C), d);
@@ -435,7 +445,7 @@ conv1d_backward_kernel(SeqIn<T> x, const T *__restrict__ w, const T *__restrict_
           count(0);
         }
         float2 o[H];
-        gradient(0, o);
+        border_gradient(0, sp.seq >= 0 ? t - sp.begin : -1, o);
         emit(lead, o);
         shift(win);
         shift(dpw);

@@ -153,3 +153,30 @@ def test_what_a_hook_hands_back_is_checked():
                 y = call()
             with pytest.raises(RuntimeError, match=text):
                 torch.autograd.grad(y.sum(), leaves)
+
+
+# ---- non-finite parameters ----------------------------------------------------------------------
+
+@by_dtype
+@pytest.mark.parametrize("value", [float("inf"), float("nan")], ids=str)
+@pytest.mark.parametrize("C", [12, 7])
+@pytest.mark.parametrize("K", [1, 2, 4, 7])
+def test_conv_taps_reach_only_rows_of_the_sequence(K, C, value, dtype):
+    """A tap that is not finite shows in the gradients of the rows that it multiplies and in no other: not behind the
+    last sequence, nor where the sequence ends before its product, nor in initial rows it does not reach."""
+    import dwconv_b200 as d
+    offsets, T, on_gpu = packed([40, 3, 0, 1, 70], 6)
+    n = 5
+    for tap in range(K):
+        x, dy, w, b, init, dstate = conv_inputs(1, T, C, K, n, dtype, 62, True, True)
+        with torch.no_grad():
+            w[::2, 0, tap] = value
+        y, state = d.depthwise_conv1d_causal(x, w, b, None, init, on_gpu, return_state=True)
+        leaves = [x, b] + ([init] if K > 1 else [])
+        got = torch.autograd.grad([y, state], leaves, [dy, dstate])
+        want, _ = ref.conv(x, w, b, None, init, offsets, dy, dstate)
+        assert not y[:, offsets[-1]:].any() and not got[0][:, offsets[-1]:].any()
+        for a, c in zip(got, (want["dx"], want["dbias"], want["dinitial"])):
+            a, c = ref.wide(a), c
+            assert torch.equal(a.isnan(), c.isnan()) and torch.equal(a == float("inf"), c == float("inf"))
+            assert torch.equal(a == float("-inf"), c == float("-inf"))
