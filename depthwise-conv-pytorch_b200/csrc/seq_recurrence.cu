@@ -812,12 +812,12 @@ __device__ __forceinline__ void backward_body(const RecMaps &maps, SeqIn<T> x, S
         h = f2(0.f);
         if ((mk.start >> j & 1u) && initial != nullptr)
           h = load_state(initial, seq_of(list, t0, j, mk.start, mk.start_seq), C, c);
-        if (mk.none >> j & 1u) g[j] = f2(0.f);
       }
-      const float2 ddx = mul2(g[j], mul2(beta, i[j]));
-      const float2 ddv = mul2(mul2(ddx, xv), one_minus2(i[j]));
-      const float2 dzz = mul2(mul2(g[j], a), fma2(mul2(a, rho), ix, mul2(s, h)));
-      const float2 ddu = mul2(dzz, one_minus2(r));
+      float2 ddx = mul2(g[j], mul2(beta, i[j]));
+      float2 ddv = mul2(mul2(ddx, xv), one_minus2(i[j]));
+      float2 dzz = mul2(mul2(g[j], a), fma2(mul2(a, rho), ix, mul2(s, h)));
+      float2 ddu = mul2(dzz, one_minus2(r));
+      if (PACKED && (mk.none >> j & 1u)) ddx = ddv = dzz = ddu = f2(0.f);  // whatever the channel's decay
       sum = add2(sum, dzz);
       h = fma2(a, h, mul2(beta, ix));
       if (j < rows) {

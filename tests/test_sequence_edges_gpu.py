@@ -180,3 +180,17 @@ def test_conv_taps_reach_only_rows_of_the_sequence(K, C, value, dtype):
             a, c = ref.wide(a), c
             assert torch.equal(a.isnan(), c.isnan()) and torch.equal(a == float("inf"), c == float("inf"))
             assert torch.equal(a == float("-inf"), c == float("-inf"))
+
+
+@by_dtype
+@pytest.mark.parametrize("value", [float("inf"), float("nan")], ids=str)
+@pytest.mark.parametrize("C", [10, 7])
+def test_recurrence_rows_of_no_sequence_are_zero_whatever_the_decay(C, value, dtype):
+    import dwconv_b200 as d
+    offsets, T, on_gpu = packed([40, 3, 0, 30], 70)
+    x, u, v, dy, decay, init, dstate = recurrence_inputs(1, T, C, 4, dtype, 63, True)
+    with torch.no_grad():
+        decay[::2] = value
+    y, state = d.gated_linear_recurrence(x, u, v, decay, init, on_gpu, return_state=True)
+    for t in (y, *torch.autograd.grad([y, state], [x, u, v], [dy, dstate])):
+        assert not t[:, offsets[-1]:].any()
