@@ -27,16 +27,20 @@ namespace {
 // ACT: the two activations that have kernels of their own, or ANY with the activation at run time.
 constexpr int ANY = -1;
 
+// A NaN stays one, and passes the gradient on.
+__device__ __forceinline__ float activate(float p, int act) {
+  return act == DWCONV_B200_ACT_RELU ? (p <= 0.f ? 0.f : p) : apply_activation<float>(p, act);
+}
 template <int ACT> __device__ __forceinline__ float2 act2(float2 p, int act) {
   if constexpr (ACT == DWCONV_B200_ACT_NONE) return p;
   if constexpr (ACT == DWCONV_B200_ACT_SILU) return mul2(p, sigmoid2(p));
-  return make_float2(apply_activation<float>(p.x, act), apply_activation<float>(p.y, act));
+  return make_float2(activate(p.x, act), activate(p.y, act));
 }
 
 __device__ __forceinline__ float slope(float p, int act) {
   switch (act) {
-    case DWCONV_B200_ACT_RELU: return p > 0.f ? 1.f : 0.f;
-    case DWCONV_B200_ACT_RELU6: return p > 0.f && p < 6.f ? 1.f : 0.f;
+    case DWCONV_B200_ACT_RELU: return p <= 0.f ? 0.f : 1.f;
+    case DWCONV_B200_ACT_RELU6: return p <= 0.f || p >= 6.f ? 0.f : 1.f;
     case DWCONV_B200_ACT_HARDSWISH: return p <= -3.f ? 0.f : (p >= 3.f ? 1.f : (2.f * p + 3.f) / 6.f);
     default: return 1.f;
   }

@@ -194,3 +194,32 @@ def test_recurrence_rows_of_no_sequence_are_zero_whatever_the_decay(C, value, dt
     y, state = d.gated_linear_recurrence(x, u, v, decay, init, on_gpu, return_state=True)
     for t in (y, *torch.autograd.grad([y, state], [x, u, v], [dy, dstate])):
         assert not t[:, offsets[-1]:].any()
+
+
+@by_dtype
+@pytest.mark.parametrize("C", [8, 5])
+@pytest.mark.parametrize("act", ["relu", "relu6", "silu", "hardswish"])
+def test_a_nan_passes_every_activation(act, C, dtype):
+    """Row 3 of one channel is NaN: so are the outputs of the taps that reach it and no others, forward and in the
+    one-row step, and the gradients of the filter; dx gets the slope that torch gives a NaN, or a NaN."""
+    import dwconv_b200 as d
+    x, dy, w, b, _, _ = conv_inputs(2, 20, C, 4, 2, dtype, 64, False, True)
+    with torch.no_grad():
+        x[0, 3, 1] = float("nan")
+    y = d.depthwise_conv1d_causal(x, w, b, act)
+    bad = torch.zeros_like(y, dtype=torch.bool)
+    bad[0, 3:7, 1] = True
+    assert torch.equal(y.isnan(), bad)
+    dx, dw, db = torch.autograd.grad(y, [x, w, b], dy)
+    keep = [c for c in range(C) if c != 1]
+    assert dw[1].isnan().all() and not dw[keep].isnan().any() and not dx[..., keep].isnan().any()
+    assert not dx[0, 7:].isnan().any() and not dx[1].isnan().any()
+    if act in ("relu", "relu6"):
+        # rows 3 to 6 pass dy on: dx[3] takes all of them and is finite, and not zero
+        want = (w[1, 0].float().flip(0) * dy[0, 3:7, 1].float()).sum()
+        assert abs(dx[0, 3, 1].float() - want) <= 4 * 2 ** -8 * (w[1, 0].float().flip(0) * dy[0, 3:7, 1].float()).abs().sum()
+    with torch.no_grad():
+        step = d.depthwise_conv1d_causal_step(x[:, 3], w, torch.zeros(2, 3, C, device="cuda", dtype=dtype), b, act)
+    only = torch.zeros_like(step, dtype=torch.bool)
+    only[0, 1] = True
+    assert torch.equal(step.isnan(), only)
