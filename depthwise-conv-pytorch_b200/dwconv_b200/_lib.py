@@ -202,7 +202,8 @@ def check_device_status(what):
 
 
 # DWCONV_B200_CHECK_STATUS=1: the autograd function synchronises and checks the device flags
-# after every backward (debugging aid: costs a device synchronisation per call).
+# after every backward, and after every call of the sequence operators (debugging aid: costs a device
+# synchronisation per call).
 CHECK_STATUS = os.environ.get("DWCONV_B200_CHECK_STATUS", "0") not in ("", "0")
 
 

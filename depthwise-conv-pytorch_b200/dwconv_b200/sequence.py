@@ -405,13 +405,13 @@ _forms = _Forms(_native)
 
 # ---- autograd ----------------------------------------------------------------------------------
 # The compiled module has nodes of its own (no interpreter in the backward pass); these functions are
-# what runs without it, and where the device flags are checked after every call.
+# what runs without it, and where the device flags are checked after every call (that is not captured).
 
 _nodes = _native if not _lib.CHECK_STATUS else None
 
 
 def _check_flags(what):
-    if _lib.CHECK_STATUS:
+    if _lib.CHECK_STATUS and not torch.cuda.is_current_stream_capturing():
         _lib.check_device_status(what)
 
 
@@ -452,6 +452,7 @@ class CausalConv1dFunction(Function):
     @staticmethod
     def forward(ctx, input, weight, bias, initial, offsets, act, want_state):
         y, state = _forms.conv1d_causal(input, weight, bias, act, initial, offsets, want_state)
+        _check_flags("depthwise_conv1d_causal")
         ctx.save_for_backward(input, weight, bias, initial, offsets)
         ctx.act, ctx.want_state = act, want_state
         ctx.set_materialize_grads(False)
@@ -474,6 +475,7 @@ class GatedLinearRecurrenceFunction(Function):
     def forward(ctx, input, recurrence_gate, input_gate, decay, initial, offsets, scale, want_state):
         y, state, ckpt = _forms.recurrence(input, recurrence_gate, input_gate, decay, initial, offsets,
                                            scale, want_state, True)
+        _check_flags("gated_linear_recurrence")
         ctx.save_for_backward(input, recurrence_gate, input_gate, decay, initial, offsets, ckpt)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
@@ -496,6 +498,7 @@ class LayerNormFunction(Function):
     @staticmethod
     def forward(ctx, input, weight, bias, eps):
         y, stats = _forms.layer_norm(input, weight, bias, eps, True)
+        _check_flags("layer_norm")
         ctx.save_for_backward(input, weight, stats)
         return y
 
@@ -532,6 +535,7 @@ def depthwise_conv1d_causal(input, weight, bias=None, activation=None, initial_s
     if _wants_grad(input, weight, bias, initial_state):
         return CausalConv1dFunction.apply(input, weight, bias, initial_state, offsets, act, bool(return_state))
     y, state = _forms.conv1d_causal(input, weight, bias, act, initial_state, offsets, bool(return_state))
+    _check_flags("depthwise_conv1d_causal")
     return (y, state) if return_state else y
 
 
@@ -546,7 +550,9 @@ def depthwise_conv1d_causal_step(input, weight, state, bias=None, activation=Non
     if _wants_grad(input, weight, state, bias):
         raise RuntimeError("dwconv_b200.depthwise_conv1d_causal_step: the state is updated in place and "
                            "has no gradient; use depthwise_conv1d_causal or torch.no_grad()")
-    return _forms.conv1d_causal_step(input, weight, state, bias, act)
+    y = _forms.conv1d_causal_step(input, weight, state, bias, act)
+    _check_flags("depthwise_conv1d_causal_step")
+    return y
 
 
 def gated_linear_recurrence(input, recurrence_gate, input_gate, decay, initial_state=None, offsets=None,
@@ -574,6 +580,7 @@ def gated_linear_recurrence(input, recurrence_gate, input_gate, decay, initial_s
                                                    offsets, scale, bool(return_state))
     y, state, _ = _forms.recurrence(input, recurrence_gate, input_gate, decay, initial_state, offsets, scale,
                                     bool(return_state), False)
+    _check_flags("gated_linear_recurrence")
     return (y, state) if return_state else y
 
 
@@ -586,7 +593,9 @@ def gated_linear_recurrence_step(input, recurrence_gate, input_gate, decay, stat
     if _wants_grad(input, recurrence_gate, input_gate, decay, state):
         raise RuntimeError("dwconv_b200.gated_linear_recurrence_step: the state is updated in place and "
                            "has no gradient; use gated_linear_recurrence or torch.no_grad()")
-    return _forms.recurrence_step(input, recurrence_gate, input_gate, decay, state, float(scale))
+    y = _forms.recurrence_step(input, recurrence_gate, input_gate, decay, state, float(scale))
+    _check_flags("gated_linear_recurrence_step")
+    return y
 
 
 def layer_norm(input, weight=None, bias=None, eps=1e-5):
@@ -602,7 +611,9 @@ def layer_norm(input, weight=None, bias=None, eps=1e-5):
     _refuse_tangents("layer_norm", input, weight, bias)
     if _wants_grad(input, weight, bias):
         return LayerNormFunction.apply(input, weight, bias, eps)
-    return _forms.layer_norm(input, weight, bias, eps, False)[0]
+    y = _forms.layer_norm(input, weight, bias, eps, False)[0]
+    _check_flags("layer_norm")
+    return y
 
 
 # ---- modules -----------------------------------------------------------------------------------

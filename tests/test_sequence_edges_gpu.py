@@ -64,6 +64,32 @@ def test_a_wait_that_runs_out_is_reported_and_ends(size, lengths, dtype, expire)
         assert _lib.device_status() == 0
 
 
+def test_checked_calls_report_a_wait_that_ran_out(expire, monkeypatch):
+    """With the status checks on, every call says so itself: with a graph, without one, and backward."""
+    import dwconv_b200 as d
+    from dwconv_b200 import sequence as S
+    monkeypatch.setattr(S._lib, "CHECK_STATUS", True)
+    monkeypatch.setattr(S, "_nodes", None)
+    x, u, v, dy, decay, _, _ = recurrence_inputs(1, 2000, 64, 1, torch.float32, 65, False)
+    y = d.gated_linear_recurrence(x, u, v, decay)
+    gone = pytest.raises(RuntimeError, match="a kernel's bounded wait expired .*sequence operators")
+    expire(1)
+    with gone:
+        d.gated_linear_recurrence(x, u, v, decay)
+    with gone, torch.no_grad():
+        d.gated_linear_recurrence(x, u, v, decay)
+    with gone:
+        torch.autograd.grad(y, x, dy)
+    expire(0)
+    for name, call, leaves in calls():
+        torch.autograd.grad(call().sum(), leaves)
+    gr = torch.cuda.CUDAGraph()     # a captured call cannot be checked, and is not
+    with torch.no_grad(), torch.cuda.graph(gr):
+        z = d.gated_linear_recurrence(x, u, v, decay)
+    gr.replay()
+    assert torch.equal(z, y)
+
+
 # ---- autograd ----------------------------------------------------------------------------------
 
 def calls(dtype=torch.float32, B=2, T=20, C=10):
