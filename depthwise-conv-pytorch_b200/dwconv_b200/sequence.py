@@ -617,6 +617,13 @@ def layer_norm(input, weight=None, bias=None, eps=1e-5):
 
 
 # ---- modules -----------------------------------------------------------------------------------
+# The functions take filter, bias and norm weights in the input's type.  Under torch.autocast, where activations
+# come in 16 bits and parameters stay in fp32, the modules convert, each as torch converts for the layer whose
+# state_dict it shares: the convolution runs in the activations' type, the norm in the parameters'.
+
+def _mixed(input, parameter):
+    return input.dtype != parameter.dtype and torch.is_autocast_enabled("cuda")
+
 
 class CausalDepthwiseConv1d(nn.Module):
     """Module form of ``depthwise_conv1d_causal``; ``state_dict`` interchangeable with
@@ -631,12 +638,19 @@ class CausalDepthwiseConv1d(nn.Module):
         self.weight = nn.Parameter(torch.randn(channels, 1, kernel_size) / kernel_size ** 0.5)
         self.bias = nn.Parameter(torch.zeros(channels)) if bias else None
 
+    def _filter(self, input):
+        w, b = self.weight, self.bias
+        if _mixed(input, w):    # rounded to the activations' type, and so are their gradients
+            w, b = w.to(input.dtype), b.to(input.dtype) if b is not None else None
+        return w, b
+
     def forward(self, input, initial_state=None, offsets=None, return_state=False):
-        return depthwise_conv1d_causal(input, self.weight, self.bias, self.activation, initial_state,
-                                       offsets, return_state)
+        w, b = self._filter(input)
+        return depthwise_conv1d_causal(input, w, b, self.activation, initial_state, offsets, return_state)
 
     def step(self, input, state):
-        return depthwise_conv1d_causal_step(input, self.weight, state, self.bias, self.activation)
+        w, b = self._filter(input)
+        return depthwise_conv1d_causal_step(input, w, state, b, self.activation)
 
 
 class GatedLinearRecurrence(nn.Module):
@@ -679,6 +693,8 @@ class LayerNorm(nn.Module):
         self.bias = nn.Parameter(torch.zeros(channels)) if bias else None
 
     def forward(self, input):
+        if _mixed(input, self.weight):
+            input = input.to(self.weight.dtype)
         return layer_norm(input, self.weight, self.bias, self.eps)
 
 
@@ -704,8 +720,12 @@ class RecurrentMixer(nn.Module):
         self.project_out = nn.Linear(width, channels)
 
     def initial_state(self, count, dtype=None, device=None):
+        """Zeros for ``count`` sequences; ``dtype``: of the convolution's rows, the type that ``project_in`` gives
+        (under autocast that of autocast)."""
         w = self.conv.weight
-        dtype, device = dtype or w.dtype, device or w.device
+        if dtype is None:
+            dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else w.dtype
+        device = device or w.device
         return (torch.zeros(count, self.taps - 1, self.width, dtype=dtype, device=device),
                 torch.zeros(count, self.width, dtype=torch.float32, device=device))
 

@@ -249,3 +249,49 @@ def test_a_nan_passes_every_activation(act, C, dtype):
     only = torch.zeros_like(step, dtype=torch.bool)
     only[0, 1] = True
     assert torch.equal(step.isnan(), only)
+
+
+# ---- mixed precision ------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("rows", ["fp32", "16 bits"])
+def test_the_mixer_trains_and_serves_under_autocast(rows, dtype):
+    """fp32 parameters, 16-bit activations: the same bits as the functions on parameters converted by hand."""
+    import dwconv_b200 as d
+    F = torch.nn.functional
+    torch.manual_seed(66)
+    m = d.RecurrentMixer(48, width=64).cuda()
+    x = torch.randn(2, 40, 48, device="cuda", dtype=torch.float32 if rows == "fp32" else dtype, requires_grad=True)
+    dy = torch.randn(2, 40, 48, device="cuda")
+    leaves = [x, *m.parameters()]
+
+    def by_hand():
+        def linear(t, layer):
+            return F.linear(t.to(dtype), layer.weight.to(dtype), layer.bias.to(dtype))
+        gate, z = linear(d.layer_norm(x.float(), m.norm.weight, m.norm.bias, m.norm.eps), m.project_in).chunk(2, -1)
+        z = d.depthwise_conv1d_causal(z, m.conv.weight.to(dtype), m.conv.bias.to(dtype))
+        u, v = linear(z, m.project_gates).chunk(2, -1)
+        h = d.gated_linear_recurrence(z, u, v, m.recurrence.decay, scale=m.recurrence.scale)
+        return x + linear(h * F.gelu(gate), m.project_out)
+
+    want = by_hand()
+    want_grads = torch.autograd.grad(want, leaves, dy.to(want.dtype))
+    with torch.autocast("cuda", dtype=dtype):
+        got, state = m(x)
+        assert torch.equal(got, want) and state[0].dtype == dtype and state[1].dtype == torch.float32
+        for (name, p), a, b in zip([("x", x), *m.named_parameters()],
+                                   torch.autograd.grad(got, leaves, dy.to(got.dtype)), want_grads):
+            assert a.dtype == p.dtype and torch.equal(a, b), name
+    with torch.no_grad(), torch.autocast("cuda", dtype=dtype):
+        step_state = m.initial_state(2)
+        assert step_state[0].dtype == dtype
+        for t in range(40):
+            m.step(x[:, t], step_state)
+        # the last rows that the convolution keeps: sums of 48 products in another order, each rounded once to 16
+        # bits, at most a step apart (2^-7 in bf16); twice that
+        assert torch.allclose(step_state[0].float(), state[0].float(), rtol=2 ** -6, atol=2 ** -6)
+    # without autocast the types have to agree, as they have to in torch's own layers
+    with pytest.raises(RuntimeError, match="weight must be float|weight must be c10::"):
+        m.conv(torch.zeros(1, 4, 64, device="cuda", dtype=dtype))
+    with pytest.raises(RuntimeError, match="weight must be c10::"):
+        m.norm(torch.zeros(1, 4, 48, device="cuda", dtype=dtype))
