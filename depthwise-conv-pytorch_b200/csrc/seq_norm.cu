@@ -368,13 +368,16 @@ inline int pow2_at_least(int v) {
 // 143; 131072 of 1536, 143 and 190; 200704 of 96, 22 and 25.  6 vectors are for rows that 3 do not hold (of 96:
 // 24) and for more than a few per warp (8192 rows of 1536: 20 and 18).  4 vectors against 2 made no
 // difference on rows of 64 to 1024 and are not in the choice.
+//
+// In 16 bits vectors of 4 are chosen by threes alone (a vector of 8 takes the place of two), and rows span warps
+// only where threads hold the most that they may: nothing else is compiled (norm_spans_warps).
 inline NormShape norm_shape(int C, int es, int most, long long rows) {
   static const NormShape choices[] = {{8, 1, 0}, {8, 2, 0}, {8, 3, 0}, {8, 6, 0}, {4, 1, 0}, {4, 2, 0},
                                       {4, 3, 0}, {4, 4, 0}, {1, 1, 0}, {1, 2, 0}, {1, 4, 0}, {1, 8, 0}};
   NormShape best{1, 0, 0};
   long long cost = 0;
   for (const NormShape &n : choices) {
-    if (n.V * n.NV > most || (n.NV == 6 && rows < 16384)) continue;
+    if (n.V * n.NV > most || (n.NV == 6 && rows < 16384) || (n.V == 4 && n.NV != 3 && es == 2)) continue;
     if (n.V != 1 ? (es == 0 || n.V * es > 16 || C % n.V != 0) : es != 0) continue;
     const int tpr = pow2_at_least(ceil_div(C / n.V, n.NV));
     if (tpr > (n.V * n.NV > NORM_MOST ? 32 : NORM_CTA) || (n.NV == 6 && tpr < 32)) continue;
@@ -387,6 +390,10 @@ inline NormShape norm_shape(int C, int es, int most, long long rows) {
   return best;
 }
 
+template <typename T, int V, int NV> constexpr bool norm_spans_warps() {
+  return V * NV == (V == 1 ? 8 : NORM_MOST) || (V == 4 && NV == 3);
+}
+
 // CTAs: enough to fill every SM, each staying for many rows.
 inline int norm_grid(long long rows, int slots, int per_sm) {
   const long long g = ceil_div_ll(rows, slots), most = 148ll * per_sm;
@@ -396,10 +403,13 @@ constexpr int NORM_PARTS = 148 * 4;  // most CTAs of the backward kernels, one p
 
 template <typename T, int V, int NV>
 void launch_forward(const T *x, const T *w, const T *b, T *y, float2 *stats, const NormParams &p, cudaStream_t st) {
-  if (p.tpr > 32)
-    norm_forward_kernel<T, V, NV, true>
-        <<<norm_grid(p.rows, NORM_CTA / p.tpr, 2), NORM_CTA, 0, st>>>(x, w, b, y, stats, p);
-  else
+  if constexpr (norm_spans_warps<T, V, NV>())
+    if (p.tpr > 32) {
+      norm_forward_kernel<T, V, NV, true>
+          <<<norm_grid(p.rows, NORM_CTA / p.tpr, 2), NORM_CTA, 0, st>>>(x, w, b, y, stats, p);
+      return;
+    }
+  if constexpr (V != 4 || sizeof(T) == 4)  // in 16 bits rows that vectors of 8 hold better
     norm_forward_kernel<T, V, NV, false>
         <<<norm_grid(p.rows, NORM_ROW_THREADS / p.tpr, 12), NORM_ROW_THREADS, 0, st>>>(x, w, b, y, stats, p);
 }
@@ -408,15 +418,17 @@ template <typename T, int V, int NV>
 int launch_backward(const T *x, const T *w, const float2 *stats, const T *dy, T *dx, float *part,
                     const NormParams &p, cudaStream_t st) {
   const size_t smem = part ? 2 * NV * p.tpr * V * sizeof(float) : 0;
-  const int grid = p.tpr > 32 ? norm_grid(p.rows, NORM_CTA / p.tpr, 1) : norm_grid(p.rows, NORM_ROW_THREADS / p.tpr, 4);
-  if (p.tpr > 32) {
-    if (smem > 40 * 1024)
-      (void)cudaFuncSetAttribute(norm_backward_kernel<T, V, NV, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 2 * NV * NORM_CTA * V * (int)sizeof(float));
-    norm_backward_kernel<T, V, NV, true><<<grid, NORM_CTA, smem, st>>>(x, w, stats, dy, dx, part, p);
-  } else {
-    norm_backward_kernel<T, V, NV, false><<<grid, NORM_ROW_THREADS, smem, st>>>(x, w, stats, dy, dx, part, p);
-  }
+  if constexpr (norm_spans_warps<T, V, NV>())
+    if (p.tpr > 32) {
+      const int grid = norm_grid(p.rows, NORM_CTA / p.tpr, 1);
+      if (smem > 40 * 1024)
+        (void)cudaFuncSetAttribute(norm_backward_kernel<T, V, NV, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   2 * NV * NORM_CTA * V * (int)sizeof(float));
+      norm_backward_kernel<T, V, NV, true><<<grid, NORM_CTA, smem, st>>>(x, w, stats, dy, dx, part, p);
+      return grid;
+    }
+  const int grid = norm_grid(p.rows, NORM_ROW_THREADS / p.tpr, 4);
+  norm_backward_kernel<T, V, NV, false><<<grid, NORM_ROW_THREADS, smem, st>>>(x, w, stats, dy, dx, part, p);
   return grid;
 }
 
@@ -427,13 +439,15 @@ int launch_backward(const T *x, const T *w, const float2 *stats, const T *dy, T 
     case 102: FN<T, 1, 2>(__VA_ARGS__); break;              \
     case 104: FN<T, 1, 4>(__VA_ARGS__); break;              \
     case 108: FN<T, 1, 8>(__VA_ARGS__); break;              \
-    case 401: FN<T, 4, 1>(__VA_ARGS__); break;              \
-    case 402: FN<T, 4, 2>(__VA_ARGS__); break;              \
-    case 403: FN<T, 4, 3>(__VA_ARGS__); break;              \
-    case 404: FN<T, 4, 4>(__VA_ARGS__); break;              \
     default:                                                \
-      if constexpr (sizeof(T) == 2) {                       \
-        if (sh.NV == 1) FN<T, 8, 1>(__VA_ARGS__);           \
+      if constexpr (sizeof(T) == 4) {                       \
+        if (sh.NV == 1) FN<T, 4, 1>(__VA_ARGS__);           \
+        else if (sh.NV == 2) FN<T, 4, 2>(__VA_ARGS__);      \
+        else if (sh.NV == 3) FN<T, 4, 3>(__VA_ARGS__);      \
+        else FN<T, 4, 4>(__VA_ARGS__);                      \
+      } else {                                              \
+        if (sh.V == 4) FN<T, 4, 3>(__VA_ARGS__);            \
+        else if (sh.NV == 1) FN<T, 8, 1>(__VA_ARGS__);      \
         else FN<T, 8, 2>(__VA_ARGS__);                      \
       }                                                     \
   }

@@ -295,3 +295,26 @@ def test_the_mixer_trains_and_serves_under_autocast(rows, dtype):
         m.conv(torch.zeros(1, 4, 64, device="cuda", dtype=dtype))
     with pytest.raises(RuntimeError, match="weight must be c10::"):
         m.norm(torch.zeros(1, 4, 48, device="cuda", dtype=dtype))
+
+
+# ---- layer norm: every way a row is held -----------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("aligned", [True, False], ids=["aligned", "unaligned"])
+def test_norm_of_every_width(aligned, dtype):
+    """All widths up to 700 and some of each kind above, three rows each: whatever vectors, threads and warps hold
+    a row, forward and backward."""
+    import dwconv_b200 as d
+    g = torch.Generator().manual_seed(67)
+    widths = list(range(1, 701)) + list(range(704, 1600, 8)) + list(range(1600, 8193, 412)) + [4095, 4097, 8191, 8193]
+    full = torch.randn(3, 8200, generator=g) * 2 + 0.5
+    x, dy = full.to(dtype).cuda(), torch.randn(3, 8200, generator=g).to(dtype).cuda()
+    w, b = (1 + 0.3 * torch.randn(8200, generator=g)).to(dtype).cuda(), torch.randn(8200, generator=g).to(dtype).cuda()
+    for C in widths:
+        leaf = (x[:, :C].contiguous() if aligned else x[:, 1:1 + C]).detach().requires_grad_()
+        wt, bt = w[:C].contiguous(), b[:C].contiguous()
+        y = d.layer_norm(leaf, wt, bt)
+        dx, = torch.autograd.grad(y, leaf, dy[:, :C])
+        want, tol = ref.norm(leaf, wt, bt, 1e-5, dy[:, :C])
+        ref.check(y, want["y"], tol["y"], dtype, f"y of {C}")
+        ref.check(dx, want["dx"], tol["dx"], dtype, f"dx of {C}")
