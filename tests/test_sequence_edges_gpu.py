@@ -318,3 +318,76 @@ def test_norm_of_every_width(aligned, dtype):
         want, tol = ref.norm(leaf, wt, bt, 1e-5, dy[:, :C])
         ref.check(y, want["y"], tol["y"], dtype, f"y of {C}")
         ref.check(dx, want["dx"], tol["dx"], dtype, f"dx of {C}")
+
+
+# ---- long runs and many rows ---------------------------------------------------------------------
+
+LONG = {
+    # batch and rows that warps walk in runs of 32 to 128, several times what is copied ahead
+    "dense": ((4, 4096, 1024), None),
+    "odd width": ((2, 4096, 1281), None),
+    # borders inside the runs, at their ends, next to one another, and rows behind the last sequence
+    "packed": ((1, 16387, 1024), [5000, 1, 0, 43, 2, 3, 1000, 4096, 47, 48, 6140]),
+    "packed, odd width": ((1, 8191, 1281), [2000, 3, 0, 4500, 1, 1680]),
+}
+
+
+@by_dtype
+@pytest.mark.parametrize("K, act", [(1, "silu"), (2, "silu"), (3, None), (4, "silu"), (4, "hardswish"), (5, None),
+                                    (7, "silu"), (8, "silu")], ids=str)
+@pytest.mark.parametrize("problem", list(LONG))
+def test_conv_in_long_runs(problem, K, act, dtype):
+    """Problems large enough that a warp's run fills its copies ahead many times over; channels at the borders of
+    lanes, warps and the tensor against the definition."""
+    import dwconv_b200 as d
+    (B, T, C), lengths = LONG[problem]
+    offsets = on_gpu = None
+    n = B
+    if lengths is not None:
+        offsets, _, on_gpu = packed(lengths)
+        n = len(lengths)
+        assert offsets[-1] <= T
+    x, dy, w, b, init, dstate = conv_inputs(B, T, C, K, n, dtype, 70 + K, True, True)
+    y, state = d.depthwise_conv1d_causal(x, w, b, act, init, on_gpu, return_state=True)
+    leaves = {"dx": x, "dweight": w, "dbias": b, "dinitial": init}
+    grads = dict(zip(leaves, torch.autograd.grad([y, state], list(leaves.values()), [dy, dstate])))
+    at = [0, 1, 2, 3, 63, 64, 66, 127, 128, C // 2 + 1, C - 5, C - 2, C - 1]
+    if act == "hardswish":
+        # away from its kinks, where fp32 and 64 bits may take different sides
+        p = ref.conv(x[..., at], w[at], b[at], None, init[..., at], offsets)[0]["y"]
+        dy = dy.clone()
+        dy[..., at] = torch.where(((p.abs() - 3).abs() < 1e-3).cuda(), torch.zeros_like(dy[..., at]), dy[..., at])
+        y, state = d.depthwise_conv1d_causal(x, w, b, act, init, on_gpu, return_state=True)
+        grads = dict(zip(leaves, torch.autograd.grad([y, state], list(leaves.values()), [dy, dstate])))
+    want, tol = ref.conv(x[..., at], w[at], b[at], act, init[..., at], offsets, dy[..., at], dstate[..., at])
+    # a run of 128 rows, 8 warps and 16 parts: 152 sums, of which the tolerance counts 144; times 1.25
+    for name in ("dweight", "dbias"):
+        tol[name] = 1.25 * tol[name]
+    ref.check(y[..., at], want["y"], tol["y"], dtype, "y")
+    ref.check(state[..., at], want["state"], tol["state"], dtype, "state")
+    for name, got in grads.items():
+        got = got[at] if name in ("dweight", "dbias") else got[..., at]
+        ref.check(got, want[name], tol[name], dtype, name)
+
+
+@by_dtype
+@pytest.mark.parametrize("size", [(4800, 4096), (4800, 2048), (4801, 1032), (200000, 96), (40001, 40), (4000, 1001),
+                                  (100003, 7), (700, 8200), (700, 5001), (299, 12288)], ids=lambda s: "x".join(map(str, s)))
+def test_norm_weight_gradients_over_many_rows(size, dtype, monkeypatch):
+    """Threads, warps and CTAs that take row after row, in every way that a row is held: what they add up over the
+    rows.  The definition on the device."""
+    import dwconv_b200 as d
+    monkeypatch.setattr(ref, "wide", lambda t: None if t is None else t.detach().double())
+    rows, C = size
+    g = torch.Generator().manual_seed(71)
+    x = (torch.randn(rows, C, generator=g) * 2 + 0.5).to(dtype).cuda().requires_grad_()
+    w = (1 + 0.3 * torch.randn(C, generator=g)).to(dtype).cuda().requires_grad_()
+    b = randn(g, C, dtype=dtype)
+    dy = randn(g, rows, C, dtype=dtype, grad=False)
+    got = torch.autograd.grad(d.layer_norm(x, w, b), [x, w, b], dy)
+    # the definition makes the bias zeros on the host where there is none; here it is there
+    want, tol = ref.norm(x, w, b, 1e-5, dy)
+    for name, a in zip(("dx", "dweight", "dbias"), got):
+        ref.check(a, want[name], tol[name], dtype, name)
+    for a, c in zip(torch.autograd.grad(d.layer_norm(x, w, b), [w, b], dy), got[1:]):
+        assert torch.equal(a, c)
