@@ -18,6 +18,7 @@
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
 #include <ATen/cuda/CUDAContext.h>
@@ -25,6 +26,7 @@
 
 #include <string>
 #include <tuple>
+#include <unordered_set>
 #include <vector>
 
 #include "dwconv_b200.h"
@@ -697,7 +699,8 @@ template <typename... T> void refuse_tangents(const char *fn, const T &...t) {
 struct OnceNode : torch::autograd::Node {
   // A leaf's gradient is accumulated on the stream that was current when a live graph first reached the
   // leaf.  Where that is the legacy default stream, which cannot take part in a capture, the engine would
-  // break the capture in the middle; refused here, before anything is recorded.
+  // break the capture in the middle; refused here, before anything is recorded.  Leaves behind views and conversions
+  // (parameters under autocast) count like those that the node reads itself.
   void check_capture() {
     const at::DeviceIndex device = this->device().index();
     const c10::cuda::CUDAStream current = c10::cuda::getCurrentCUDAStream(device);
@@ -705,15 +708,28 @@ struct OnceNode : torch::autograd::Node {
     cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
     if (cudaStreamIsCapturing(current.stream(), &status) != cudaSuccess || status == cudaStreamCaptureStatusNone)
       return;
-    for (size_t i = 0; i < num_outputs(); ++i) {
-      const auto &fn = next_edge(i).function;
-      if (fn == nullptr || !task_should_compute_output(i) ||
-          dynamic_cast<torch::autograd::AccumulateGrad *>(fn.get()) == nullptr)
-        continue;
-      const auto stream = fn->stream();
-      TORCH_CHECK(!stream.has_value() || stream->id() != 0, "dwconv_b200: ", name(),
-                  " is being captured into a CUDA graph, but an eager autograd graph of the same leaf is still alive "
-                  "on the default stream; release it before the capture");
+    const auto *info = torch::autograd::get_current_graph_task_exec_info();  // empty: every node runs
+    std::vector<torch::autograd::Node *> todo{this};
+    std::unordered_set<torch::autograd::Node *> seen;
+    while (!todo.empty()) {
+      const torch::autograd::Node *n = todo.back();
+      todo.pop_back();
+      for (const torch::autograd::Edge &edge : n->next_edges()) {
+        torch::autograd::Node *fn = edge.function.get();
+        if (fn == nullptr || !seen.insert(fn).second) continue;
+        if (info != nullptr && !info->empty()) {
+          const auto at = info->find(fn);
+          if (at == info->end() || !at->second.should_execute()) continue;
+        }
+        if (dynamic_cast<torch::autograd::AccumulateGrad *>(fn) == nullptr) {
+          todo.push_back(fn);
+          continue;
+        }
+        const auto stream = fn->stream();
+        TORCH_CHECK(!stream.has_value() || stream->id() != 0, "dwconv_b200: ", name(),
+                    " is being captured into a CUDA graph, but an eager autograd graph of the same leaf is still alive "
+                    "on the default stream; release it before the capture");
+      }
     }
   }
   variable_list apply(variable_list &&grads) override {

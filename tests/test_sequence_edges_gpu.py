@@ -391,3 +391,43 @@ def test_norm_weight_gradients_over_many_rows(size, dtype, monkeypatch):
         ref.check(a, want[name], tol[name], dtype, name)
     for a, c in zip(torch.autograd.grad(d.layer_norm(x, w, b), [w, b], dy), got[1:]):
         assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("op", ["conv", "recurrence", "norm"])
+def test_capture_beside_a_live_eager_graph_of_leaves_further_down(op):
+    """The leaf is behind a view and a conversion: a captured backward is refused there too, and runs once the eager
+    graph is gone.  A leaf that the backward is not asked for is no reason."""
+    import gc
+    import dwconv_b200 as d
+    if not d.sequence._nodes:
+        pytest.skip("the compiled nodes are not in use")
+    g = torch.Generator().manual_seed(72)
+    x, other = randn(g, 2, 20, 8), randn(g, 2, 20, 8)
+    w, decay = randn(g, 8, 1, 4, grad=False, dtype=torch.float16), torch.zeros(8, device="cuda")
+
+    def work():
+        a = (x.half() + other.half())[:, 1:]
+        if op == "conv":
+            return d.depthwise_conv1d_causal(a, w)
+        return d.gated_linear_recurrence(a, a, a, decay) if op == "recurrence" else d.layer_norm(a)
+
+    seeds = torch.ones(2, 19, 8, device="cuda", dtype=torch.float16)
+
+    def captured():
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            got, = torch.autograd.grad(work(), x, seeds)
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+    want, = torch.autograd.grad(work(), x, seeds)
+    alive = x * 2
+    with pytest.raises(RuntimeError, match="still alive on the default stream"):
+        captured()
+    del alive
+    gc.collect()
+    captured()
+    alive = other * 2
+    captured()
+    assert alive.requires_grad
