@@ -26,11 +26,15 @@ struct ConvArgs {
   int taps, act;
 };
 
-// Rows of a run: the choice whose rounds of resident CTAs (three per SM forward, two backward), each a run and
-// what it costs beside its rows, take least.  That cost is worth 5 rows forward (the filter, the K-1 rows
-// in front) and 12 backward (those on both sides, the sums at the end).  Measured on 4 x 4096 rows of 2560
-// channels in bf16, four taps, before rows were copied ahead, with runs of 16 / 32 / 48 / 64 / 128 rows:
-// forward 46 / 44 / 44 / 47 / 49 us, backward 134 / 107 / 99 / 105 / 118 us; the rule takes 48 for both.
+// Rows of a run: the choice whose rounds of resident CTAs (counted as three per SM forward, two backward), each a
+// run and what it costs beside its rows, take least.  That cost is worth 5 rows forward (the filter, the K-1 rows
+// in front) and 12 backward (those on both sides, the sums at the end).  Forward kernels of five taps and more
+// are bounded to two CTAs per SM, which the count does not know.  Measured with runs of 16 / 24 / 32 / 48 / 64 / 128
+// rows (microseconds, start included): 4 x 4096 rows of 2560 channels, bf16, four taps: forward 43 / 39 / 37 / 37 /
+// 39 / 43 (it takes 48), backward 125 / 102 / 92 / 82 / 82 / 82 (48); 8 x 8192 rows of 4096: 215 / 193 / 182 / 178 /
+// 172 / 176 (128), backward 707 / 557 / 475 / 410 / 373 / 332 (128); 2 x 8192 rows of 576, fp32, seven taps: 23 / 23 /
+// 27 / 25 / 25 / 31 (24), backward 68 / 59 / 51 / 51 / 41 / 47 (64); 4099 rows of 1001, fp16: 18 / 14 / 16 / 18 / 21 /
+// 33 (24), backward 31 / 35 / 25 / 29 / 33 / 47 (32).
 inline int conv_run(const dwconv_b200_sequence &s, int group, bool backward) {
   static const int runs[] = {8, 16, 24, 32, 48, 64, 96, 128};
   const long long slots = 148 * (backward ? 2 : 3), per_block = (long long)s.B * ceil_div(s.C, group);

@@ -34,9 +34,12 @@
 // The forward pass keeps the fp32 state that enters every 32nd row; the backward pass starts from it, so it
 // reads y nowhere and its h[t-1] have not been rounded to the data's type.
 //
-// Measured (bf16, 8 x 8192 rows of 4096 channels): forward 437 us, 4.9 TB/s; backward 900 us, 4.2 TB/s.  Both are
-// bound by the issue of instructions: 74 and 145 per warp and row, of which the special-function unit
-// takes 8 at a quarter of the rate.
+// Measured (bf16, 8 x 8192 rows of 4096 channels): forward 432 us, 5.0 TB/s; backward 893 us, 4.2 TB/s.  Neither
+// memory (76 % and 64 % of a copy's rate) nor the issue of instructions (58 % and 57 % of the slots, with 74 and 146
+// per warp and row) is full: what is left is the latency of a tile's steps, one after another, which 23 and 14
+// active warps per SM do not cover.  Where some channel of a CTA decays faster (scale softplus(decay) above REC_SERIES) the
+// exponential takes the series' place: 559 and 1049 us with decays from 0.3 to 0.999; 4 x 2048 rows of 2048: 43 and
+// 84 us, then 53 and 96.  Rows that the copy engine cannot address (2047 channels): 74 and 160.
 #include <atomic>
 #include <cmath>
 
@@ -110,8 +113,9 @@ __device__ __forceinline__ float2 beta_square2(float2 s) {
 }
 __device__ __forceinline__ float2 rsq2(float2 q) { return make_float2(rsqf(q.x), rsqf(q.y)); }
 
-// a = exp(s), good to a few units in its own last place; SERIES: no s of this CTA's channels is below
-// -REC_SERIES.
+// a = exp(s).  By the series good to a unit or two in its own last place; below -REC_SERIES, which SERIES rules out
+// for this CTA's channels, s log2(e) is rounded before the exponential, whose relative error grows by 6e-8 per
+// unit of |s| (absolutely it stays below 3e-8).
 template <bool SERIES> __device__ __forceinline__ float2 keep2(float2 s) {
   float2 a = add2(expm1_series2(s), f2(1.f));
   if constexpr (!SERIES) {
@@ -853,7 +857,7 @@ template <typename T, bool FAST> __device__ __forceinline__ Rate cta_rate(const 
 }
 
 // CTAs per SM that the registers are cut for.  (Eight warps with two CTAs per SM and 128 registers took 160 us
-// instead of 133 on 32768 fp32 rows of 1152 channels: clusters of 16 then leave SMs of a GPC unused.)
+// where three took 133 on 32768 fp32 rows of 1152 channels: clusters of 16 then leave SMs of a GPC unused.)
 constexpr int rec_forward_ctas(int W) { return W == 4 ? 8 : 3; }
 constexpr int REC_BACKWARD_CTAS = 4;
 
@@ -920,10 +924,13 @@ struct RecShape {
 
 // CTAs of a cluster along T, and the time that goes with it in microseconds, by a model: n CTAs of an SM take
 // (tile n) and (chain) per tile, the larger nearly alone; CTAs beyond those that fit follow them; a start
-// is worth two tiles.  Measured against all sizes: one packed list of 8191 rows of 2560 channels in bf16,
-// forward, clusters of 4 / 6 / 8 / 10 / 12 / 16: 114 / 87 / 83 / 73 / 99 / 91 us (it takes 10); 8 x 8192 rows of
-// 4096, backward, 1 / 2 / 4 / 8: 980 / 900 / 947 / 982 us (it takes 2).  Odd sizes and 14 leave SMs of a
-// GPC without work and are not in the choice.
+// is worth two tiles.  It is for choosing alone: its times are near for many channels (475 us and 432 measured) and
+// too short for few (packed list below: 50 and 76; 32771 fp32 rows of 1152: 98 and 135), since it knows neither
+// sequence borders nor the wider type nor the eight-warp packed kernel's spills (440 bytes loaded).  Measured
+// against all sizes: one packed list of 8191 rows of 2560 channels in bf16, forward, eight warps, clusters of
+// 4 / 6 / 8 / 10 / 12 / 16: 115 / 90 / 86 / 74 / 104 / 96 us (it takes 10); 8 x 8192 rows of 4096, backward, 1 / 2 / 4 / 8:
+// 971 / 893 / 944 / 985 us (it takes 2); 4 x 2048 rows of 2048, backward, 2 / 4 / 6 / 8 / 10: 92 / 82 / 86 / 84 / 94 (it
+// takes 8).  Odd sizes and 14 leave SMs of a GPC without work and are not in the choice.
 struct RecChoice {
   int cs;
   float us;
@@ -1044,8 +1051,8 @@ int launch_backward(const RecArgs &a, const RecMaps &maps, cudaStream_t st) {
 }
 
 // CTAs of four warps have the cheapest barriers and pack best; those of eight take twice the rows between two
-// exchanges, which counts where there are few of them.  8 x 8192 rows of 4096 channels in bf16: 437 us with
-// four, 441 with eight; one sequence of 32768 fp32 rows of 1152: 155 and 124.
+// exchanges, which counts where there are few of them.  8 x 8192 rows of 4096 channels in bf16: 432 us with
+// four, 447 with eight; one sequence of 32771 fp32 rows of 1152: 158 and 135; the packed list above: 92 and 74.
 template <typename T, bool FAST, bool PACKED> void forward_v(const RecArgs &a, const RecMaps &maps, cudaStream_t st) {
   const RecChoice four = rec_cluster(*a.s, forward_shape<T, 4, FAST, PACKED>());
   const RecChoice eight = rec_cluster(*a.s, forward_shape<T, 8, FAST, PACKED>());

@@ -3,7 +3,8 @@ and the layer norm, forward and backward, and the one-row steps that serve token
 
 They have no counterpart in the reference, whose maps are two-dimensional; names, argument checks,
 streams and errors follow ``depthwise_conv2d``.  Kernels: ``csrc/seq_*.cu`` through the C entry
-points of ``include/dwconv_b200.h``.  fp32, fp16 and bf16 tensors; arithmetic and state in fp32.
+points of ``include/dwconv_b200.h``.  fp32, fp16 and bf16 tensors; arithmetic and the recurrence's state in
+fp32 (the convolution's state holds input rows, in their type).
 
 Packed sequences: ``offsets`` is an int32 tensor of S + 1 ascending row numbers on the input's device
 (``offsets[0] == 0``); the input is [1, T, C] and sequence j is its rows ``offsets[j]`` to
@@ -12,8 +13,10 @@ sequence: zeros in every output, and what they hold is not looked at.  The list 
 a list that is not ascending gives unspecified values (never an access out of bounds).
 
 Every function runs on the current stream of the input's device, never synchronises, and may be
-captured into a CUDA graph.  Gradients are first-order and reverse-mode only.  A backward pass is not
-captured while an eager graph of the same leaves is alive on the default stream (refused).
+captured into a CUDA graph.  Gradients are first-order and reverse-mode only: with ``create_graph`` they carry
+an error for whoever differentiates them.  A backward pass is not to be captured while an eager graph of the same
+leaves is alive on the default stream: PyTorch's engine would break the capture, which can end the process.  The
+compiled module refuses it where its own nodes lead to such a leaf; without the module nothing notices.
 """
 import functools
 

@@ -400,9 +400,11 @@ DWCONV_B200_API int dwconv_b200_backward_filter_static(const void *x, const void
  * ([B, T, C]).  No counterpart in the reference, which has two-dimensional maps
  * only; they are the per-channel operators of models that mix tokens with a
  * short causal depthwise convolution and a gated linear recurrence, and the norm
- * in front of them.  f32 / f16 / bf16 data, all arithmetic and state in fp32 and
- * one rounding per stored value.  Results do not depend on timing: every sum has
- * one fixed order.
+ * in front of them.  f32 / f16 / bf16 data, all arithmetic and the recurrence's state
+ * in fp32 (the convolution's state holds input rows, in their type) and one rounding
+ * per stored value.  Sigmoids and the recurrence's exponentials of large arguments
+ * are good to about 2 + 1.2 |v| units of 2^-23, relative (the product with log2(e)
+ * is rounded).  Results do not depend on timing: every sum has one fixed order.
  *
  * Packed sequences: with `offsets` (device memory, S + 1 ascending row numbers,
  * offsets[0] = 0) B is 1 and sequence j is rows offsets[j] .. offsets[j+1]-1 of
